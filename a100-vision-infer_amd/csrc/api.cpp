@@ -14,6 +14,8 @@
 
 #include "../../include/fp8lin.h"
 #include "internal.hpp"
+#include "paged.hpp"
+#include "verify.hpp"
 
 namespace {
 
@@ -496,6 +498,50 @@ void linear_candidates_impl(const uint16_t* x, const uint8_t* codes, const float
     linear_impl(x, codes, scales, S, logits, N, M, N, K, stream);
     check_hip(fp8lin::launch_vocab_candidates(logits, (int)M, (int)N, offset, part, out, stream),
               "vocabulary candidates launch");
+}
+
+// ---- serving over a paged cache ----
+
+int page_bits(int64_t page_size) {
+    int bits = 0;
+    while (((int64_t)1 << bits) < page_size && bits < 40) ++bits;
+    return bits;
+}
+
+void check_pages(int64_t width, int64_t page_size) {
+    require(page_size >= fp8lin::kPagedMinPage && page_size <= ((int64_t)1 << 20) && (page_size & (page_size - 1)) == 0,
+            FP8LIN_ERR_SHAPE, "paged cache: page_size must be a power of two, 16 or more");
+    require(width > 0 && width <= ((int64_t)1 << 30) / page_size, FP8LIN_ERR_SHAPE,
+            "paged cache: need 0 < width and width * page_size <= 2^30");
+}
+
+void check_requests(int64_t requests, int64_t rows) {
+    require(requests > 0 && requests <= FP8LIN_PAGED_MAX_REQUESTS, FP8LIN_ERR_SHAPE, "paged cache: 1 to 8192 requests");
+    require(rows >= 0 && rows < kMaxDim, FP8LIN_ERR_SHAPE, "paged cache: invalid number of rows");
+}
+
+void check_cache(const fp8lin_paged_cache* c, fp8lin::PagedCache& k, fp8lin::PagedCache& v) {
+    require(c != nullptr && c->k && c->v, FP8LIN_ERR_ARGUMENT, "paged cache: null pointer");
+    check_pages(1, c->page_size);
+    require(c->pages > 0 && c->pages < kMaxDim && c->kv_heads > 0 && c->kv_heads < kMaxDim && c->head_dim > 0 &&
+                c->head_dim <= 4096,
+            FP8LIN_ERR_SHAPE, "paged cache: invalid dimensions");
+    const int64_t unit = c->fp8 ? 16 : 8, rows = 16 * (c->fp8 ? 1 : 2);
+    auto good = [&](const void* p, int64_t page, int64_t slot, int64_t head) {
+        return aligned16(p) && page % unit == 0 && slot % unit == 0 && head % unit == 0 && page >= 0 && head >= 0 &&
+               slot >= c->head_dim && slot < ((int64_t)1 << 30) / rows;
+    };
+    require(good(c->k, c->k_page, c->k_slot, c->k_head) && good(c->v, c->v_page, c->v_slot, c->v_head), FP8LIN_ERR_ARGUMENT,
+            "paged cache: data and strides must be multiples of 16 bytes, a slot at least head_dim elements");
+    require(c->fp8 ? c->k_scale && c->v_scale : !c->k_scale && !c->v_scale, FP8LIN_ERR_ARGUMENT,
+            "paged cache: an 8-bit cache needs k_scale and v_scale, a BF16 cache has none");
+    k = fp8lin::PagedCache{c->k, c->k_page, c->k_slot, c->k_head};
+    v = fp8lin::PagedCache{c->v, c->v_page, c->v_slot, c->v_head};
+}
+
+// Rows of a request per kv head.
+int64_t paged_rows(int64_t heads, int64_t kv_heads, int64_t max_count) {
+    return heads / kv_heads * std::min<int64_t>(std::max<int64_t>(max_count, 1), kMaxDim);
 }
 
 }  // namespace
@@ -1000,6 +1046,136 @@ int fp8lin_decode_chain(const fp8lin_chain_link* links, int nlinks, void* worksp
         ensure_device();
         check_hip(fp8lin::launch_chain(dev, nlinks, static_cast<uint64_t*>(workspace), as_stream(stream)),
                   "decode chain launch");
+    });
+}
+
+size_t fp8lin_paged_layout_workspace_bytes(int64_t requests) {
+    return requests > 0 && requests <= FP8LIN_PAGED_MAX_REQUESTS ? fp8lin::paged_layout_ws_bytes(requests) : 0;
+}
+
+int fp8lin_paged_layout(const int32_t* lengths, const int32_t* counts, const int32_t* table, int64_t table_ld,
+                        const int32_t* free_pages, int64_t free_count, const int32_t* cursor, int64_t requests,
+                        int64_t width, int64_t page_size, int64_t tokens, int32_t* offsets, int32_t* new_lengths,
+                        int64_t* slots, int64_t* positions, int32_t* new_table, int64_t new_table_ld,
+                        int32_t* new_cursor, void* workspace, size_t workspace_bytes, fp8lin_stream_t stream) {
+    return guarded([&] {
+        require(lengths && counts && table && offsets && new_lengths && new_table && new_cursor &&
+                    (tokens == 0 || (slots && positions)) && (free_count == 0 || free_pages),
+                FP8LIN_ERR_ARGUMENT, "paged layout: null pointer");
+        check_requests(requests, tokens);
+        check_pages(width, page_size);
+        require(free_count >= 0 && free_count < kMaxDim && table_ld >= width && new_table_ld >= width, FP8LIN_ERR_SHAPE,
+                "paged layout: invalid table strides or free list");
+        require(new_table != table || new_table_ld == table_ld, FP8LIN_ERR_ARGUMENT,
+                "paged layout: a table written in place keeps its stride");
+        check_workspace(workspace, workspace_bytes, fp8lin::paged_layout_ws_bytes(requests), "paged layout: workspace too small");
+        ensure_device();
+        check_hip(fp8lin::launch_paged_layout(lengths, counts, table, table_ld, free_pages, free_count, cursor, (int)requests,
+                                              (int)width, page_bits(page_size), tokens, offsets, new_lengths, slots, positions,
+                                              new_table, new_table_ld, new_cursor, static_cast<int32_t*>(workspace),
+                                              as_stream(stream)),
+                  "paged layout launch");
+    });
+}
+
+int fp8lin_paged_append(const fp8lin_paged_cache* cache, const uint16_t* k, int64_t k_token, int64_t k_head,
+                        const uint16_t* v, int64_t v_token, int64_t v_head, const int64_t* slots, int64_t tokens,
+                        fp8lin_stream_t stream) {
+    return guarded([&] {
+        fp8lin::PagedCache kc, vc;
+        check_cache(cache, kc, vc);
+        require(tokens >= 0 && tokens < kMaxDim, FP8LIN_ERR_SHAPE, "paged append: invalid number of tokens");
+        if (tokens == 0) return;
+        require(k && v && slots, FP8LIN_ERR_ARGUMENT, "paged append: null pointer");
+        require(cache->head_dim % (cache->fp8 ? 16 : 8) == 0, FP8LIN_ERR_UNSUPPORTED,
+                "paged append: head_dim must be a multiple of 8 (16 in an 8-bit cache)");
+        require(tokens * (cache->kv_heads * cache->head_dim / 8) < ((int64_t)1 << 38), FP8LIN_ERR_SHAPE,
+                "paged append: too many values");
+        ensure_device();
+        check_hip(fp8lin::launch_paged_append(k, v, k_token, k_head, v_token, v_head, slots, kc, vc, cache->fp8 != 0,
+                                              cache->k_scale, cache->v_scale, tokens, (int)cache->kv_heads,
+                                              (int)cache->head_dim, page_bits(cache->page_size), cache->pages,
+                                              as_stream(stream)),
+                  "paged append launch");
+    });
+}
+
+size_t fp8lin_paged_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_count) {
+    if (heads <= 0 || heads >= kMaxDim || kv_heads <= 0 || heads % kv_heads || head_dim <= 0 || head_dim > 256) return 0;
+    return fp8lin::paged_attention_ws_bytes((int)head_dim, paged_rows(heads, kv_heads, max_count));
+}
+
+int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, int64_t q_token, int64_t q_head,
+                           const uint16_t* gate, int64_t gate_token, int64_t gate_head, const int32_t* table,
+                           int64_t table_ld, int64_t width, const int32_t* offsets, const int32_t* lengths,
+                           int64_t requests, int64_t tokens, int64_t heads, int64_t max_count, int causal, double scale,
+                           uint16_t* out, int64_t out_token, int64_t out_head, void* workspace, size_t workspace_bytes,
+                           fp8lin_stream_t stream) {
+    return guarded([&] {
+        fp8lin::PagedAttention a{};
+        check_cache(cache, a.k, a.v);
+        check_requests(requests, tokens);
+        require(heads > 0 && heads % cache->kv_heads == 0 && heads < kMaxDim && tokens * heads < kMaxDim - 1024,
+                FP8LIN_ERR_SHAPE, "paged attention: heads must be a multiple of kv_heads, tokens * heads below 2^31");
+        require(cache->head_dim == 64 || cache->head_dim == 128 || cache->head_dim == 256, FP8LIN_ERR_UNSUPPORTED,
+                "paged attention: head_dim must be 64, 128 or 256");
+        check_pages(width, cache->page_size);
+        require(table_ld >= width, FP8LIN_ERR_SHAPE, "paged attention: invalid table stride");
+        const double scale2 = scale * 1.4426950408889634;
+        require(scale > 0.0 && std::isfinite((float)scale2) && (float)scale2 > 0.0f, FP8LIN_ERR_ARGUMENT,
+                "paged attention: scale must be positive");
+        if (tokens == 0) return;
+        require(q && table && offsets && lengths && out, FP8LIN_ERR_ARGUMENT, "paged attention: null pointer");
+        const int64_t rows = paged_rows(heads, cache->kv_heads, max_count);
+        check_workspace(workspace, workspace_bytes, fp8lin::paged_attention_ws_bytes((int)cache->head_dim, rows),
+                        "paged attention: workspace too small");
+        ensure_device();
+        auto on = [](const void* p, int64_t s0, int64_t s1, int64_t elements) {
+            return reinterpret_cast<uintptr_t>(p) % (2 * elements) == 0 && s0 % elements == 0 && s1 % elements == 0;
+        };
+        a.q = q, a.gate = gate, a.out = out;
+        a.q_tok = q_token, a.q_head = q_head, a.g_tok = gate_token, a.g_head = gate_head;
+        a.o_tok = out_token, a.o_head = out_head;
+        a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
+        a.table = table, a.offsets = offsets, a.lengths = lengths, a.ldt = table_ld;
+        a.width = (int)width, a.page_bits = page_bits(cache->page_size), a.pages = (int)cache->pages;
+        a.B = (int)requests, a.T = (int)tokens, a.H = (int)heads, a.HK = (int)cache->kv_heads;
+        a.G = a.H / a.HK;
+        a.causal = causal != 0;
+        a.q_vec = on(q, q_token, q_head, 8), a.g_vec = on(gate, gate_token, gate_head, 4);
+        a.o_vec = on(out, out_token, out_head, 4);
+        a.scale2 = (float)scale2;
+        a.ws = static_cast<float*>(workspace);
+        check_hip(fp8lin::launch_paged_attention(a, (int)cache->head_dim, cache->fp8 != 0, rows, as_stream(stream)),
+                  "paged attention launch");
+    });
+}
+
+size_t fp8lin_verify_drafts_workspace_bytes(int64_t requests, int64_t rows, int64_t vocab) {
+    if (requests <= 0 || requests > FP8LIN_PAGED_MAX_REQUESTS || rows < 0 || rows >= kMaxDim || vocab <= 0 || vocab >= kMaxDim)
+        return 0;
+    return fp8lin::verify_ws_bytes(rows, requests, vocab);
+}
+
+int fp8lin_verify_drafts(const void* logits, int logits_f32, int64_t logits_ld, const float* draft_probs,
+                         int64_t draft_ld, int64_t prob_rows, const int64_t* tokens, const float* uniforms,
+                         const int32_t* offsets, const float* temperature, int64_t requests, int64_t rows, int64_t vocab,
+                         int32_t* accepted, int64_t* out, void* workspace, size_t workspace_bytes,
+                         fp8lin_stream_t stream) {
+    return guarded([&] {
+        check_requests(requests, rows);
+        require(vocab > 0 && vocab < kMaxDim - 65536 && logits_ld >= vocab && (!draft_probs || draft_ld >= vocab) &&
+                    prob_rows >= 0,
+                FP8LIN_ERR_SHAPE, "verify drafts: invalid vocabulary or row strides");
+        require(offsets && accepted && (rows == 0 || (logits && tokens && uniforms && out)), FP8LIN_ERR_ARGUMENT,
+                "verify drafts: null pointer");
+        check_workspace(workspace, workspace_bytes, fp8lin::verify_ws_bytes(rows, requests, vocab),
+                        "verify drafts: workspace too small");
+        ensure_device();
+        check_hip(fp8lin::launch_verify(logits, logits_f32 == 0, logits_ld, draft_probs, draft_ld, prob_rows, tokens, uniforms,
+                                        offsets, temperature, rows, (int)requests, (int)vocab, accepted, out, workspace,
+                                        as_stream(stream)),
+                  "verify drafts launch");
     });
 }
 

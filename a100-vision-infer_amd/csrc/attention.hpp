@@ -1,0 +1,195 @@
+// Attention of new tokens over a paged cache: what the two kernels of
+// attention_few.hip and attention_tile.hip share.
+//
+// For row i of a request (a new token at position p_i, one query head),
+//   o_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = 2^(c q_i.k_j - m_i),
+// over the keys j <= p_i (all keys when not causal), c = scale * log2(e).
+// One pass over the keys keeps a running m_i, the sum of weights and the
+// weighted sum of values in FP32; two parts (m, l, O) of a row are joined as
+// (M, l 2^(m-M) + l' 2^(m'-M), O 2^(m-M) + O' 2^(m'-M)), M = max(m, m').
+// The weights are rounded to BF16 for the product with V, as the matrix
+// cores take it (half a step of 2^-8 each, averaged over the keys); the sum
+// of weights adds them unrounded.
+//
+// m_i only moves when a score passes it by more than 2^8: any m_i gives the
+// same o_i, and weights up to 2^8 lose nothing in FP32 or BF16, so most key
+// tiles need no rescaling of O and no maximum across lanes.
+#pragma once
+#include "device.hpp"
+#include "gemm_fp8.hpp"
+#include "paged.hpp"
+
+namespace fp8lin {
+namespace attn {
+
+using gemm_fp8::i32x4;
+using gemm_fp8::make_desc;
+using gemm_fp8::wait_lgkm;
+using gemm_fp8::wait_vm;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLazy = 8.0f;  // log2 of the largest weight before m moves
+constexpr int kGroups = 256;   // workgroups of a launch at one per CU
+
+// 64 lanes x 16 B from global (voff, bounds-checked) into LDS [m0v, m0v + 1024).
+// K and V rows that one workgroup reads take the non-temporal policy.
+template <bool NT>
+__device__ __forceinline__ void dma(uint32_t m0v, uint32_t voff, i32x4 desc) {
+    if constexpr (NT)
+        gemm_fp8::dma16_nt(m0v, voff, desc, 0);
+    else
+        gemm_fp8::dma16(m0v, voff, desc, 0);
+}
+
+// Four values of a 16-bit matrix in LDS, read across rows: the 16 lanes of a
+// group give the addresses of 4 rows x 16 columns (lane i: row i / 4, columns
+// 4 (i % 4) ..), and lane i receives column i of the 4 rows.
+__device__ __forceinline__ s16x4 read_tr16(uint32_t addr) {
+    typedef __attribute__((address_space(3))) s16x4 lds_t;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(uintptr_t)addr);
+}
+// The same of an 8-bit matrix: 8 rows x 16 columns (lane i: row i / 2, columns
+// 8 (i % 2) ..), lane i receives column i of the 8 rows.
+__device__ __forceinline__ i32x2 read_tr8(uint32_t addr) {
+    typedef __attribute__((address_space(3))) i32x2 lds_t;
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_t*)(uintptr_t)addr);
+}
+__device__ __forceinline__ u32x4 read16(uint32_t addr) {
+    typedef __attribute__((address_space(3))) u32x4 lds_t;
+    return *(lds_t*)(uintptr_t)addr;
+}
+
+// Two E4M3FN codes to BF16, exactly (every code has 4 significant bits).
+template <bool HI>
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+}
+__device__ __forceinline__ bf16x8 codes8_bf16(uint32_t lo, uint32_t hi) {
+    return __builtin_bit_cast(bf16x8, u32x4{codes_bf16<false>(lo), codes_bf16<true>(lo), codes_bf16<false>(hi),
+                                            codes_bf16<true>(hi)});
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 8 query values of a row from element d (16 bytes when the rows start on
+// them), zeros for a row past the tile.
+__device__ __forceinline__ u32x4 load_q8(const PagedAttention& a, const uint16_t* row, bool valid, int d) {
+    if (!valid) return u32x4{0, 0, 0, 0};
+    if (a.q_vec) return load_u32x4(row + d);
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (uint32_t)row[d + 2 * i] | (uint32_t)row[d + 2 * i + 1] << 16;
+    return v;
+}
+
+// out[d .. d+3] = bf16(o * sigmoid(gate)): one rounding.
+__device__ __forceinline__ void store4(const PagedAttention& a, int64_t tok, int head, int d, f32x4 o) {
+    if (a.gate) {
+        const uint16_t* g = a.gate + tok * a.g_tok + head * a.g_head + d;
+        u32x2 gv;
+        if (a.g_vec) {
+            gv = *reinterpret_cast<const u32x2*>(g);
+        } else {
+            gv.x = (uint32_t)g[0] | (uint32_t)g[1] << 16;
+            gv.y = (uint32_t)g[2] | (uint32_t)g[3] << 16;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = bf16_bits_to_f32(((i < 2 ? gv.x : gv.y) >> (16 * (i & 1))) & 0xffffu);
+            o[i] /= 1.0f + expf(-x);
+        }
+    }
+    uint16_t* y = a.out + tok * a.o_tok + head * a.o_head + d;
+    const uint32_t lo = pack_bf16x2(f32x2{o.x, o.y}), hi = pack_bf16x2(f32x2{o.z, o.w});
+    if (a.o_vec) {
+        *reinterpret_cast<u32x2*>(y) = u32x2{lo, hi};
+    } else {
+        y[0] = (uint16_t)lo;
+        y[1] = (uint16_t)(lo >> 16);
+        y[2] = (uint16_t)hi;
+        y[3] = (uint16_t)(hi >> 16);
+    }
+}
+
+// Partial sums of a split unit's piece in the workspace: O (BM x D floats, the
+// kernel's own order), then m and l of the BM rows.  A workgroup leaves at
+// most two: slot 0 for the piece that begins inside a unit (its first), slot 1
+// for the one that begins a unit (its last).
+template <int BM, int D>
+struct Partial {
+    static constexpr int64_t kFloats = (int64_t)BM * D + 2 * BM;
+    static __device__ __forceinline__ float* at(float* ws, int group, int slot) {
+        return ws + (2 * group + slot) * kFloats;
+    }
+};
+
+hipError_t launch_few(const PagedAttention& a, int D, bool fp8, int rows, hipStream_t stream);
+hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t stream);
+
+// Joins the pieces of the units that the boundaries between workgroups cut.
+// Workgroup (w, y): boundary w + 1, the y-th part of the unit's rows; only the
+// first boundary inside a unit has work.  Each thread joins 4 values of one
+// row, reading the pieces in order.  ROW(e, row, d): row and first dimension
+// of the e-th 4 floats of a piece's O.
+template <int BM, int BN, int D, class Order>
+__global__ __launch_bounds__(256) void join_kernel(PagedAttention a, int groups, int min_tiles) {
+    extern __shared__ __align__(16) int64_t pre[];
+    using Split = PagedSplit<BM, BN>;
+    Split::prefix(a, pre, 256);
+    const int64_t total = pre[a.B], chunk = Split::chunk(a, total, groups, min_tiles);
+    const int w = blockIdx.x + 1;
+    const int64_t p = w * chunk;
+    if (p >= total) return;
+    const auto u = Split::locate(a, pre, p);
+    if (u.kt == 0) return;
+    if (w > 1) {
+        const auto v = Split::locate(a, pre, p - chunk);
+        if (v.b == u.b && v.hk == u.hk && v.r == u.r && v.kt > 0) return;
+    }
+    const PagedSeq s = paged_seq(a, u.b);
+    const int r0 = u.r * BM, nr = (int)min((int64_t)BM, (int64_t)s.n * a.G - r0);
+    const int e = blockIdx.y * 256 + threadIdx.x;
+    int row, d;
+    Order::place(e, row, d);
+    const float vs = a.v_scale ? a.v_scale[u.hk] : 1.0f;
+    // piece i: [kt_i, kt_{i+1}), by workgroup w - 1 + i
+    float M = -__builtin_inff(), l = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    int kt = 0, slot = 1;
+    for (int g = w - 1;; ++g) {
+        const int64_t pn = (g + 1) * chunk;
+        bool more = false;
+        int next = 0;
+        if (pn < total) {
+            const auto v = Split::locate(a, pre, pn);
+            more = v.b == u.b && v.hk == u.hk && v.r == u.r;
+            next = v.kt;
+        }
+        if (!more || next > kt) {
+            const float* part = Partial<BM, D>::at(a.ws, g, slot);
+            const float m1 = part[(int64_t)BM * D + row], l1 = part[(int64_t)BM * D + BM + row];
+            const f32x4 o1 = *reinterpret_cast<const f32x4*>(part + 4 * (int64_t)e);
+            const float mn = fmaxf(M, m1);
+            const float f0 = M == -__builtin_inff() ? 0.0f : exp2_fast(M - mn);
+            const float f1 = m1 == -__builtin_inff() ? 0.0f : exp2_fast(m1 - mn);
+            l = l * f0 + l1 * f1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = (f0 == 0.0f ? 0.0f : o[i] * f0) + (f1 == 0.0f ? 0.0f : o1[i] * f1);
+            M = mn;
+            kt = next;
+            slot = 0;
+        }
+        if (!more) break;
+    }
+    if (row >= nr) return;
+    const float inv = l == 0.0f ? 0.0f : vs / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : o[i] * inv;
+    const int flat = r0 + row;
+    store4(a, s.off + flat / a.G, u.hk * a.G + flat % a.G, d, o);
+}
+
+}  // namespace attn
+}  // namespace fp8lin

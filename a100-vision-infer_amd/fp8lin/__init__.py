@@ -13,5 +13,6 @@ from .ops import (add_bias, decode_chain, decode_chain_workspace, fp8_decode, fp
                   gemm_bf16, gen_activations, gen_normal, gen_weights, linear_candidates,
                   linear_swiglu, merge_candidates, mfma_ceiling, qk_norm_rope, reduce_residual_rms, residual_rms,
                   small_linear_shared, stream_read, tilelang_fp8_small, vocabulary_candidates)
+from .paged import PagedLayout, paged_append, paged_attention, paged_layout, verify_drafts  # noqa: F401
 from .engine import LinearEngine, StoredWeight  # noqa: F401
 from .artifact import load_linear_engine, read_manifest, read_tensor  # noqa: F401

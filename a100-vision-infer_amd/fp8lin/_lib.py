@@ -46,6 +46,9 @@ EXPORTED = [
     "fp8lin_linear_workspace_bytes", "fp8lin_linear_ws",
     "fp8lin_linear_scaled_workspace_bytes", "fp8lin_linear_swiglu_scaled_workspace_bytes", "fp8lin_gemm_plan",
     "fp8lin_decode_chain_workspace_bytes", "fp8lin_decode_chain",
+    "fp8lin_paged_layout_workspace_bytes", "fp8lin_paged_layout", "fp8lin_paged_append",
+    "fp8lin_paged_attention_workspace_bytes", "fp8lin_paged_attention",
+    "fp8lin_verify_drafts_workspace_bytes", "fp8lin_verify_drafts",
 ]
 
 
@@ -70,6 +73,19 @@ class ChainLink(ctypes.Structure):
 
 
 CHAIN_MAX_LINKS = 8
+
+
+class PagedCacheRecord(ctypes.Structure):
+    """struct fp8lin_paged_cache"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_page", ctypes.c_int64), ("k_slot", ctypes.c_int64), ("k_head", ctypes.c_int64),
+                ("v_page", ctypes.c_int64), ("v_slot", ctypes.c_int64), ("v_head", ctypes.c_int64),
+                ("pages", ctypes.c_int64), ("page_size", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("head_dim", ctypes.c_int64), ("fp8", ctypes.c_int), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p)]
+
+
+PAGED_MAX_REQUESTS = 8192
 
 
 class LinearOptions(ctypes.Structure):
@@ -154,6 +170,15 @@ def lib():
                                                                  ctypes.POINTER(Weight), i64]),
         "fp8lin_engine_linear_candidates": (i32, [ctypes.POINTER(LinearOptions), ctypes.POINTER(Weight), vp,
                                                   i64, i64, vp, vp, sz, ctypes.POINTER(ctypes.c_int), vp]),
+        "fp8lin_paged_layout_workspace_bytes": (sz, [i64]),
+        "fp8lin_paged_layout": (i32, [vp, vp, vp, i64, vp, i64, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, i64, vp, vp,
+                                      sz, vp]),
+        "fp8lin_paged_append": (i32, [ctypes.POINTER(PagedCacheRecord), vp, i64, i64, vp, i64, i64, vp, i64, vp]),
+        "fp8lin_paged_attention_workspace_bytes": (sz, [i64, i64, i64, i64]),
+        "fp8lin_paged_attention": (i32, [ctypes.POINTER(PagedCacheRecord), vp, i64, i64, vp, i64, i64, vp, i64, i64, vp,
+                                         vp, i64, i64, i64, i64, i32, ctypes.c_double, vp, i64, i64, vp, sz, vp]),
+        "fp8lin_verify_drafts_workspace_bytes": (sz, [i64, i64, i64]),
+        "fp8lin_verify_drafts": (i32, [vp, i32, i64, vp, i64, i64, vp, vp, vp, vp, i64, i64, i64, vp, vp, vp, sz, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -17,6 +17,7 @@ import torch
 
 from ._lib import (ERR_ARGUMENT, PATH_FP8_GEMM, PATH_FP8_GEMV, PATH_TENSOR_SMALL, Fp8linError, LinearOptions, Weight, check, lib)
 from .ops import fp8_decode, fused_swiglu, qk_norm_rope
+from .paged import paged_append, paged_attention
 
 
 def check_options(options):
@@ -204,6 +205,32 @@ class LinearEngine:
         q, k = qk_norm_rope(projected, q_norm, k_norm, positions, heads, kv_heads, head_dim, rotary,
                             rope["rope_theta"], sections[1], sections[2], eps)
         return q, gate, k, v
+
+    def full_attention(self, x, prefix, layout, k_cache, v_cache, q_norm, k_norm, heads, kv_heads, head_dim, rope, eps,
+                       max_count=None, positions=None, k_scale=None, v_scale=None):
+        """`Engine::full_attention` (src/engine.cpp:275-331) on one rank for a
+        step of many requests over a paged cache: the QKV-gate projection of x
+        [tokens, hidden], its Q/K epilogue, the new keys and values into their
+        slots, attention over the requests' pages with the output gate, and
+        linear(o_proj); the cross-rank reduce is the caller's.  layout: the
+        step's PagedLayout (paged_layout).  positions int64 [3, tokens]: the
+        mRoPE positions (default: layout.positions on every axis).  The gate
+        and the values are read where the projection wrote them."""
+        projected = self.linear(x, prefix + ".qkv_gate")
+        T, H, HK, D = projected.size(0), heads, kv_heads, head_dim
+        if projected.size(-1) != 2 * (H + HK) * D:
+            raise Fp8linError(ERR_ARGUMENT, "QKV-gate output width does not match the head layout")
+        if positions is None:
+            positions = layout.positions.expand(3, T)
+        rotary, sections = int(D * rope.get("partial_rotary_factor", 0.25)), rope["mrope_section"]
+        q, k = qk_norm_rope(projected, q_norm, k_norm, positions, H, HK, D, rotary, rope["rope_theta"], sections[1],
+                            sections[2], eps)
+        gate = projected[:, :2 * H * D].view(T, H, 2 * D)[..., D:]
+        v = projected[:, (2 * H + HK) * D:].view(T, HK, D)
+        paged_append(k, v, layout.slots, k_cache, v_cache, k_scale=k_scale, v_scale=v_scale)
+        core = paged_attention(q, k_cache, v_cache, layout.block_table, layout.offsets, layout.lengths, max_count=max_count,
+                               gate=gate, k_scale=k_scale, v_scale=v_scale)
+        return self.linear(core.view(T, H * D), prefix + ".o_proj")
 
     # -- steps -----------------------------------------------------------------
     @contextlib.contextmanager

@@ -522,6 +522,122 @@ int fp8lin_decode_chain(const fp8lin_chain_link* links, int nlinks, void* worksp
                         fp8lin_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Serving over a paged cache: what stands between the Q/K epilogue of the
+ * QKV-gate projection (fp8lin_qk_norm_rope) and the output projection, for a
+ * step of many requests, and between the output head and the next step.
+ * Counterparts in the reference, over one contiguous cache of one request:
+ * append_kv / append_chunk (src/optimized.cu:81,173), attention_parts /
+ * attention_merge (src/optimized.cu:82-94,177), GreedyVerification
+ * (include/avi/speculative.h:10-26).
+ *
+ * A cache holds pages of page_size tokens (a power of two, 16 or more).
+ * Request b's token at position p lies in page table[b][p / page_size], slot
+ * p % page_size; its slot number is page * page_size + p % page_size.  The
+ * strides are in elements; a token's head_dim elements are contiguous, and
+ * data and strides are multiples of 16 bytes.  fp8: E4M3FN codes that stand
+ * for code * k_scale[head] (v_scale[head]), positive floats on the device;
+ * else BF16 and null scales.
+ */
+typedef struct fp8lin_paged_cache {
+    void* k;
+    void* v;
+    int64_t k_page, k_slot, k_head;
+    int64_t v_page, v_slot, v_head;
+    int64_t pages, page_size, kv_heads, head_dim;
+    int fp8;
+    const float* k_scale;
+    const float* v_scale;
+} fp8lin_paged_cache;
+
+/* The layout of a step, from lengths on the device: request b holds
+ * lengths[b] tokens and gets counts[b] more (negative numbers count as 0).
+ * Entries of its table row [requests, width] for those tokens that hold no
+ * page (< 0) get the next pages of free_pages, from index cursor[0] (null: 0),
+ * in the order of the requests and their entries; an entry past the list stays
+ * -1.  Writes
+ *   offsets [requests + 1]  first row of each request's new tokens, and the end;
+ *   new_lengths [requests]  lengths + counts;
+ *   slots, positions [tokens]  of the new tokens; slot -1 where there is no
+ *       page (none left, a negative id, a position past the table); rows from
+ *       offsets[requests] on: slot -1, position 0; rows past `tokens` are dropped;
+ *   new_table [requests, width]  the table with the pages taken, which may be
+ *       `table` itself (and may overlap no other argument);
+ *   new_cursor [1]  cursor + pages wanted: above free_count, the list was short.
+ * Page ids are not checked here; fp8lin_paged_append and
+ * fp8lin_paged_attention check them.  0 < requests <= 8192; width * page_size
+ * <= 2^30.
+ */
+#define FP8LIN_PAGED_MAX_REQUESTS 8192
+size_t fp8lin_paged_layout_workspace_bytes(int64_t requests);
+int fp8lin_paged_layout(const int32_t* lengths, const int32_t* counts, const int32_t* table, int64_t table_ld,
+                        const int32_t* free_pages, int64_t free_count, const int32_t* cursor, int64_t requests,
+                        int64_t width, int64_t page_size, int64_t tokens, int32_t* offsets, int32_t* new_lengths,
+                        int64_t* slots, int64_t* positions, int32_t* new_table, int64_t new_table_ld,
+                        int32_t* new_cursor, void* workspace, size_t workspace_bytes, fp8lin_stream_t stream);
+
+/* Keys and values [tokens, kv_heads, head_dim] (BF16, strides in elements, the
+ * last dimension contiguous) into their slots: BF16 as they are, 8-bit as
+ * E4M3FN(x / scale), to nearest even, above 448 as 448, NaN as NaN.  A row
+ * whose slot is outside [0, pages * page_size) is skipped.  Two rows of one
+ * slot: it is not defined which of them each 8 values come from.  head_dim % 8
+ * == 0 (16 in an 8-bit cache).
+ */
+int fp8lin_paged_append(const fp8lin_paged_cache* cache, const uint16_t* k, int64_t k_token, int64_t k_head,
+                        const uint16_t* v, int64_t v_token, int64_t v_head, const int64_t* slots, int64_t tokens,
+                        fp8lin_stream_t stream);
+
+/* Attention of new tokens over the cache, which holds them already.  Request b
+ * has rows offsets[b] .. offsets[b+1] of q [tokens, heads, head_dim] (the last
+ * of its lengths[b] tokens) and reads kv head h / (heads / kv_heads):
+ *   out = softmax(scale q K^T) V * sigmoid(gate)
+ * over the keys up to each row's own token (causal), or all lengths[b] keys.
+ * gate [tokens, heads, head_dim] may be null.  FP32 sums, one rounding of the
+ * result; the weights are rounded to BF16 for the product with V.  A row
+ * without keys (or whose every score is -inf) gives 0; a page id outside
+ * [0, pages) reads as keys and values of 0; lengths are cut to the table's
+ * width; rows from offsets[requests] on are left as they are.
+ * max_count: the most rows that a request is expected to have; more give the
+ * same results, slower.  head_dim 64, 128 or 256; scale > 0; 0 < requests <=
+ * 8192; width * page_size <= 2^30; tokens * heads < 2^31.  out may not overlap
+ * the inputs.  A call's result does not depend on timing, but a row's does on
+ * the lengths of the whole batch (FP32 summation order).
+ * Workspace: the bytes below, 16-byte aligned, any content.
+ */
+size_t fp8lin_paged_attention_workspace_bytes(int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_count);
+int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, int64_t q_token, int64_t q_head,
+                           const uint16_t* gate, int64_t gate_token, int64_t gate_head, const int32_t* table,
+                           int64_t table_ld, int64_t width, const int32_t* offsets, const int32_t* lengths,
+                           int64_t requests, int64_t tokens, int64_t heads, int64_t max_count, int causal, double scale,
+                           uint16_t* out, int64_t out_token, int64_t out_head, void* workspace, size_t workspace_bytes,
+                           fp8lin_stream_t stream);
+
+/* Verification of drafted tokens.  Request b has rows offsets[b] ..
+ * offsets[b+1] of logits [rows, vocab] (BF16, or FP32 with logits_f32): the
+ * target's after its last token and after each draft; tokens [rows] are the
+ * tokens that were fed in, so draft i of the request is tokens[offsets[b] + i].
+ * With p = softmax(logits / temperature[b]) (null: 1; 0: the most likely token,
+ * lowest index of equal ones) and q the draft model's distribution,
+ * draft_probs [prob_rows, vocab] (FP32; the rows of all requests but each one's
+ * last, in order; null: drafts taken without probabilities, q = 1 at the
+ * draft), draft i = 1.. is kept while uniforms[row i - 1] * q < p.  The next
+ * token is drawn with the request's last number, from max(p - q, 0) of the
+ * first row that refused its draft (from p if nothing is left of that), else
+ * from p of the last row: the first index whose running sum of weights exceeds
+ * the number times their sum.
+ *   accepted [requests]: drafts kept; out [rows]: the kept drafts, the next
+ *   token, then -1 (as in rows behind the last request).
+ * A row without a distribution (NaN, +inf, all -inf) keeps no draft and draws
+ * -1; a draft outside [0, vocab) is refused.  64-bit sums.  0 < requests <=
+ * 8192; vocab < 2^31.  Workspace: the bytes below, 16-byte aligned, any content.
+ */
+size_t fp8lin_verify_drafts_workspace_bytes(int64_t requests, int64_t rows, int64_t vocab);
+int fp8lin_verify_drafts(const void* logits, int logits_f32, int64_t logits_ld, const float* draft_probs,
+                         int64_t draft_ld, int64_t prob_rows, const int64_t* tokens, const float* uniforms,
+                         const int32_t* offsets, const float* temperature, int64_t requests, int64_t rows, int64_t vocab,
+                         int32_t* accepted, int64_t* out, void* workspace, size_t workspace_bytes,
+                         fp8lin_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Deterministic synthetic inputs (no reference counterpart; used by the
  * benchmark and tests so that the device and a host checker see the same
  * bits).  Element i of stream `tag` is a standard normal from Philox4x32-10
