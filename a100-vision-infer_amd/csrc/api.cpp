@@ -516,7 +516,7 @@ void check_pages(int64_t width, int64_t page_size) {
 }
 
 void check_requests(int64_t requests, int64_t rows) {
-    require(requests > 0 && requests <= FP8LIN_PAGED_MAX_REQUESTS, FP8LIN_ERR_SHAPE, "paged cache: 1 to 8192 requests");
+    require(requests > 0 && requests <= FP8LIN_PAGED_MAX_REQUESTS, FP8LIN_ERR_SHAPE, "paged cache: 1 to FP8LIN_PAGED_MAX_REQUESTS requests");
     require(rows >= 0 && rows < kMaxDim, FP8LIN_ERR_SHAPE, "paged cache: invalid number of rows");
 }
 

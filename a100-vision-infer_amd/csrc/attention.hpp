@@ -73,15 +73,23 @@ __device__ __forceinline__ bf16x8 codes8_bf16(uint32_t lo, uint32_t hi) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// 8 query values of a row from element d (16 bytes when the rows start on
-// them), zeros for a row past the tile.
-__device__ __forceinline__ u32x4 load_q8(const PagedAttention& a, const uint16_t* row, bool valid, int d) {
-    if (!valid) return u32x4{0, 0, 0, 0};
-    if (a.q_vec) return load_u32x4(row + d);
-    u32x4 v;
+// N fragments of 8 values of a query row, from elements at(t) (16 bytes when
+// the rows start on them); zeros for a row past the tile, whose pointer is
+// that of some row.  Loaded without a condition, so that all are in flight.
+template <int N, class AT>
+__device__ __forceinline__ void load_queries(const PagedAttention& a, const uint16_t* row, bool valid, bf16x8 (&qf)[N], AT at) {
+    u32x4 v[N];
+    if (a.q_vec) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (uint32_t)row[d + 2 * i] | (uint32_t)row[d + 2 * i + 1] << 16;
-    return v;
+        for (int t = 0; t < N; ++t) v[t] = load_u32x4(row + at(t));
+    } else {
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[t][i] = (uint32_t)row[at(t) + 2 * i] | (uint32_t)row[at(t) + 2 * i + 1] << 16;
+    }
+#pragma unroll
+    for (int t = 0; t < N; ++t) qf[t] = __builtin_bit_cast(bf16x8, valid ? v[t] : u32x4{0, 0, 0, 0});
 }
 
 // out[d .. d+3] = bf16(o * sigmoid(gate)): one rounding.
@@ -113,82 +121,122 @@ __device__ __forceinline__ void store4(const PagedAttention& a, int64_t tok, int
     }
 }
 
-// Partial sums of a split unit's piece in the workspace: O (BM x D floats, the
-// kernel's own order), then m and l of the BM rows.  A workgroup leaves at
-// most two: slot 0 for the piece that begins inside a unit (its first), slot 1
-// for the one that begins a unit (its last).
+// The workspace: where each workgroup's piece begins (request, kv head, row
+// tile, key tile; request -1: no piece; the request's first row, the tile's
+// rows), then the partial sums of split units:
+// O (BM x D floats, the kernel's own order), m and l of the BM rows.  A
+// workgroup leaves at most two: slot 0 for the piece that begins inside a unit
+// (its first), slot 1 for the one that begins a unit (its last).
+typedef int i32x4v __attribute__((ext_vector_type(4)));
+constexpr int kBeginFloats = kGroups * 8;
 template <int BM, int D>
 struct Partial {
     static constexpr int64_t kFloats = (int64_t)BM * D + 2 * BM;
+    static constexpr int64_t kBytes = 4 * (kBeginFloats + 2 * kGroups * kFloats);
     static __device__ __forceinline__ float* at(float* ws, int group, int slot) {
-        return ws + (2 * group + slot) * kFloats;
+        return ws + kBeginFloats + (2 * group + slot) * kFloats;
     }
 };
 
 hipError_t launch_few(const PagedAttention& a, int D, bool fp8, int rows, hipStream_t stream);
 hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t stream);
 
-// Joins the pieces of the units that the boundaries between workgroups cut.
-// Workgroup (w, y): boundary w + 1, the y-th part of the unit's rows; only the
-// first boundary inside a unit has work.  Each thread joins 4 values of one
-// row, reading the pieces in order.  ROW(e, row, d): row and first dimension
-// of the e-th 4 floats of a piece's O.
-template <int BM, int BN, int D, class Order>
-__global__ __launch_bounds__(256) void join_kernel(PagedAttention a, int groups, int min_tiles) {
-    extern __shared__ __align__(16) int64_t pre[];
-    using Split = PagedSplit<BM, BN>;
-    Split::prefix(a, pre, 256);
-    const int64_t total = pre[a.B], chunk = Split::chunk(a, total, groups, min_tiles);
-    const int w = blockIdx.x + 1;
-    const int64_t p = w * chunk;
-    if (p >= total) return;
-    const auto u = Split::locate(a, pre, p);
-    if (u.kt == 0) return;
-    if (w > 1) {
-        const auto v = Split::locate(a, pre, p - chunk);
-        if (v.b == u.b && v.hk == u.hk && v.r == u.r && v.kt > 0) return;
+// Joins the pieces of the units that the boundaries between workgroups cut,
+// and writes their rows.  Every workgroup lists the split units from the
+// pieces' beginnings and takes every gridDim.x-th part of them: 64 (WAVES 4:
+// its waves share the pieces of a unit, which are many and small in a decode
+// step) or 256 (WAVES 1) groups of 4 values.  ORDER::place(e, row, d): row and
+// first dimension of the e-th 4 floats of a piece's O.
+template <int BM, int D, int WAVES, class ORDER>
+__global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
+    constexpr int PER = 256 / WAVES, PARTS = BM * D / 4 / PER;
+    __shared__ i32x4v begin[kGroups], rows[kGroups];
+    __shared__ int unit[kGroups], unit_last[kGroups], wave_units[4];
+    __shared__ f32x4 so[WAVES][PER];
+    __shared__ float sm[WAVES][PER], sl[WAVES][PER];
+    static_assert(kGroups == 256, "a thread per piece");
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    begin[tid] = reinterpret_cast<const i32x4v*>(a.ws)[2 * tid];
+    rows[tid] = reinterpret_cast<const i32x4v*>(a.ws)[2 * tid + 1];
+    __syncthreads();
+    auto same = [](const i32x4v& x, const i32x4v& y) { return x.x == y.x && x.y == y.y && x.z == y.z; };
+    // the first boundary inside a unit
+    const i32x4v mine = begin[tid];
+    const bool first = tid > 0 && mine.x >= 0 && mine.w > 0 && !(same(begin[tid - 1], mine) && begin[tid - 1].w > 0);
+    const uint64_t mask = __ballot(first);
+    if (lane == 0) wave_units[wave] = __popcll(mask);
+    __syncthreads();
+    int at = __popcll(mask & ((1ull << lane) - 1)), units = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) at += wave_units[w];
+        units += wave_units[w];
     }
-    const PagedSeq s = paged_seq(a, u.b);
-    const int r0 = u.r * BM, nr = (int)min((int64_t)BM, (int64_t)s.n * a.G - r0);
-    const int e = blockIdx.y * 256 + threadIdx.x;
-    int row, d;
-    Order::place(e, row, d);
-    const float vs = a.v_scale ? a.v_scale[u.hk] : 1.0f;
-    // piece i: [kt_i, kt_{i+1}), by workgroup w - 1 + i
-    float M = -__builtin_inff(), l = 0.0f;
-    f32x4 o = {0, 0, 0, 0};
-    int kt = 0, slot = 1;
-    for (int g = w - 1;; ++g) {
-        const int64_t pn = (g + 1) * chunk;
-        bool more = false;
-        int next = 0;
-        if (pn < total) {
-            const auto v = Split::locate(a, pre, pn);
-            more = v.b == u.b && v.hk == u.hk && v.r == u.r;
-            next = v.kt;
-        }
-        if (!more || next > kt) {
-            const float* part = Partial<BM, D>::at(a.ws, g, slot);
-            const float m1 = part[(int64_t)BM * D + row], l1 = part[(int64_t)BM * D + BM + row];
-            const f32x4 o1 = *reinterpret_cast<const f32x4*>(part + 4 * (int64_t)e);
+    if (first) unit[at] = tid;
+    if (tid > 0 && mine.x >= 0 && mine.w > 0 && (tid == kGroups - 1 || !same(begin[tid + 1], mine)))
+        unit_last[at + (first ? 0 : -1)] = tid;
+    __syncthreads();
+    const int q = WAVES > 1 ? wave : 0, et = WAVES > 1 ? lane : tid;
+    for (int item = blockIdx.x; item < units * PARTS; item += gridDim.x) {
+        const int w = unit[item / PARTS], e = (item % PARTS) * PER + et;
+        const i32x4v u = begin[w];
+        const int r0 = u.z * BM, off = rows[w].x, nr = rows[w].y;
+        int row, d;
+        ORDER::place(e, row, d);
+        const bool ok = row < nr;
+        // the unit's pieces: workgroups w - 1 (slot 1), w, .. last (slot 0)
+        const int last = unit_last[item / PARTS];
+        float M = -__builtin_inff(), l = 0.0f;
+        f32x4 o = {0, 0, 0, 0};
+        auto add = [&](float m1, float l1, f32x4 o1) {
             const float mn = fmaxf(M, m1);
             const float f0 = M == -__builtin_inff() ? 0.0f : exp2_fast(M - mn);
             const float f1 = m1 == -__builtin_inff() ? 0.0f : exp2_fast(m1 - mn);
-            l = l * f0 + l1 * f1;
+            l = (f0 == 0.0f ? 0.0f : l * f0) + (f1 == 0.0f ? 0.0f : l1 * f1);
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = (f0 == 0.0f ? 0.0f : o[i] * f0) + (f1 == 0.0f ? 0.0f : o1[i] * f1);
             M = mn;
-            kt = next;
-            slot = 0;
-        }
-        if (!more) break;
-    }
-    if (row >= nr) return;
-    const float inv = l == 0.0f ? 0.0f : vs / l;
+        };
+        if (ok) {
+            constexpr int UN = WAVES > 1 ? 8 : 4;  // pieces whose loads are in flight together
+            for (int g0 = w - 1 + q; g0 <= last; g0 += WAVES * UN) {
+                float m1[UN], l1[UN];
+                f32x4 o1[UN];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : o[i] * inv;
-    const int flat = r0 + row;
-    store4(a, s.off + flat / a.G, u.hk * a.G + flat % a.G, d, o);
+                for (int i = 0; i < UN; ++i) {
+                    const int g = g0 + i * WAVES;
+                    // an empty piece: the next one begins where it does
+                    const bool there = g <= last && !(g < last && g >= w && begin[g + 1].w == begin[g].w);
+                    // loaded without a condition (another piece's), so that all are in flight
+                    const int from = there ? g : w - 1;
+                    const float* part = Partial<BM, D>::at(a.ws, from, from < w);
+                    m1[i] = part[(int64_t)BM * D + row];
+                    l1[i] = part[(int64_t)BM * D + BM + row];
+                    o1[i] = *reinterpret_cast<const f32x4*>(part + 4 * (int64_t)e);
+                    if (!there) m1[i] = -__builtin_inff();
+                }
+#pragma unroll
+                for (int i = 0; i < UN; ++i) add(m1[i], l1[i], o1[i]);
+            }
+        }
+        if constexpr (WAVES > 1) {
+            __syncthreads();
+            so[q][et] = o;
+            sm[q][et] = M;
+            sl[q][et] = l;
+            __syncthreads();
+            if (q == 0)
+#pragma unroll
+                for (int i = 1; i < WAVES; ++i) add(sm[i][et], sl[i][et], so[i][et]);
+        }
+        if (q == 0 && ok) {
+            const float inv = l == 0.0f ? 0.0f : (a.v_scale ? a.v_scale[u.y] : 1.0f) / l;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : o[i] * inv;
+            const int flat = r0 + row;
+            store4(a, off + flat / a.G, u.y * a.G + flat % a.G, d, o);
+        }
+    }
 }
 
 }  // namespace attn

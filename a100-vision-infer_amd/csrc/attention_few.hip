@@ -35,6 +35,9 @@ struct Few {
     static constexpr int DEPTH = 16384 / SLOT;        // tiles of a wave's ring
     static constexpr int WAVE = 2 * DEPTH * SLOT;     // 32 KB per wave
     static constexpr int LDS = kFewWaves * WAVE;      // 128 KB
+    // What a unit's start and end cost, as keys that stream in that time: 5 us
+    // (its queries and first tiles, the join) at a CU's 30 KB per us.
+    static constexpr int START = 160 * 1024 / (2 * ROWB);
     static constexpr int IN_FLIGHT = (2 * DEPTH - 1) * NI;
 
     // Chunk permutations: 16 keys (K) at one chunk, or the keys of a
@@ -61,7 +64,7 @@ template <int D, bool F8, int NT>
 __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a) {
     using F = Few<D, F8>;
     constexpr int BM = 16 * NT, KT = F::KT, SUB = KT / 16, ES = F8 ? 1 : 2;
-    using Split = PagedSplit<BM, KT>;
+    using Split = PagedSplit<BM, KT, F::START>;
     extern __shared__ __align__(1024) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int quad = lane >> 4, col = lane & 15;
@@ -72,10 +75,18 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
     // consecutive pieces on one XCD
     const int group = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     const int64_t p0 = group * chunk, p1 = min(p0 + chunk, total);
-    if (p0 >= total) return;
-    auto cur = Split::locate(a, pre, p0);
-    typename Split::Loc end{a.B, 0, 0, 0};
-    if (p1 < total) end = Split::locate(a, pre, p1);
+    i32x4v* begin = reinterpret_cast<i32x4v*>(a.ws) + 2 * group;
+    if (p0 >= total) {
+        if (tid == 0) begin[0] = i32x4v{-1, 0, 0, 0};
+        return;
+    }
+    typename Split::Loc cur, end;
+    Split::piece(a, pre, p0, p1, cur, end);
+    PagedSeq s = paged_seq(a, cur.b);
+    if (tid == 0) {
+        begin[0] = i32x4v{cur.b, cur.hk, cur.r, cur.kt};
+        begin[1] = i32x4v{s.off, (int)min((int64_t)BM, (int64_t)s.n * a.G - (int64_t)cur.r * BM), 0, 0};
+    }
     __syncthreads();
 
     const uint32_t ring = (uint32_t)(uintptr_t)lds + wave * F::WAVE;
@@ -83,7 +94,6 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
     const int lr = lane / F::LPR, lc = lane % F::LPR;
 
     for (;;) {
-        const PagedSeq s = paged_seq(a, cur.b);
         const int R = Split::tiles(a, s);
         const int nkt = R ? Split::key_tiles(a, s, cur.r) : 0;
         const bool last = cur.b == end.b && cur.hk == end.hk && cur.r == end.r;
@@ -91,6 +101,17 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
         if (R && k1 > k0) {
             const int r0 = cur.r * BM, nr = (int)min((int64_t)BM, (int64_t)s.n * a.G - r0);
             const int nt_used = (nr + 15) >> 4;
+            // page ids of this wave's next key tiles, a lane each; the first ones
+            // come with the queries
+            const int32_t* table = a.table + (int64_t)cur.b * a.ldt;
+            constexpr int BATCH = 64 / SUB;  // tiles whose page ids one load brings
+            int ids;
+            auto load_ids = [&](int j0) {
+                const int64_t key = ((int64_t)k0 + wave + (int64_t)kFewWaves * (j0 + lane / SUB)) * KT + 16 * (lane % SUB);
+                const int id = table[min(key, (int64_t)s.len - 1 + (s.len == 0)) >> a.page_bits];
+                ids = key < s.len ? id : -1;
+            };
+            load_ids(0);
             const float c = a.scale2 * (F8 ? a.k_scale[cur.hk] : 1.0f);
             // queries (B operand: row col, dimensions 64 t + 16 quad + 8 e ..)
             bf16x8 qf[NT][D / 32];
@@ -100,11 +121,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                 const int row = 16 * nt + col, flat = r0 + row, tok = flat / a.G;
                 const bool ok = row < nr;
                 const uint16_t* q = a.q + (int64_t)(s.off + (ok ? tok : 0)) * a.q_tok + (int64_t)(cur.hk * a.G + flat % a.G) * a.q_head;
-#pragma unroll
-                for (int t = 0; t < D / 64; ++t)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        qf[nt][2 * t + e] = __builtin_bit_cast(bf16x8, load_q8(a, q, ok, 64 * t + 16 * quad + 8 * e));
+                load_queries<D / 32>(a, q, ok, qf[nt], [&](int t) { return 32 * (t & ~1) + 16 * quad + 8 * (t & 1); });
                 lim[nt] = !ok ? 0 : a.causal ? min(max(s.len - s.n + tok + 1, 0), s.len) : s.len;
             }
             // the fewest keys that a row of the tile may see: tiles below need no mask
@@ -123,13 +140,6 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
             const int n = k0 + wave < k1 ? (k1 - k0 - wave + kFewWaves - 1) / kFewWaves : 0;
             const char* kbase = static_cast<const char*>(a.k.data) + cur.hk * a.k.head * ES;
             const char* vbase = static_cast<const char*>(a.v.data) + cur.hk * a.v.head * ES;
-            const int32_t* table = a.table + (int64_t)cur.b * a.ldt;
-            constexpr int BATCH = 64 / SUB;  // tiles whose page ids one load brings
-            int ids = -1;
-            auto load_ids = [&](int j0) {
-                const int64_t key = ((int64_t)k0 + wave + (int64_t)kFewWaves * (j0 + lane / SUB)) * KT + 16 * (lane % SUB);
-                ids = key < s.len ? table[key >> a.page_bits] : -1;
-            };
             // K (V) of the wave's tile j into its ring place
             auto issue = [&](int j, bool is_v) {
                 const PagedCache& cache = is_v ? a.v : a.k;
@@ -151,7 +161,6 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                     }
                 }
             };
-            load_ids(0);
 #pragma unroll 1
             for (int j = 0; j < F::DEPTH; ++j) {
                 issue(j, false);
@@ -186,9 +195,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                         for (int e = 0; e < 2; ++e)
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
-                                if (NT == 1 || nt < nt_used)
-                                    st[nt][sub] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[e], qf[nt][2 * t + e],
-                                                                                          st[nt][sub], 0, 0, 0);
+                                st[nt][sub] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[e], qf[nt][2 * t + e], st[nt][sub],
+                                                                                      0, 0, 0);
                     }
                 }
                 wait_lgkm<0>();
@@ -244,21 +252,19 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                         const i32x2 w = read_tr8(vs + row * F::ROWB + ((dt ^ F::xv(row)) << 4) + 8 * (col & 1));
                         const bf16x8 vf = codes8_bf16((uint32_t)w.x, (uint32_t)w.y);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            if (NT == 1 || nt < nt_used) {
-                                const u32x4 pb = {pw[nt][0].x, pw[nt][0].y, pw[nt][SUB - 1].x, pw[nt][SUB - 1].y};
-                                o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, pb),
-                                                                                    o[nt][dt], 0, 0, 0);
-                            }
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const u32x4 pb = {pw[nt][0].x, pw[nt][0].y, pw[nt][SUB - 1].x, pw[nt][SUB - 1].y};
+                            o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, pb), o[nt][dt],
+                                                                                0, 0, 0);
+                        }
                     } else {
                         // 4 keys 4 quad + 0..3 of dimension 16 dt + col
                         const int row = 4 * quad + (col >> 2), ch = 2 * dt + ((col & 3) >> 1);
                         const s16x4 vf = read_tr16(vs + row * F::ROWB + ((ch ^ F::xv(row)) << 4) + 8 * (col & 1));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
-                            if (NT == 1 || nt < nt_used)
-                                o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
-                                    vf, __builtin_bit_cast(s16x4, pw[nt][0]), o[nt][dt], 0, 0, 0);
+                            o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+                                vf, __builtin_bit_cast(s16x4, pw[nt][0]), o[nt][dt], 0, 0, 0);
                     }
                 }
                 wait_lgkm<0>();
@@ -337,7 +343,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                 cur.hk = 0;
                 do {
                     if (++cur.b >= a.B) return;
-                } while (paged_seq(a, cur.b).n == 0);
+                    s = paged_seq(a, cur.b);
+                } while (s.n == 0);
             }
         }
     }
@@ -354,7 +361,7 @@ struct FewOrder {
 template <int D, bool F8, int NT>
 hipError_t run(const PagedAttention& a, hipStream_t stream) {
     constexpr int BM = 16 * NT, LDS = Few<D, F8>::LDS;
-    static_assert(LDS >= kPagedMaxRequests * 8 + 8, "the prefix of the requests' costs fits");
+    static_assert(LDS >= PagedSplit<BM, 16, 0>::lds_bytes(kPagedMaxRequests), "the prefix of the requests' costs fits");
     static_assert(LDS >= kFewWaves * 16 * (D + 6) * 4, "the waves' sums fit");
     auto* kern = few_kernel<D, F8, NT>;
     static const hipError_t attr =
@@ -363,8 +370,8 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
     hipLaunchKernelGGL(kern, dim3(kGroups), dim3(64 * kFewWaves), LDS, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    auto* join = join_kernel<BM, Few<D, F8>::KT, D, FewOrder<D>>;
-    hipLaunchKernelGGL(join, dim3(kGroups - 1, BM * D / 1024), dim3(256), (a.B + 1) * 8, stream, a, kGroups, kFewMinTiles);
+    auto* join = join_kernel<BM, D, 4, FewOrder<D>>;
+    hipLaunchKernelGGL(join, dim3(2 * kGroups), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

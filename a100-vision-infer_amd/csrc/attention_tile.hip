@@ -15,6 +15,8 @@
 // BF16 caches go to LDS by direct DMA; the codes of an 8-bit cache through
 // registers, converted once per workgroup on the way, so that the products see
 // the same layout.
+#include <algorithm>
+
 #include "attention.hpp"
 
 namespace fp8lin {
@@ -23,6 +25,7 @@ namespace {
 
 constexpr int kTileKeys = 64;
 constexpr int kTileMinTiles = 4;
+constexpr int kTileStart = 128;  // a unit's start and end, in keys
 constexpr int kTileWaves = 8;
 
 template <int D>
@@ -41,7 +44,7 @@ template <int D, bool F8, int W>
 __global__ __launch_bounds__(64 * W, 1) void tile_kernel(PagedAttention a) {
     using L = Tile<D>;
     constexpr int BM = 32 * W, KEYS = kTileKeys / W;  // keys that a wave brings of each tile
-    using Split = PagedSplit<BM, kTileKeys>;
+    using Split = PagedSplit<BM, kTileKeys, kTileStart>;
     extern __shared__ __align__(1024) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = lane >> 5, col = lane & 31;
@@ -51,15 +54,22 @@ __global__ __launch_bounds__(64 * W, 1) void tile_kernel(PagedAttention a) {
     const int64_t total = pre[a.B], chunk = Split::chunk(a, total, gridDim.x, kTileMinTiles);
     const int group = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     const int64_t p0 = group * chunk, p1 = min(p0 + chunk, total);
-    if (p0 >= total) return;
-    auto cur = Split::locate(a, pre, p0);
-    typename Split::Loc end{a.B, 0, 0, 0};
-    if (p1 < total) end = Split::locate(a, pre, p1);
+    i32x4v* begin = reinterpret_cast<i32x4v*>(a.ws) + 2 * group;
+    if (p0 >= total) {
+        if (tid == 0) begin[0] = i32x4v{-1, 0, 0, 0};
+        return;
+    }
+    typename Split::Loc cur, end;
+    Split::piece(a, pre, p0, p1, cur, end);
+    PagedSeq s = paged_seq(a, cur.b);
+    if (tid == 0) {
+        begin[0] = i32x4v{cur.b, cur.hk, cur.r, cur.kt};
+        begin[1] = i32x4v{s.off, (int)min((int64_t)BM, (int64_t)s.n * a.G - (int64_t)cur.r * BM), 0, 0};
+    }
     __syncthreads();
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
 
     for (;;) {
-        const PagedSeq s = paged_seq(a, cur.b);
         const int R = Split::tiles(a, s);
         const int nkt = R ? Split::key_tiles(a, s, cur.r) : 0;
         const bool last = cur.b == end.b && cur.hk == end.hk && cur.r == end.r;
@@ -73,8 +83,7 @@ __global__ __launch_bounds__(64 * W, 1) void tile_kernel(PagedAttention a) {
             bf16x8 qf[D / 16];  // B operand: row col, dimensions 16 t + 8 half ..
             {
                 const uint16_t* q = a.q + (int64_t)(s.off + (ok ? tok : 0)) * a.q_tok + (int64_t)(cur.hk * a.G + flat % a.G) * a.q_head;
-#pragma unroll
-                for (int t = 0; t < D / 16; ++t) qf[t] = __builtin_bit_cast(bf16x8, load_q8(a, q, ok, 16 * t + 8 * half));
+                load_queries<D / 16>(a, q, ok, qf, [&](int t) { return 16 * t + 8 * half; });
             }
             const int ctx = s.len - s.n;
             const int lim = !ok ? 0 : a.causal ? min(max(ctx + tok + 1, 0), s.len) : s.len;
@@ -277,7 +286,8 @@ __global__ __launch_bounds__(64 * W, 1) void tile_kernel(PagedAttention a) {
                 cur.hk = 0;
                 do {
                     if (++cur.b >= a.B) return;
-                } while (paged_seq(a, cur.b).n == 0);
+                    s = paged_seq(a, cur.b);
+                } while (s.n == 0);
             }
         }
     }
@@ -294,7 +304,7 @@ struct TileOrder {
 
 template <int D, bool F8, int W>
 hipError_t run(const PagedAttention& a, hipStream_t stream) {
-    constexpr int BM = 32 * W, LDS = Tile<D>::LDS > (kPagedMaxRequests + 1) * 8 ? Tile<D>::LDS : (kPagedMaxRequests + 1) * 8;
+    constexpr int BM = 32 * W, LDS = std::max<int>(Tile<D>::LDS, PagedSplit<BM, kTileKeys, 0>::lds_bytes(kPagedMaxRequests));
     auto* kern = tile_kernel<D, F8, W>;
     static const hipError_t attr =
         hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -302,8 +312,8 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
     hipLaunchKernelGGL(kern, dim3(kGroups), dim3(64 * W), LDS, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    auto* join = join_kernel<BM, kTileKeys, D, TileOrder<D>>;
-    hipLaunchKernelGGL(join, dim3(kGroups - 1, BM * D / 1024), dim3(256), (a.B + 1) * 8, stream, a, kGroups, kTileMinTiles);
+    auto* join = join_kernel<BM, D, 1, TileOrder<D>>;
+    hipLaunchKernelGGL(join, dim3(4 * kGroups), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
@@ -323,7 +333,7 @@ constexpr int kFewRows = 64;  // rows that the few-rows kernel takes; see launch
 
 size_t paged_attention_ws_bytes(int D, int64_t max_rows) {
     const int64_t bm = max_rows <= 16 ? 16 : max_rows <= 32 ? 32 : max_rows <= kFewRows ? 64 : 32 * attn::kTileWaves;
-    return (size_t)(2 * attn::kGroups * (bm * D + 2 * bm) * 4);
+    return (size_t)(4 * (attn::kBeginFloats + 2 * attn::kGroups * (bm * D + 2 * bm)));
 }
 
 // Either kernel computes any number of rows; the rule is what each is fast at.

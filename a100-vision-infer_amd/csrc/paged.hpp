@@ -30,7 +30,7 @@ struct PagedAttention {
     float* ws;
 };
 
-constexpr int kPagedMaxRequests = 8192;
+constexpr int kPagedMaxRequests = 4096;
 constexpr int kPagedMinPage = 16;
 
 // Workgroups of the attention launch for D and the row tile that max_rows
@@ -55,8 +55,8 @@ size_t paged_layout_ws_bytes(int64_t B);
 // A unit is one row tile (BM rows: consecutive tokens of a request, the G
 // query heads of one kv head side by side) against the keys that its last row
 // may see.  The units in the order (request, kv head, row tile) are laid on a
-// line, each as long as it costs (its keys times G), and workgroup w computes
-// the piece [w, w + 1) * chunk of that line: every workgroup has the same
+// line, each as long as it costs (START and its keys, times G), and workgroup w
+// computes the piece [w, w + 1) * chunk of that line: every workgroup has the same
 // amount of work, whatever the lengths.  A unit that falls into several
 // pieces is joined afterwards from their partial sums.  The split depends on
 // the lengths alone, so a call's result does not depend on timing.
@@ -73,7 +73,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttention& a, int b) {
     return PagedSeq{lo, hi - lo, (int)len};
 }
 
-template <int BM, int BN>
+template <int BM, int BN, int START>
 struct PagedSplit {
     struct Loc {
         int b, hk, r, kt;
@@ -81,16 +81,16 @@ struct PagedSplit {
 
     // Cost of the first x row tiles, x < R; ctx: keys before the new tokens.
     static __device__ __forceinline__ int64_t first(const PagedAttention& a, const PagedSeq& s, int64_t x) {
-        if (!a.causal) return x * a.G * max(s.len, 1);
-        return x * a.G * max(s.len - s.n, 0) + BM * (x * (x + 1) / 2);
+        if (!a.causal) return x * a.G * (START + max(s.len, 1));
+        return x * a.G * (START + max(s.len - s.n, 0)) + BM * (x * (x + 1) / 2);
     }
     static __device__ __forceinline__ int tiles(const PagedAttention& a, const PagedSeq& s) {
         return (int)(((int64_t)s.n * a.G + BM - 1) / BM);
     }
     // Cost of row tile r of R.
     static __device__ __forceinline__ int64_t tile(const PagedAttention& a, const PagedSeq& s, int r) {
-        if (!a.causal) return (int64_t)a.G * max(s.len, 1);
-        return (int64_t)a.G * max(s.len - s.n, 0) + min((int64_t)(r + 1) * BM, (int64_t)s.n * a.G);
+        if (!a.causal) return (int64_t)a.G * (START + max(s.len, 1));
+        return (int64_t)a.G * (START + max(s.len - s.n, 0)) + min((int64_t)(r + 1) * BM, (int64_t)s.n * a.G);
     }
     // All row tiles of one kv head.
     static __device__ __forceinline__ int64_t head(const PagedAttention& a, const PagedSeq& s) {
@@ -108,52 +108,73 @@ struct PagedSplit {
         return max((limit + BN - 1) / BN, 1);
     }
 
-    // prefix[b] = cost of the requests before b, for b <= B; all threads of
-    // the workgroup, which synchronise here.
+    // floor(x / y) for 0 <= x, 0 < y, both below 2^52: by the FP64 quotient,
+    // whose error of under half a unit of the result the two checks take back.
+    static __device__ __forceinline__ int64_t div(int64_t x, int64_t y) {
+        int64_t q = (int64_t)((double)x / (double)y);
+        if (q * y > x) --q;
+        if ((q + 1) * y <= x) ++q;
+        return q;
+    }
+
+    // What a workgroup knows of the batch while it finds its piece, in LDS:
+    // prefix[b] = cost of the requests before b, b <= B, then each request's
+    // (new tokens, keys).
+    static constexpr size_t lds_bytes(int64_t B) { return (size_t)(16 * B + 16); }
+    static __device__ __forceinline__ int* held(const PagedAttention& a, int64_t* pre) {
+        return reinterpret_cast<int*>(pre + a.B + 1);
+    }
+    // All threads of the workgroup, which synchronise here.
     static __device__ void prefix(const PagedAttention& a, int64_t* pre, int threads) {
         __shared__ int64_t wave_total[16];
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
-        const int per = (a.B + threads - 1) / threads;
-        const int lo = min(tid * per, a.B), hi = min(lo + per, a.B);
-        int64_t sum = 0;
-        for (int b = lo; b < hi; ++b) sum += (int64_t)a.HK * head(a, paged_seq(a, b));
-        int64_t run = sum;
+        int* h = held(a, pre);
+        int64_t base = 0;
+        for (int b0 = 0; b0 < a.B; b0 += threads) {
+            const int b = b0 + tid;
+            int64_t cost = 0;
+            if (b < a.B) {
+                const PagedSeq s = paged_seq(a, b);
+                cost = (int64_t)a.HK * head(a, s);
+                h[2 * b] = s.n;
+                h[2 * b + 1] = s.len;
+            }
+            int64_t run = cost;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t o = __shfl_up(run, d, 64);
-            if (lane >= d) run += o;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int64_t o = __shfl_up(run, d, 64);
+                if (lane >= d) run += o;
+            }
+            if (lane == 63) wave_total[wave] = run;
+            __syncthreads();
+            int64_t before = base + run - cost;
+            for (int w = 0; w < waves; ++w) {
+                if (w < wave) before += wave_total[w];
+                base += wave_total[w];
+            }
+            if (b < a.B) pre[b] = before;
+            __syncthreads();
         }
-        if (lane == 63) wave_total[wave] = run;
-        __syncthreads();
-        int64_t base = run - sum;
-        for (int w = 0; w < waves; ++w)
-            if (w < wave) base += wave_total[w];
-        for (int b = lo; b < hi; ++b) {
-            pre[b] = base;
-            base += (int64_t)a.HK * head(a, paged_seq(a, b));
-        }
-        if (tid == 0) {
-            int64_t t = 0;
-            for (int w = 0; w < waves; ++w) t += wave_total[w];
-            pre[a.B] = t;
-        }
+        if (tid == 0) pre[a.B] = base;
         __syncthreads();
     }
 
-    // The place p of the line, 0 <= p < prefix[B]: within its unit, key tile
-    // kt = floor(part of the unit's cost before p * its key tiles).
-    static __device__ Loc locate(const PagedAttention& a, const int64_t* pre, int64_t p) {
+    // The place p of the line, 0 <= p < prefix[B]: within its unit, behind the
+    // START, key tile kt = floor(part of the unit's cost before p * its key
+    // tiles).
+    static __device__ Loc locate(const PagedAttention& a, int64_t* pre, int64_t p) {
         int lo = 0, hi = a.B;  // pre[lo] <= p < pre[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (pre[mid] <= p) lo = mid; else hi = mid;
         }
-        const PagedSeq s = paged_seq(a, lo);
+        const int* h = held(a, pre) + 2 * lo;
+        const PagedSeq s{0, h[0], h[1]};
         const int64_t per_head = head(a, s);
         int64_t q = p - pre[lo];
         Loc l;
         l.b = lo;
-        l.hk = (int)(q / per_head);
+        l.hk = (int)div(q, per_head);
         q -= l.hk * per_head;
         int rl = 0, rh = tiles(a, s);
         while (rh - rl > 1) {
@@ -161,8 +182,21 @@ struct PagedSplit {
             if (first(a, s, mid) <= q) rl = mid; else rh = mid;
         }
         l.r = rl;
-        l.kt = (int)((q - first(a, s, rl)) * key_tiles(a, s, rl) / tile(a, s, rl));
+        const int64_t start = (int64_t)START * a.G;
+        q = max(q - first(a, s, rl) - start, (int64_t)0);
+        l.kt = (int)div(q * key_tiles(a, s, rl), tile(a, s, rl) - start);
         return l;
+    }
+    // The pieces [p0, p1) of every wave's workgroup: even lanes find where it
+    // begins, odd lanes where it ends (request B if it ends the line).
+    static __device__ void piece(const PagedAttention& a, int64_t* pre, int64_t p0, int64_t p1, Loc& begin, Loc& end) {
+        const int64_t p = (threadIdx.x & 1) ? p1 : p0;
+        Loc l{a.B, 0, 0, 0};
+        if (p < pre[a.B]) l = locate(a, pre, p);
+        begin = Loc{__builtin_amdgcn_readlane(l.b, 0), __builtin_amdgcn_readlane(l.hk, 0), __builtin_amdgcn_readlane(l.r, 0),
+                    __builtin_amdgcn_readlane(l.kt, 0)};
+        end = Loc{__builtin_amdgcn_readlane(l.b, 1), __builtin_amdgcn_readlane(l.hk, 1), __builtin_amdgcn_readlane(l.r, 1),
+                  __builtin_amdgcn_readlane(l.kt, 1)};
     }
     // Length of a piece: an even share, but no shorter than min_tiles key
     // tiles of a unit.

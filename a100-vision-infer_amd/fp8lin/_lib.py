@@ -85,8 +85,6 @@ class PagedCacheRecord(ctypes.Structure):
                 ("v_scale", ctypes.c_void_p)]
 
 
-PAGED_MAX_REQUESTS = 8192
-
 
 class LinearOptions(ctypes.Structure):
     """struct fp8lin_linear_options (the EngineOptions linear flags,

@@ -564,10 +564,10 @@ typedef struct fp8lin_paged_cache {
  *       `table` itself (and may overlap no other argument);
  *   new_cursor [1]  cursor + pages wanted: above free_count, the list was short.
  * Page ids are not checked here; fp8lin_paged_append and
- * fp8lin_paged_attention check them.  0 < requests <= 8192; width * page_size
+ * fp8lin_paged_attention check them.  0 < requests <= 4096; width * page_size
  * <= 2^30.
  */
-#define FP8LIN_PAGED_MAX_REQUESTS 8192
+#define FP8LIN_PAGED_MAX_REQUESTS 4096
 size_t fp8lin_paged_layout_workspace_bytes(int64_t requests);
 int fp8lin_paged_layout(const int32_t* lengths, const int32_t* counts, const int32_t* table, int64_t table_ld,
                         const int32_t* free_pages, int64_t free_count, const int32_t* cursor, int64_t requests,
@@ -598,7 +598,7 @@ int fp8lin_paged_append(const fp8lin_paged_cache* cache, const uint16_t* k, int6
  * width; rows from offsets[requests] on are left as they are.
  * max_count: the most rows that a request is expected to have; more give the
  * same results, slower.  head_dim 64, 128 or 256; scale > 0; 0 < requests <=
- * 8192; width * page_size <= 2^30; tokens * heads < 2^31.  out may not overlap
+ * 4096; width * page_size <= 2^30; tokens * heads < 2^31.  out may not overlap
  * the inputs.  A call's result does not depend on timing, but a row's does on
  * the lengths of the whole batch (FP32 summation order).
  * Workspace: the bytes below, 16-byte aligned, any content.
@@ -628,7 +628,7 @@ int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, i
  *   token, then -1 (as in rows behind the last request).
  * A row without a distribution (NaN, +inf, all -inf) keeps no draft and draws
  * -1; a draft outside [0, vocab) is refused.  64-bit sums.  0 < requests <=
- * 8192; vocab < 2^31.  Workspace: the bytes below, 16-byte aligned, any content.
+ * 4096; vocab < 2^31.  Workspace: the bytes below, 16-byte aligned, any content.
  */
 size_t fp8lin_verify_drafts_workspace_bytes(int64_t requests, int64_t rows, int64_t vocab);
 int fp8lin_verify_drafts(const void* logits, int logits_f32, int64_t logits_ld, const float* draft_probs,
