@@ -26,6 +26,8 @@ namespace {
 
 constexpr int kThreads = 256;
 
+struct Decision;
+
 struct Args {
     const void* logits;
     int64_t ld;
@@ -35,14 +37,17 @@ struct Args {
     const float* u;
     const int32_t* offsets;
     const float* temperature;
-    int B, slices, V, per;  // per: columns of a slice, a multiple of 8
+    int B, V;
+    int slices, per;    // of a row; per: columns of a slice, a multiple of 8
+    int cuts, cut_per;  // of a request's deciding row
     int64_t T;
     int32_t* accepted;
     int64_t* out;
     double* row_sum;    // [T][slices]
     float* row_max;     // [T][slices]
     int32_t* row_at;    // [T][slices] first column of the maximum
-    double* weight;     // [B][slices][2] sums of max(p - q, 0) and of p
+    double* weight;     // [B][cuts][2] sums of max(p - q, 0) and of p
+    Decision* decision;  // [B], by verify_weigh_kernel
 };
 
 struct Request {
@@ -54,39 +59,71 @@ __device__ __forceinline__ Request request(const Args& g, int b) {
     return Request{lo, hi - lo};
 }
 
-template <bool BF16>
-__device__ __forceinline__ float logit(const Args& g, int64_t row, int64_t j) {
-    if constexpr (BF16) return bf16_bits_to_f32(static_cast<const uint16_t*>(g.logits)[row * g.ld + j]);
-    return static_cast<const float*>(g.logits)[row * g.ld + j];
-}
-
 // A temperature of zero (or below) stands for the most likely token.
 __device__ __forceinline__ float temperature(const Args& g, int b) { return g.temperature ? g.temperature[b] : 1.0f; }
 __device__ __forceinline__ bool greedy(float t) { return t <= 0.0f; }
-__device__ __forceinline__ double slope(float t) { return greedy(t) ? 1.0 : 1.0 / (double)t; }
+__device__ __forceinline__ double slope(float t) { return 1.4426950408889634074 / (greedy(t) ? 1.0 : (double)t); }
 
-// e^((x - m) s), nothing for a logit of -inf; NaN for a NaN or a row of +inf.
-__device__ __forceinline__ double weigh(float x, float m, double s) {
-    return x == -__builtin_inff() ? 0.0 : exp(((double)x - (double)m) * s);
-}
+// 2^t for t <= 0 in 64 bits, nothing below 2^-1100 (and for NaN): 2^n 2^f,
+// |f| <= 1/2, 2^f = sum (f ln 2)^k / k! to k = 11, whose next term is below
+// 2^-47.  A relative error of 7e-15 moves a draw among 250 000 tokens with
+// probability 2e-9.  20 instructions without a branch, where the library's exp
+// takes 65: the rows of a batch of 48 requests (170 x 248320) 78 -> ROWS us.
+// The coefficients stay in scalar registers (laundered, or the compiler would
+// load each into a vector register before every use).
+struct Exp2 {
+    double c[12];
+    __device__ Exp2() {
+        constexpr double ln2 = 0.693147180559945309417;
+        double v = 1.0;
+#pragma unroll
+        for (int k = 0; k < 12; ++k) {
+            c[k] = v;
+            v *= ln2 / (k + 1);
+        }
+#pragma unroll
+        for (int k = 0; k < 12; ++k) asm("" : "+s"(c[k]));
+    }
+    __device__ __forceinline__ double operator()(double t) const {
+        t = fmax(t, -1100.0);
+        const double n = __builtin_rint(t), f = t - n;
+        double p = c[11];
+#pragma unroll
+        for (int k = 10; k >= 0; --k) p = __builtin_fma(p, f, c[k]);
+        return __builtin_ldexp(p, (int)n);
+    }
+};
+// e^((x - m) / T) with s = log2(e) / T; nothing for x of -inf (m finite) or
+// NaN.  The difference first: logits may be far larger than their differences.
+__device__ __forceinline__ double weigh(const Exp2& e, float x, float m, double s) { return e(((double)x - (double)m) * s); }
 
-// Maximum, its first column and the sum of exponentials, joined.
+// Maximum, its first column and the sum of exponentials of a part of a row:
+// maximum -inf and sum 0 for a part of nothing but -inf, sum NaN for one that
+// holds a NaN or +inf.
 struct Stat {
     float m;
     int at;
     double sum;
 };
-__device__ __forceinline__ void join(Stat& a, const Stat& b, double s) {
-    const float m = fmaxf(a.m, b.m);
-    const double fa = a.m == m ? 1.0 : a.m == -__builtin_inff() ? 0.0 : exp(((double)a.m - (double)m) * s);
-    const double fb = b.m == m ? 1.0 : b.m == -__builtin_inff() ? 0.0 : exp(((double)b.m - (double)m) * s);
-    // a part without finite logits has sum 0, or NaN that must stay
-    a.sum = (a.sum == 0.0 ? 0.0 : a.sum * (a.sum != a.sum ? 1.0 : fa)) + (b.sum == 0.0 ? 0.0 : b.sum * (b.sum != b.sum ? 1.0 : fb));
-    if (b.m > a.m || (b.m == a.m && b.at < a.at)) a.at = b.at;
-    a.m = m;
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+    return v;
 }
-__device__ __forceinline__ Stat lane_xor(const Stat& v, int d) {
-    return Stat{__shfl_xor(v.m, d, 64), __shfl_xor(v.at, d, 64), __shfl_xor(v.sum, d, 64)};
+// The statistics of a wave's 64 parts; every lane gets them.
+__device__ __forceinline__ Stat wave_join(const Exp2& e, const Stat& v, double s) {
+    Stat r = v;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        const float m = __shfl_xor(r.m, d, 64);
+        const int at = __shfl_xor(r.at, d, 64);
+        if (m > r.m || (m == r.m && at < r.at)) {
+            r.m = m;
+            r.at = at;
+        }
+    }
+    r.sum = wave_sum64(v.sum == 0.0 || v.sum != v.sum ? v.sum : v.sum * weigh(e, v.m, r.m, s));
+    return r;
 }
 
 __device__ __forceinline__ int owner_of(const Args& g, int64_t row) {
@@ -98,8 +135,38 @@ __device__ __forceinline__ int owner_of(const Args& g, int64_t row) {
     return lo;
 }
 
-// Workgroup (row, slice).  VEC: rows start on 16 bytes.
-template <bool BF16, bool VEC>
+// 8 values of a row from column j, `fill` behind `end`.  VEC: rows start on 16
+// bytes (and j is a multiple of 8).
+template <class T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int j, int end, float fill, float (&x)[8]) {
+    if (VEC && j + 8 <= end) {
+        if constexpr (sizeof(T) == 2) {
+            const u32x4 w = load_u32x4(row + j);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = bf16_bits_to_f32((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(row + j), b = *reinterpret_cast<const f32x4*>(row + j + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = a[i];
+                x[4 + i] = b[i];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // a column past the end loads the last one instead, so that all loads are in flight
+            const T v = row[min(j + i, end - 1)];
+            float f;
+            if constexpr (sizeof(T) == 2) f = bf16_bits_to_f32(v);
+            else f = v;
+            x[i] = j + i < end ? f : fill;
+        }
+    }
+}
+
+// Workgroup (row, slice).
+template <class T, bool VEC>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(Args g) {
     __shared__ Stat part[kThreads / 64];
     const int64_t row = blockIdx.x;
@@ -107,67 +174,52 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(Args g) {
     if (row >= g.offsets[g.B]) return;  // behind the last request
     const double s = slope(temperature(g, owner_of(g, row)));
     const int lo = slice * g.per, hi = min(lo + g.per, g.V);
+    const T* logits = static_cast<const T*>(g.logits) + row * g.ld;
+    const Exp2 e;
     Stat v{-__builtin_inff(), INT32_MAX, 0.0};
-    auto take = [&](const float (&x)[8], int j) {
+    bool bad = false;
+    for (int j = lo + 8 * tid; j < hi; j += 8 * kThreads) {
+        float x[8];
+        load8<T, VEC>(logits, j, hi, -__builtin_inff(), x);
         float top = x[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
         if (top > v.m) {
-            if (v.m != -__builtin_inff()) v.sum *= exp(((double)v.m - (double)top) * s);
+            v.sum *= v.sum == 0.0 ? 0.0 : weigh(e, v.m, top, s);
             v.m = top;
 #pragma unroll
             for (int i = 7; i >= 0; --i)
                 if (x[i] == top) v.at = j + i;
         }
+        const float m = v.m == -__builtin_inff() ? 0.0f : v.m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.sum += weigh(x[i], v.m, s);
-    };
-    for (int j = lo + 8 * tid; j < hi; j += 8 * kThreads) {
-        float x[8];
-        if (VEC && j + 8 <= hi) {
-            if constexpr (BF16) {
-                const u32x4 w = load_u32x4(static_cast<const uint16_t*>(g.logits) + row * g.ld + j);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = bf16_bits_to_f32((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
-            } else {
-                const float* p = static_cast<const float*>(g.logits) + row * g.ld + j;
-                const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[i] = a[i];
-                    x[4 + i] = b[i];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = j + i < hi ? logit<BF16>(g, row, j + i) : -__builtin_inff();
+        for (int i = 0; i < 8; ++i) {
+            bad |= x[i] != x[i];
+            v.sum += weigh(e, x[i], m, s);
         }
-        take(x, j);
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) join(v, lane_xor(v, d), s);
+    if (bad || v.m == __builtin_inff()) v.sum = __builtin_nan("");
+    v = wave_join(e, v, s);
     if ((tid & 63) == 0) part[tid >> 6] = v;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kThreads / 64; ++w) join(v, part[w], s);
-        const int64_t at = row * g.slices + slice;
-        g.row_max[at] = v.m;
-        g.row_at[at] = v.at;
-        g.row_sum[at] = v.sum;
+    if (tid < 64) {
+        v = wave_join(e, tid < kThreads / 64 ? part[tid] : Stat{-__builtin_inff(), INT32_MAX, 0.0}, s);
+        if (tid == 0) {
+            const int64_t at = row * g.slices + slice;
+            g.row_max[at] = v.m;
+            g.row_at[at] = v.at;
+            g.row_sum[at] = v.sum;
+        }
     }
 }
 
-// A row's statistics from its slices, by one wave; every lane gets them.
-__device__ __forceinline__ Stat row_stat(const Args& g, int64_t row, double s) {
+// A row's statistics from its slices (at most 64), by one wave.
+__device__ __forceinline__ Stat row_stat(const Args& g, const Exp2& e, int64_t row, double s) {
     const int lane = threadIdx.x & 63;
-    Stat v{-__builtin_inff(), INT32_MAX, 0.0};
-    for (int i = lane; i < g.slices; i += 64) {
-        const int64_t at = row * g.slices + i;
-        join(v, Stat{g.row_max[at], g.row_at[at], g.row_sum[at]}, s);
-    }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) join(v, lane_xor(v, d), s);
-    return v;
+    const int64_t at = row * g.slices + min(lane, g.slices - 1);
+    Stat v{g.row_max[at], g.row_at[at], g.row_sum[at]};
+    if (lane >= g.slices) v = Stat{-__builtin_inff(), INT32_MAX, 0.0};
+    return wave_join(e, v, s);
 }
 
 // Whether the row is a distribution: some finite logit, no NaN, no +inf.
@@ -189,78 +241,108 @@ __device__ int64_t probs_row(const Args& g, int b, const Request& r) {
     }
     return r.a - before;
 }
-__device__ __forceinline__ double draft_prob(const Args& g, int64_t row, int64_t j) {
-    return row >= 0 && row < g.prob_rows ? (double)g.probs[row * g.ldp + j] : 0.0;
-}
 
 // By all threads of a workgroup: wave w tests drafts w, w + 4, ...
-template <bool BF16>
+template <class T>
 __device__ Decision decide(const Args& g, int b, const Request& r) {
+    constexpr int kWaves = kThreads / 64;
     __shared__ int first;
-    __shared__ Stat stat;
+    __shared__ Stat stats[kWaves];
     const int tid = threadIdx.x, wave = tid >> 6;
     const float t = temperature(g, b);
     const double s = slope(t);
+    const Exp2 e;
     const int64_t probs = g.probs ? probs_row(g, b, r) : 0;
     if (tid == 0) first = (int)(r.n - 1);
     __syncthreads();
-    for (int64_t i0 = 0; i0 < r.n - 1 && i0 <= first; i0 += kThreads / 64) {
+    // the row behind the last draft refuses nothing: it ends the loop
+    for (int64_t i0 = 0;; i0 += kWaves) {
         const int64_t i = i0 + wave;
-        if (i < r.n - 1) {
-            const Stat v = row_stat(g, r.a + i, s);
-            const int64_t x = g.tokens[r.a + i + 1];
-            bool keep = false;
-            if (x >= 0 && x < g.V && valid(v)) {
-                const double p = greedy(t) ? (v.at == x ? 1.0 : 0.0) : weigh(logit<BF16>(g, r.a + i, x), v.m, s) / v.sum;
-                const double q = g.probs ? draft_prob(g, probs + i, x) : 1.0;
-                keep = (double)g.u[r.a + i] * q < p;
+        if (i < r.n) {
+            const int64_t row = r.a + i, x = i < r.n - 1 ? g.tokens[row + 1] : -1;
+            const bool in = x >= 0 && x < g.V;
+            const T* logits = static_cast<const T*>(g.logits) + row * g.ld;
+            float at;
+            if constexpr (sizeof(T) == 2) at = bf16_bits_to_f32(logits[in ? x : 0]);
+            else at = logits[in ? x : 0];
+            const int64_t qr = probs + i;
+            const bool q_in = g.probs && in && qr >= 0 && qr < g.prob_rows;
+            const double q = q_in ? (double)g.probs[qr * g.ldp + x] : g.probs ? 0.0 : 1.0;
+            const double u = (double)g.u[row];
+            const Stat v = row_stat(g, e, row, s);
+            const double p = greedy(t) ? (v.at == x ? 1.0 : 0.0) : weigh(e, at, v.m, s) / v.sum;
+            const bool keep = in && valid(v) && u * q < p;
+            if ((tid & 63) == 0) {
+                stats[wave] = v;
+                if (!keep) atomicMin(&first, (int)i);
             }
-            if (!keep && (tid & 63) == 0) atomicMin(&first, (int)i);
         }
         __syncthreads();
+        if (first < i0 + kWaves) break;
     }
-    const int64_t kept = first;
-    if (wave == 0) {
-        const Stat v = row_stat(g, r.a + kept, s);
-        if (tid == 0) stat = v;
-    }
-    __syncthreads();
-    return Decision{kept, stat, probs};
+    return Decision{first, stats[first % kWaves], probs};
 }
 
-// The weight of column j in the deciding row, and its p.
-template <bool BF16>
-__device__ __forceinline__ double weight_at(const Args& g, const Request& r, const Decision& c, float t, double s,
-                                            int64_t x, int j, double& p) {
-    p = greedy(t) ? (j == c.stat.at ? 1.0 : 0.0) : weigh(logit<BF16>(g, r.a + c.kept, j), c.stat.m, s) / c.stat.sum;
-    if (c.kept == r.n - 1) return p;
-    if (!g.probs) return j == x ? 0.0 : p;
-    return fmax(p - draft_prob(g, c.probs + c.kept, j), 0.0);
-}
+// The weights of 8 columns in the deciding row: max(p - q, 0) in w, and p.
+template <class T, bool VEC>
+struct Weights {
+    Exp2 e;
+    const T* logits;
+    const float* q;
+    float m;
+    double s, scale;
+    int at;      // the column of all weight, or -1
+    int64_t x;   // the refused draft without probabilities, or -1
+    bool q_vec;
 
-__device__ __forceinline__ double wave_sum64(double v) {
+    __device__ Weights(const Args& g, int b, const Request& r, const Decision& c) {
+        const float t = temperature(g, b);
+        const bool refused = c.kept < r.n - 1;
+        const int64_t qr = c.probs + c.kept;
+        logits = static_cast<const T*>(g.logits) + (r.a + c.kept) * g.ld;
+        q = refused && g.probs && qr >= 0 && qr < g.prob_rows ? g.probs + qr * g.ldp : nullptr;
+        q_vec = reinterpret_cast<uintptr_t>(q) % 16 == 0;
+        x = refused && !g.probs ? g.tokens[r.a + c.kept + 1] : -1;
+        m = c.stat.m;
+        s = slope(t);
+        scale = 1.0 / c.stat.sum;
+        at = greedy(t) ? c.stat.at : -1;
+    }
+    __device__ __forceinline__ void get(int j, int end, double (&w)[8], double (&p)[8]) const {
+        float lx[8], qx[8];
+        load8<T, VEC>(logits, j, end, -__builtin_inff(), lx);
+        if (q) {
+            if (q_vec) load8<float, true>(q, j, end, 0.0f, qx);
+            else load8<float, false>(q, j, end, 0.0f, qx);
+        }
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
-    return v;
-}
+        for (int i = 0; i < 8; ++i) {
+            p[i] = at >= 0 ? (j + i == at ? 1.0 : 0.0) : weigh(e, lx[i], m, s) * scale;
+            w[i] = q ? fmax(p[i] - (double)qx[i], 0.0) : j + i == x ? 0.0 : p[i];
+        }
+    }
+};
 
 // Workgroup (request, slice).
-template <bool BF16>
+template <class T, bool VEC>
 __global__ __launch_bounds__(kThreads) void verify_weigh_kernel(Args g) {
     __shared__ double ws[kThreads / 64], ps[kThreads / 64];
     const int b = blockIdx.x, slice = blockIdx.y, tid = threadIdx.x;
     const Request r = request(g, b);
     if (r.n == 0) return;
-    const Decision c = decide<BF16>(g, b, r);
-    const float t = temperature(g, b);
-    const double s = slope(t);
-    const int64_t x = c.kept < r.n - 1 ? g.tokens[r.a + c.kept + 1] : -1;
-    const int lo = slice * g.per, hi = min(lo + g.per, g.V);
+    const Decision c = decide<T>(g, b, r);
+    if (slice == 0 && tid == 0) g.decision[b] = c;
+    const Weights<T, VEC> weights(g, b, r, c);
+    const int lo = min(slice * g.cut_per, g.V), hi = min(lo + g.cut_per, g.V);
     double w = 0.0, p = 0.0;
-    for (int j = lo + tid; j < hi; j += kThreads) {
-        double pj;
-        w += weight_at<BF16>(g, r, c, t, s, x, j, pj);
-        p += pj;
+    for (int j = lo + 8 * tid; j < hi; j += 8 * kThreads) {
+        double w8[8], p8[8];
+        weights.get(j, hi, w8, p8);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            w += w8[i];
+            p += p8[i];
+        }
     }
     w = wave_sum64(w);
     p = wave_sum64(p);
@@ -274,17 +356,27 @@ __global__ __launch_bounds__(kThreads) void verify_weigh_kernel(Args g) {
             w += ws[i];
             p += ps[i];
         }
-        g.weight[((int64_t)b * g.slices + slice) * 2] = w;
-        g.weight[((int64_t)b * g.slices + slice) * 2 + 1] = p;
+        g.weight[((int64_t)b * g.cuts + slice) * 2] = w;
+        g.weight[((int64_t)b * g.cuts + slice) * 2 + 1] = p;
     }
 }
 
+// Running sums over the lanes of a wave.
+__device__ __forceinline__ double wave_scan64(double v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double o = __shfl_up(v, d, 64);
+        if ((threadIdx.x & 63) >= d) v += o;
+    }
+    return v;
+}
+
 // One workgroup per request; the last one also clears the rows behind them.
-template <bool BF16>
+template <class T, bool VEC>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(Args g) {
-    __shared__ double run[kThreads], before_s;
+    __shared__ double wave_total[kThreads / 64], target_s;
     __shared__ int slice_s, pick_s, last_s;
-    const int b = blockIdx.x, tid = threadIdx.x;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Request r = request(g, b);
     if (b == g.B - 1)
         for (int64_t i = r.a + r.n + tid; i < g.T; i += kThreads) g.out[i] = -1;
@@ -292,114 +384,117 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(Args g) {
         if (tid == 0) g.accepted[b] = 0;
         return;
     }
-    const Decision c = decide<BF16>(g, b, r);
-    const float t = temperature(g, b);
-    const double s = slope(t);
-    const int64_t x = c.kept < r.n - 1 ? g.tokens[r.a + c.kept + 1] : -1;
-    const bool ok = valid(c.stat);
-    const double* weight = g.weight + (int64_t)b * g.slices * 2;
-    if (tid == 0) {
-        // nothing left where the target is not above the draft: p itself
-        double total = 0.0;
-        for (int i = 0; i < g.slices; ++i) total += weight[2 * i];
-        const int of = total > 0.0 ? 0 : 1;
-        if (of) {
-            total = 0.0;
-            for (int i = 0; i < g.slices; ++i) total += weight[2 * i + 1];
+    if (wave == 0) {
+        // a lane per slice; p itself where the target is nowhere above the draft
+        const double* weight = g.weight + ((int64_t)b * g.cuts + min(lane, g.cuts - 1)) * 2;
+        double w = lane < g.cuts ? weight[0] : 0.0;
+        const double p = lane < g.cuts ? weight[1] : 0.0;
+        const int of = __ballot(w > 0.0) ? 0 : 1;
+        if (of) w = p;
+        const double run = wave_scan64(w), target = (double)g.u[r.a + r.n - 1] * __shfl(run, 63, 64);
+        const uint64_t some = __ballot(w > 0.0), past = __ballot(w > 0.0 && run > target);
+        const int slice = past ? __ffsll((unsigned long long)past) - 1 : some ? 63 - __clzll((long long)some) : 0;
+        const double before = __shfl(run - w, slice, 64);
+        if (lane == 0) {
+            slice_s = 2 * slice + of;
+            target_s = target - before;
+            pick_s = INT32_MAX;
+            last_s = -1;
         }
-        const double target = (double)g.u[r.a + r.n - 1] * total;
-        double sum = 0.0, before = 0.0;
-        int slice = 0;
-        for (int i = 0; i < g.slices; ++i) {
-            const double w = weight[2 * i + of];
-            if (w > 0.0) {
-                slice = i;
-                before = sum;
-            }
-            sum += w;
-            if (w > 0.0 && sum > target) break;
-        }
-        slice_s = 2 * slice + of;
-        before_s = target - before;
-        pick_s = INT32_MAX;
-        last_s = -1;
     }
+    const Decision c = g.decision[b];
+    const Weights<T, VEC> weights(g, b, r, c);
     __syncthreads();
     const int slice = slice_s >> 1, of = slice_s & 1;
-    const double target = before_s;
-    const int lo = slice * g.per, hi = min(lo + g.per, g.V), mine = g.per / kThreads + 1;
-    const int j0 = min(lo + tid * mine, hi), j1 = min(j0 + mine, hi);
-    double sum = 0.0;
-    for (int j = j0; j < j1; ++j) {
-        double p;
-        const double w = weight_at<BF16>(g, r, c, t, s, x, j, p);
-        sum += of ? p : w;
-    }
-    run[tid] = sum;
-    __syncthreads();
-    double before = 0.0;
-    for (int i = 0; i < tid; ++i) before += run[i];
+    const double target = target_s;
+    const int lo = min(slice * g.cut_per, g.V), hi = min(lo + g.cut_per, g.V);
+    double base = 0.0;
     int pick = INT32_MAX, last = -1;
-    for (int j = j0; j < j1; ++j) {
-        double p;
-        const double w = weight_at<BF16>(g, r, c, t, s, x, j, p), v = of ? p : w;
-        before += v;
-        if (v > 0.0) {
-            last = j;
-            if (before > target && pick == INT32_MAX) pick = j;
+    for (int j0 = lo; j0 < hi; j0 += 8 * kThreads) {
+        const int j = j0 + 8 * tid;
+        double w8[8], p8[8], sum = 0.0;
+        if (j < hi) {
+            weights.get(j, hi, w8, p8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += of ? p8[i] : w8[i];
         }
+        const double run = wave_scan64(sum);
+        if (lane == 63) wave_total[wave] = run;
+        __syncthreads();
+        double before = base + run - sum;
+        for (int w = 0; w < kThreads / 64; ++w) {
+            if (w < wave) before += wave_total[w];
+            base += wave_total[w];
+        }
+        if (j < hi) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const double v = of ? p8[i] : w8[i];
+                before += v;
+                if (v > 0.0) {
+                    last = j + i;
+                    if (before > target && pick == INT32_MAX) pick = j + i;
+                }
+            }
+        }
+        __syncthreads();
+        if (base > target) break;  // by all threads: what follows is behind the token
     }
     if (pick != INT32_MAX) atomicMin(&pick_s, pick);
     if (last >= 0) atomicMax(&last_s, last);
     __syncthreads();
-    const int64_t token = !ok ? -1 : pick_s != INT32_MAX ? pick_s : last_s;
+    const int64_t token = !valid(c.stat) ? -1 : pick_s != INT32_MAX ? pick_s : last_s;
     for (int64_t i = tid; i < r.n; i += kThreads)
         g.out[r.a + i] = i < c.kept ? g.tokens[r.a + i + 1] : i == c.kept ? token : -1;
     if (tid == 0) g.accepted[b] = (int32_t)c.kept;
 }
 
-// Columns of a slice: enough slices to fill the chip, few enough to be joined
-// by one wave in one go.
-int slice_columns(int64_t T, int64_t V) {
-    const int64_t want = std::min<int64_t>(64, std::max<int64_t>(1, 2048 / std::max<int64_t>(T, 1)));
+// Columns of a slice of one of `rows` rows: enough slices to fill the chip, few
+// enough to be joined by one wave in one go (64).
+int slice_columns(int64_t rows, int64_t V) {
+    const int64_t want = std::min<int64_t>(64, std::max<int64_t>(1, 2048 / std::max<int64_t>(rows, 1)));
     const int64_t per = std::max<int64_t>((V + want - 1) / want, 2048);
     return (int)((per + 7) / 8 * 8);
+}
+int64_t slices_of(int64_t V, int per) { return (V + per - 1) / per; }
+
+template <class T, bool VEC>
+hipError_t run(const Args& g, hipStream_t stream) {
+    const dim3 block(kThreads);
+    if (g.T) {
+        hipLaunchKernelGGL((verify_rows_kernel<T, VEC>), dim3((unsigned)g.T, g.slices), block, 0, stream, g);
+        hipLaunchKernelGGL((verify_weigh_kernel<T, VEC>), dim3(g.B, g.cuts), block, 0, stream, g);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((verify_draw_kernel<T, VEC>), dim3(g.B), block, 0, stream, g);
+    return hipGetLastError();
 }
 
 }  // namespace
 
 size_t verify_ws_bytes(int64_t T, int64_t B, int64_t V) {
-    const int64_t per = slice_columns(T, V), slices = (V + per - 1) / per;
-    return (size_t)(T * slices * 16 + B * slices * 16);
+    return (size_t)(T * slices_of(V, slice_columns(T, V)) * 16 + B * slices_of(V, slice_columns(B, V)) * 16 +
+                    B * (int64_t)sizeof(Decision));
 }
 
 hipError_t launch_verify(const void* logits, bool bf16, int64_t ld, const float* probs, int64_t ldp, int64_t prob_rows,
                          const int64_t* tokens, const float* u, const int32_t* offsets, const float* temperature, int64_t T,
                          int B, int V, int32_t* accepted, int64_t* out, void* ws, hipStream_t stream) {
-    const int per = slice_columns(T, V), slices = (V + per - 1) / per;
-    double* sums = static_cast<double*>(ws);
-    double* weight = sums + T * slices;
-    float* row_max = reinterpret_cast<float*>(weight + (int64_t)B * slices * 2);
-    const Args g{logits, ld, probs, ldp, prob_rows, tokens, u, offsets, temperature, B, slices, V, per, T, accepted, out,
-                 sums, row_max, reinterpret_cast<int32_t*>(row_max + T * slices), weight};
+    Args g{};
+    g.logits = logits, g.ld = ld, g.probs = probs, g.ldp = ldp, g.prob_rows = prob_rows;
+    g.tokens = tokens, g.u = u, g.offsets = offsets, g.temperature = temperature;
+    g.B = B, g.V = V, g.T = T, g.accepted = accepted, g.out = out;
+    g.per = slice_columns(T, V), g.slices = (int)slices_of(V, g.per);
+    g.cut_per = slice_columns(B, V), g.cuts = (int)slices_of(V, g.cut_per);
+    g.row_sum = static_cast<double*>(ws);
+    g.weight = g.row_sum + T * g.slices;
+    g.decision = reinterpret_cast<Decision*>(g.weight + (int64_t)B * g.cuts * 2);
+    g.row_max = reinterpret_cast<float*>(g.decision + B);
+    g.row_at = reinterpret_cast<int32_t*>(g.row_max + T * g.slices);
     const bool vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld % (bf16 ? 8 : 4) == 0;
-    const dim3 rows((unsigned)T, slices), requests(B, slices), block(kThreads);
-    if (T) {
-        if (bf16) {
-            if (vec) hipLaunchKernelGGL((verify_rows_kernel<true, true>), rows, block, 0, stream, g);
-            else hipLaunchKernelGGL((verify_rows_kernel<true, false>), rows, block, 0, stream, g);
-            hipLaunchKernelGGL(verify_weigh_kernel<true>, requests, block, 0, stream, g);
-        } else {
-            if (vec) hipLaunchKernelGGL((verify_rows_kernel<false, true>), rows, block, 0, stream, g);
-            else hipLaunchKernelGGL((verify_rows_kernel<false, false>), rows, block, 0, stream, g);
-            hipLaunchKernelGGL(verify_weigh_kernel<false>, requests, block, 0, stream, g);
-        }
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    if (bf16) hipLaunchKernelGGL(verify_draw_kernel<true>, dim3(B), block, 0, stream, g);
-    else hipLaunchKernelGGL(verify_draw_kernel<false>, dim3(B), block, 0, stream, g);
-    return hipGetLastError();
+    return bf16 ? (vec ? run<uint16_t, true>(g, stream) : run<uint16_t, false>(g, stream))
+                : (vec ? run<float, true>(g, stream) : run<float, false>(g, stream));
 }
 
 }  // namespace fp8lin
