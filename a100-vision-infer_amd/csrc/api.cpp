@@ -1049,8 +1049,8 @@ int fp8lin_decode_chain(const fp8lin_chain_link* links, int nlinks, void* worksp
     });
 }
 
-size_t fp8lin_paged_layout_workspace_bytes(int64_t requests) {
-    return requests > 0 && requests <= FP8LIN_PAGED_MAX_REQUESTS ? fp8lin::paged_layout_ws_bytes(requests) : 0;
+size_t fp8lin_paged_layout_workspace_bytes(int64_t requests, int in_place) {
+    return requests > 0 && requests <= FP8LIN_PAGED_MAX_REQUESTS ? fp8lin::paged_layout_ws_bytes(requests, in_place != 0) : 0;
 }
 
 int fp8lin_paged_layout(const int32_t* lengths, const int32_t* counts, const int32_t* table, int64_t table_ld,
@@ -1068,7 +1068,7 @@ int fp8lin_paged_layout(const int32_t* lengths, const int32_t* counts, const int
                 "paged layout: invalid table strides or free list");
         require(new_table != table || new_table_ld == table_ld, FP8LIN_ERR_ARGUMENT,
                 "paged layout: a table written in place keeps its stride");
-        check_workspace(workspace, workspace_bytes, fp8lin::paged_layout_ws_bytes(requests), "paged layout: workspace too small");
+        check_workspace(workspace, workspace_bytes, fp8lin::paged_layout_ws_bytes(requests, new_table == table), "paged layout: workspace too small");
         ensure_device();
         check_hip(fp8lin::launch_paged_layout(lengths, counts, table, table_ld, free_pages, free_count, cursor, (int)requests,
                                               (int)width, page_bits(page_size), tokens, offsets, new_lengths, slots, positions,

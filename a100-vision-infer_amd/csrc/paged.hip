@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256) void append_kernel(Append a) {
 
 }  // namespace
 
-size_t paged_layout_ws_bytes(int64_t B) { return (size_t)(8 * B); }
+size_t paged_layout_ws_bytes(int64_t B, bool in_place) { return in_place || B > kScanRequests ? (size_t)(8 * B) : 0; }
 
 hipError_t launch_paged_layout(const int32_t* lengths, const int32_t* counts, const int32_t* table, int64_t ldt,
                                const int32_t* free_pages, int64_t free_count, const int32_t* cursor, int B, int width,

@@ -48,7 +48,7 @@ hipError_t launch_paged_layout(const int32_t* lengths, const int32_t* counts, co
                                int page_bits, int64_t T, int32_t* offsets, int32_t* new_lengths, int64_t* slots,
                                int64_t* positions, int32_t* new_table, int64_t ldn, int32_t* new_cursor, int32_t* ws,
                                hipStream_t stream);
-size_t paged_layout_ws_bytes(int64_t B);
+size_t paged_layout_ws_bytes(int64_t B, bool in_place);
 
 // ---- the split of an attention launch over its workgroups -------------------
 //

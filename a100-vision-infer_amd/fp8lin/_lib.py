@@ -168,7 +168,7 @@ def lib():
                                                                  ctypes.POINTER(Weight), i64]),
         "fp8lin_engine_linear_candidates": (i32, [ctypes.POINTER(LinearOptions), ctypes.POINTER(Weight), vp,
                                                   i64, i64, vp, vp, sz, ctypes.POINTER(ctypes.c_int), vp]),
-        "fp8lin_paged_layout_workspace_bytes": (sz, [i64]),
+        "fp8lin_paged_layout_workspace_bytes": (sz, [i64, i32]),
         "fp8lin_paged_layout": (i32, [vp, vp, vp, i64, vp, i64, vp, i64, i64, i64, i64, vp, vp, vp, vp, vp, i64, vp, vp,
                                       sz, vp]),
         "fp8lin_paged_append": (i32, [ctypes.POINTER(PagedCacheRecord), vp, i64, i64, vp, i64, i64, vp, i64, vp]),

@@ -561,14 +561,14 @@ typedef struct fp8lin_paged_cache {
  *       page (none left, a negative id, a position past the table); rows from
  *       offsets[requests] on: slot -1, position 0; rows past `tokens` are dropped;
  *   new_table [requests, width]  the table with the pages taken, which may be
- *       `table` itself (and may overlap no other argument);
+ *       `table` itself (in_place; it may overlap no other argument);
  *   new_cursor [1]  cursor + pages wanted: above free_count, the list was short.
  * Page ids are not checked here; fp8lin_paged_append and
  * fp8lin_paged_attention check them.  0 < requests <= 4096; width * page_size
  * <= 2^30.
  */
 #define FP8LIN_PAGED_MAX_REQUESTS 4096
-size_t fp8lin_paged_layout_workspace_bytes(int64_t requests);
+size_t fp8lin_paged_layout_workspace_bytes(int64_t requests, int in_place);
 int fp8lin_paged_layout(const int32_t* lengths, const int32_t* counts, const int32_t* table, int64_t table_ld,
                         const int32_t* free_pages, int64_t free_count, const int32_t* cursor, int64_t requests,
                         int64_t width, int64_t page_size, int64_t tokens, int32_t* offsets, int32_t* new_lengths,
