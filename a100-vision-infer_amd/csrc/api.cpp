@@ -1130,9 +1130,6 @@ int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, i
         check_workspace(workspace, workspace_bytes, fp8lin::paged_attention_ws_bytes((int)cache->head_dim, rows),
                         "paged attention: workspace too small");
         ensure_device();
-        auto on = [](const void* p, int64_t s0, int64_t s1, int64_t elements) {
-            return reinterpret_cast<uintptr_t>(p) % (2 * elements) == 0 && s0 % elements == 0 && s1 % elements == 0;
-        };
         a.q = q, a.gate = gate, a.out = out;
         a.q_tok = q_token, a.q_head = q_head, a.g_tok = gate_token, a.g_head = gate_head;
         a.o_tok = out_token, a.o_head = out_head;
@@ -1142,8 +1139,6 @@ int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, i
         a.B = (int)requests, a.T = (int)tokens, a.H = (int)heads, a.HK = (int)cache->kv_heads;
         a.G = a.H / a.HK;
         a.causal = causal != 0;
-        a.q_vec = on(q, q_token, q_head, 8), a.g_vec = on(gate, gate_token, gate_head, 4);
-        a.o_vec = on(out, out_token, out_head, 4);
         a.scale2 = (float)scale2;
         a.ws = static_cast<float*>(workspace);
         check_hip(fp8lin::launch_paged_attention(a, (int)cache->head_dim, cache->fp8 != 0, rows, as_stream(stream)),

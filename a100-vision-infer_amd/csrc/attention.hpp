@@ -73,51 +73,128 @@ __device__ __forceinline__ bf16x8 codes8_bf16(uint32_t lo, uint32_t hi) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// N fragments of 8 values of a query row, from elements at(t) (16 bytes when
-// the rows start on them); zeros for a row past the tile, whose pointer is
-// that of some row.  Loaded without a condition, so that all are in flight.
+// 16 and 8 bytes at any BF16 element: gfx950 takes unaligned global accesses,
+// so operands off the 16-byte grid need no other path.
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+typedef u32x2 __attribute__((aligned(2))) u32x2_any;
+
+// N fragments of 8 values of a query row, from elements at(t).  A row past the
+// tile gives those of some row: its scores and sums stay in its own lanes, and
+// it is not written.
 template <int N, class AT>
-__device__ __forceinline__ void load_queries(const PagedAttention& a, const uint16_t* row, bool valid, bf16x8 (&qf)[N], AT at) {
-    u32x4 v[N];
-    if (a.q_vec) {
+__device__ __forceinline__ void load_queries(const uint16_t* row, bf16x8 (&qf)[N], AT at) {
 #pragma unroll
-        for (int t = 0; t < N; ++t) v[t] = load_u32x4(row + at(t));
-    } else {
-#pragma unroll
-        for (int t = 0; t < N; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[t][i] = (uint32_t)row[at(t) + 2 * i] | (uint32_t)row[at(t) + 2 * i + 1] << 16;
-    }
-#pragma unroll
-    for (int t = 0; t < N; ++t) qf[t] = __builtin_bit_cast(bf16x8, valid ? v[t] : u32x4{0, 0, 0, 0});
+    for (int t = 0; t < N; ++t) qf[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_any*>(row + at(t)));
 }
 
+__device__ __forceinline__ u32x2 load_gate4(const uint16_t* g) { return *reinterpret_cast<const u32x2_any*>(g); }
+// o * sigmoid(gate) by the hardware's 2^x and reciprocal, a few units of FP32
+// off; a gate of -inf gives 0, whatever o is short of NaN.
+__device__ __forceinline__ void apply_gate(f32x4& o, u32x2 gv) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = bf16_bits_to_f32(((i < 2 ? gv.x : gv.y) >> (16 * (i & 1))) & 0xffffu);
+        o[i] *= __builtin_amdgcn_rcpf(1.0f + exp2_fast(x * -1.44269504088896340736f));
+    }
+}
+// The same of N groups of 4: a value's chain of six instructions waits on each,
+// so all values take each step together.
+template <int N>
+__device__ __forceinline__ void apply_gates(f32x4 (&o)[N], const u32x2 (&gv)[N]) {
+    float e[4 * N];
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) {
+        const u32x2 w = gv[i / 4];
+        e[i] = exp2_fast(-1.44269504088896340736f * bf16_bits_to_f32(((i % 4 < 2 ? w.x : w.y) >> (16 * (i & 1))) & 0xffffu));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) e[i] = __builtin_amdgcn_rcpf(1.0f + e[i]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) o[i / 4][i % 4] *= e[i];
+}
+__device__ __forceinline__ void store_bf16x4(uint16_t* y, f32x4 o) {
+    *reinterpret_cast<u32x2_any*>(y) = u32x2{pack_bf16x2(f32x2{o.x, o.y}), pack_bf16x2(f32x2{o.z, o.w})};
+}
 // out[d .. d+3] = bf16(o * sigmoid(gate)): one rounding.
 __device__ __forceinline__ void store4(const PagedAttention& a, int64_t tok, int head, int d, f32x4 o) {
-    if (a.gate) {
-        const uint16_t* g = a.gate + tok * a.g_tok + head * a.g_head + d;
-        u32x2 gv;
-        if (a.g_vec) {
-            gv = *reinterpret_cast<const u32x2*>(g);
-        } else {
-            gv.x = (uint32_t)g[0] | (uint32_t)g[1] << 16;
-            gv.y = (uint32_t)g[2] | (uint32_t)g[3] << 16;
-        }
+    if (a.gate) apply_gate(o, load_gate4(a.gate + tok * a.g_tok + head * a.g_head + d));
+    store_bf16x4(a.out + tok * a.o_tok + head * a.o_head + d, o);
+}
+
+// The result of a 32-row MFMA tile from O^T in registers (lane: row lane & 31,
+// dimensions 32 dt + 8 b + 4 (lane >> 5) ..): through this wave's part of LDS,
+// kStoreRows rows of it at a time, so that gates and results move as whole
+// rows.  (Straight from the registers, 8 bytes per row and instruction, two
+// 32 x 256 tiles took 30 us.)  flat: the tile's first row (token * G + head),
+// rows: how many it has.  A loop, so that its registers stay few: the kernels'
+// accumulators are live here.
+constexpr int kStoreRows = 16;
+template <int D>
+constexpr int store_bytes() { return kStoreRows * (D + 4) * 4; }
+template <int D>
+__device__ __forceinline__ void store_tile(const PagedAttention& a, float* buf, const f32x16 (&o)[D / 32], float inv, int off,
+                                           int hk, int flat, int rows) {
+    constexpr int LD = D + 4, LANES = D / 4, PER = 64 / LANES;  // lanes of a row, rows of an instruction
+    constexpr int N = kStoreRows / PER;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, tok = (flat + col) / a.G;
+    const int64_t head = hk * a.G + (flat + col) - tok * a.G;
+    const int64_t at_o = (off + tok) * a.o_tok + head * a.o_head, at_g = (off + tok) * a.g_tok + head * a.g_head;
+    const int d = 4 * (lane % LANES), sub = lane / LANES;
+    // without a condition per row (some row of the tile), so that all are in flight
+    u32x2 next[N];
+    auto load = [&](int row0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = bf16_bits_to_f32(((i < 2 ? gv.x : gv.y) >> (16 * (i & 1))) & 0xffffu);
-            o[i] /= 1.0f + expf(-x);
+        for (int i = 0; i < N; ++i)
+            next[i] = load_gate4(a.gate + __shfl(at_g, min(row0 + i * PER + sub, rows - 1), 64) + d);
+    };
+    if (a.gate && rows > 0) load(0);
+#pragma unroll 1
+    for (int row0 = 0; row0 < min(rows, 32); row0 += kStoreRows) {
+        __builtin_amdgcn_sched_barrier(0);
+        wait_lgkm<0>();  // other lanes' rows: the compiler may not move reads over the writes
+        if ((unsigned)(col - row0) < (unsigned)kStoreRows) {
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    f32x4 x;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = inv == 0.0f ? 0.0f : o[dt][4 * b + i] * inv;
+                    *reinterpret_cast<f32x4*>(buf + (col - row0) * LD + 32 * dt + 8 * b + 4 * half) = x;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-    }
-    uint16_t* y = a.out + tok * a.o_tok + head * a.o_head + d;
-    const uint32_t lo = pack_bf16x2(f32x2{o.x, o.y}), hi = pack_bf16x2(f32x2{o.z, o.w});
-    if (a.o_vec) {
-        *reinterpret_cast<u32x2*>(y) = u32x2{lo, hi};
-    } else {
-        y[0] = (uint16_t)lo;
-        y[1] = (uint16_t)(lo >> 16);
-        y[2] = (uint16_t)hi;
-        y[3] = (uint16_t)(hi >> 16);
+        wait_lgkm<0>();
+        u32x2 g[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = next[i];
+        if (a.gate && row0 + kStoreRows < rows) load(row0 + kStoreRows);
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int BATCH = N < 8 ? N : 8;
+#pragma unroll
+        for (int i0 = 0; i0 < N; i0 += BATCH) {
+            f32x4 x[BATCH];
+            int64_t to[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int r = (i0 + i) * PER + sub;
+                x[i] = *reinterpret_cast<const f32x4*>(buf + r * LD + d);
+                to[i] = __shfl(at_o, row0 + r, 64) + d;
+            }
+            if (a.gate) {
+                u32x2 gb[BATCH];
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) gb[i] = g[i0 + i];
+                apply_gates<BATCH>(x, gb);
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i)
+                if (row0 + (i0 + i) * PER + sub < rows) store_bf16x4(a.out + to[i], x[i]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 }
 
@@ -139,6 +216,7 @@ struct Partial {
 };
 
 hipError_t launch_few(const PagedAttention& a, int D, bool fp8, int rows, hipStream_t stream);
+hipError_t launch_wide(const PagedAttention& a, hipStream_t stream);  // D 256, BF16
 hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t stream);
 
 // Joins the pieces of the units that the boundaries between workgroups cut,
@@ -184,6 +262,9 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
         int row, d;
         ORDER::place(e, row, d);
         const bool ok = row < nr;
+        const int flat = r0 + min(row, nr - 1), tok = off + flat / a.G, head = u.y * a.G + flat % a.G;
+        u32x2 gate = {0, 0};
+        if (a.gate) gate = load_gate4(a.gate + tok * a.g_tok + head * a.g_head + d);
         // the unit's pieces: workgroups w - 1 (slot 1), w, .. last (slot 0)
         const int last = unit_last[item / PARTS];
         float M = -__builtin_inff(), l = 0.0f;
@@ -233,11 +314,22 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
             const float inv = l == 0.0f ? 0.0f : (a.v_scale ? a.v_scale[u.y] : 1.0f) / l;
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : o[i] * inv;
-            const int flat = r0 + row;
-            store4(a, off + flat / a.G, u.y * a.G + flat % a.G, d, o);
+            if (a.gate) apply_gate(o, gate);
+            store_bf16x4(a.out + tok * a.o_tok + head * a.o_head + d, o);
         }
     }
 }
+
+// The order of O in the partial sums of the kernels with 32 rows per MFMA tile:
+// as their registers hold it.
+template <int D>
+struct TileOrder {
+    static __device__ __forceinline__ void place(int e, int& row, int& d) {
+        const int lane = e & 63, b = (e >> 6) & 3, dt = (e >> 8) % (D / 32), wave = (e >> 8) / (D / 32);
+        row = 32 * wave + (lane & 31);
+        d = 32 * dt + 8 * b + 4 * (lane >> 5);
+    }
+};
 
 }  // namespace attn
 }  // namespace fp8lin

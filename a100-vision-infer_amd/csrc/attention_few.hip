@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                 const int row = 16 * nt + col, flat = r0 + row, tok = flat / a.G;
                 const bool ok = row < nr;
                 const uint16_t* q = a.q + (int64_t)(s.off + (ok ? tok : 0)) * a.q_tok + (int64_t)(cur.hk * a.G + flat % a.G) * a.q_head;
-                load_queries<D / 32>(a, q, ok, qf[nt], [&](int t) { return 32 * (t & ~1) + 16 * quad + 8 * (t & 1); });
+                load_queries<D / 32>(q, qf[nt], [&](int t) { return 32 * (t & ~1) + 16 * quad + 8 * (t & 1); });
                 lim[nt] = !ok ? 0 : a.causal ? min(max(s.len - s.n + tok + 1, 0), s.len) : s.len;
             }
             // the fewest keys that a row of the tile may see: tiles below need no mask

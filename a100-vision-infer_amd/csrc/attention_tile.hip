@@ -83,7 +83,7 @@ __global__ __launch_bounds__(64 * W, 1) void tile_kernel(PagedAttention a) {
             bf16x8 qf[D / 16];  // B operand: row col, dimensions 16 t + 8 half ..
             {
                 const uint16_t* q = a.q + (int64_t)(s.off + (ok ? tok : 0)) * a.q_tok + (int64_t)(cur.hk * a.G + flat % a.G) * a.q_head;
-                load_queries<D / 16>(a, q, ok, qf, [&](int t) { return 16 * t + 8 * half; });
+                load_queries<D / 16>(q, qf, [&](int t) { return 16 * t + 8 * half; });
             }
             const int ctx = s.len - s.n;
             const int lim = !ok ? 0 : a.causal ? min(max(ctx + tok + 1, 0), s.len) : s.len;
@@ -251,18 +251,9 @@ __global__ __launch_bounds__(64 * W, 1) void tile_kernel(PagedAttention a) {
             l += __shfl_xor(l, 32, 64);
 
             if (k0 == 0 && k1 == nkt) {
-                if (ok) {
-                    const float inv = l == 0.0f ? 0.0f : (F8 ? a.v_scale[cur.hk] : 1.0f) / l;
-#pragma unroll
-                    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-                        for (int b = 0; b < 4; ++b) {
-                            f32x4 x;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) x[i] = l == 0.0f ? 0.0f : o[dt][4 * b + i] * inv;
-                            store4(a, s.off + tok, cur.hk * a.G + flat % a.G, 32 * dt + 8 * b + 4 * half, x);
-                        }
-                }
+                __syncthreads();
+                store_tile<D>(a, reinterpret_cast<float*>(lds + wave * store_bytes<D>()), o,
+                              l == 0.0f ? 0.0f : (F8 ? a.v_scale[cur.hk] : 1.0f) / l, s.off, cur.hk, r0 + 32 * wave, nr - 32 * wave);
             } else if (busy) {
                 float* part = Partial<BM, D>::at(a.ws, group, k0 == 0);
 #pragma unroll
@@ -293,18 +284,9 @@ __global__ __launch_bounds__(64 * W, 1) void tile_kernel(PagedAttention a) {
     }
 }
 
-template <int D>
-struct TileOrder {
-    static __device__ __forceinline__ void place(int e, int& row, int& d) {
-        const int lane = e & 63, b = (e >> 6) & 3, dt = (e >> 8) % (D / 32), wave = (e >> 8) / (D / 32);
-        row = 32 * wave + (lane & 31);
-        d = 32 * dt + 8 * b + 4 * (lane >> 5);
-    }
-};
-
 template <int D, bool F8, int W>
 hipError_t run(const PagedAttention& a, hipStream_t stream) {
-    constexpr int BM = 32 * W, LDS = std::max<int>(Tile<D>::LDS, PagedSplit<BM, kTileKeys, 0>::lds_bytes(kPagedMaxRequests));
+    constexpr int BM = 32 * W, LDS = std::max<int>({Tile<D>::LDS, PagedSplit<BM, kTileKeys, 0>::lds_bytes(kPagedMaxRequests), W * store_bytes<D>()});
     auto* kern = tile_kernel<D, F8, W>;
     static const hipError_t attr =
         hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -313,7 +295,7 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     auto* join = join_kernel<BM, D, 1, TileOrder<D>>;
-    hipLaunchKernelGGL(join, dim3(4 * kGroups), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(join, dim3(8 * kGroups), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
@@ -322,7 +304,7 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
 hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t stream) {
     if (D == 64) return fp8 ? run<64, true, kTileWaves>(a, stream) : run<64, false, kTileWaves>(a, stream);
     if (D == 128) return fp8 ? run<128, true, kTileWaves>(a, stream) : run<128, false, kTileWaves>(a, stream);
-    return fp8 ? run<256, true, kTileWaves>(a, stream) : run<256, false, kTileWaves>(a, stream);
+    return fp8 ? run<256, true, kTileWaves>(a, stream) : launch_wide(a, stream);
 }
 
 }  // namespace attn

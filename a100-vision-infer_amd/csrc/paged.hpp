@@ -25,8 +25,8 @@ struct PagedAttention {
     int64_t ldt;
     int width, page_bits, pages;
     int B, T, H, HK, G;
-    bool causal, q_vec, g_vec, o_vec;  // *_vec: rows start on 16 (q) or 8 bytes
-    float scale2;                      // softmax scale * log2(e)
+    bool causal;
+    float scale2;  // softmax scale * log2(e)
     float* ws;
 };
 
@@ -120,7 +120,7 @@ struct PagedSplit {
     // What a workgroup knows of the batch while it finds its piece, in LDS:
     // prefix[b] = cost of the requests before b, b <= B, then each request's
     // (new tokens, keys).
-    static constexpr size_t lds_bytes(int64_t B) { return (size_t)(16 * B + 16); }
+    static constexpr int lds_bytes(int B) { return 16 * B + 16; }
     static __device__ __forceinline__ int* held(const PagedAttention& a, int64_t* pre) {
         return reinterpret_cast<int*>(pre + a.B + 1);
     }
@@ -201,7 +201,7 @@ struct PagedSplit {
     // Length of a piece: an even share, but no shorter than min_tiles key
     // tiles of a unit.
     static __device__ __forceinline__ int64_t chunk(const PagedAttention& a, int64_t total, int groups, int min_tiles) {
-        return max((total + groups - 1) / groups, (int64_t)min_tiles * BN * a.G);
+        return max(div(total + groups - 1, groups), (int64_t)min_tiles * BN * a.G);
     }
 };
 
