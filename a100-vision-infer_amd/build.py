@@ -20,7 +20,7 @@ OBJ = os.path.join(HERE, "build")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libfp8lin.so")
 SOURCES = ["api.cpp", "gemv.hip", "small_m.hip", "gemm.hip", "gemm_tile.hip", "skinny.hip", "elementwise.hip", "epilogue.hip",
-           "chain.hip", "paged.hip", "attention_few.hip", "attention_tile.hip", "attention_wide.hip", "verify.hip"]
+           "chain.hip", "paged.hip", "attention_few.hip", "attention_tile.hip", "verify.hip"]
 ARCH = "gfx950"
 
 COMMON = [

@@ -32,6 +32,8 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLazy = 8.0f;  // log2 of the largest weight before m moves
 constexpr int kGroups = 256;   // workgroups of a launch at one per CU
+constexpr int kFewRows = 64;   // rows of a request that the few-rows kernel takes
+constexpr int kTileRows = 256;  // rows of a tile of the other
 
 // 64 lanes x 16 B from global (voff, bounds-checked) into LDS [m0v, m0v + 1024).
 // K and V rows that one workgroup reads take the non-temporal policy.
@@ -123,81 +125,6 @@ __device__ __forceinline__ void store4(const PagedAttention& a, int64_t tok, int
     store_bf16x4(a.out + tok * a.o_tok + head * a.o_head + d, o);
 }
 
-// The result of a 32-row MFMA tile from O^T in registers (lane: row lane & 31,
-// dimensions 32 dt + 8 b + 4 (lane >> 5) ..): through this wave's part of LDS,
-// kStoreRows rows of it at a time, so that gates and results move as whole
-// rows.  (Straight from the registers, 8 bytes per row and instruction, two
-// 32 x 256 tiles took 30 us.)  flat: the tile's first row (token * G + head),
-// rows: how many it has.  A loop, so that its registers stay few: the kernels'
-// accumulators are live here.
-constexpr int kStoreRows = 16;
-template <int D>
-constexpr int store_bytes() { return kStoreRows * (D + 4) * 4; }
-template <int D>
-__device__ __forceinline__ void store_tile(const PagedAttention& a, float* buf, const f32x16 (&o)[D / 32], float inv, int off,
-                                           int hk, int flat, int rows) {
-    constexpr int LD = D + 4, LANES = D / 4, PER = 64 / LANES;  // lanes of a row, rows of an instruction
-    constexpr int N = kStoreRows / PER;
-    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, tok = (flat + col) / a.G;
-    const int64_t head = hk * a.G + (flat + col) - tok * a.G;
-    const int64_t at_o = (off + tok) * a.o_tok + head * a.o_head, at_g = (off + tok) * a.g_tok + head * a.g_head;
-    const int d = 4 * (lane % LANES), sub = lane / LANES;
-    // without a condition per row (some row of the tile), so that all are in flight
-    u32x2 next[N];
-    auto load = [&](int row0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            next[i] = load_gate4(a.gate + __shfl(at_g, min(row0 + i * PER + sub, rows - 1), 64) + d);
-    };
-    if (a.gate && rows > 0) load(0);
-#pragma unroll 1
-    for (int row0 = 0; row0 < min(rows, 32); row0 += kStoreRows) {
-        __builtin_amdgcn_sched_barrier(0);
-        wait_lgkm<0>();  // other lanes' rows: the compiler may not move reads over the writes
-        if ((unsigned)(col - row0) < (unsigned)kStoreRows) {
-#pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    f32x4 x;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = inv == 0.0f ? 0.0f : o[dt][4 * b + i] * inv;
-                    *reinterpret_cast<f32x4*>(buf + (col - row0) * LD + 32 * dt + 8 * b + 4 * half) = x;
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        wait_lgkm<0>();
-        u32x2 g[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = next[i];
-        if (a.gate && row0 + kStoreRows < rows) load(row0 + kStoreRows);
-        __builtin_amdgcn_sched_barrier(0);
-        constexpr int BATCH = N < 8 ? N : 8;
-#pragma unroll
-        for (int i0 = 0; i0 < N; i0 += BATCH) {
-            f32x4 x[BATCH];
-            int64_t to[BATCH];
-#pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                const int r = (i0 + i) * PER + sub;
-                x[i] = *reinterpret_cast<const f32x4*>(buf + r * LD + d);
-                to[i] = __shfl(at_o, row0 + r, 64) + d;
-            }
-            if (a.gate) {
-                u32x2 gb[BATCH];
-#pragma unroll
-                for (int i = 0; i < BATCH; ++i) gb[i] = g[i0 + i];
-                apply_gates<BATCH>(x, gb);
-            }
-#pragma unroll
-            for (int i = 0; i < BATCH; ++i)
-                if (row0 + (i0 + i) * PER + sub < rows) store_bf16x4(a.out + to[i], x[i]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-}
-
 // The workspace: where each workgroup's piece begins (request, kv head, row
 // tile, key tile; request -1: no piece; the request's first row, the tile's
 // rows), then the partial sums of split units:
@@ -216,7 +143,6 @@ struct Partial {
 };
 
 hipError_t launch_few(const PagedAttention& a, int D, bool fp8, int rows, hipStream_t stream);
-hipError_t launch_wide(const PagedAttention& a, hipStream_t stream);  // D 256, BF16
 hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t stream);
 
 // Joins the pieces of the units that the boundaries between workgroups cut,

@@ -25,6 +25,7 @@ struct PagedAttention {
     int64_t ldt;
     int width, page_bits, pages;
     int B, T, H, HK, G;
+    int64_t rows_from, rows_to;  // requests of rows_from < new tokens * G <= rows_to are computed, others left
     bool causal;
     float scale2;  // softmax scale * log2(e)
     float* ws;
@@ -37,7 +38,7 @@ constexpr int kPagedMinPage = 16;
 // (the most rows, tokens times heads per kv head, that a request should
 // bring) selects; the workspace that goes with them.
 size_t paged_attention_ws_bytes(int D, int64_t max_rows);
-hipError_t launch_paged_attention(const PagedAttention& a, int D, bool fp8, int64_t max_rows, hipStream_t stream);
+hipError_t launch_paged_attention(PagedAttention a, int D, bool fp8, int64_t max_rows, hipStream_t stream);
 
 hipError_t launch_paged_append(const uint16_t* k, const uint16_t* v, int64_t k_tok, int64_t k_head, int64_t v_tok,
                                int64_t v_head, const int64_t* slots, const PagedCache& kc, const PagedCache& vc, bool fp8,
@@ -68,6 +69,8 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttention& a, int b) {
     int lo = a.offsets[b], hi = a.offsets[b + 1];
     lo = min(max(lo, 0), a.T);
     hi = min(max(hi, lo), a.T);
+    const int64_t rows = (int64_t)(hi - lo) * a.G;
+    if (rows <= a.rows_from || rows > a.rows_to) hi = lo;
     const int64_t cap = (int64_t)a.width << a.page_bits;
     const int64_t len = min((int64_t)max(a.lengths[b], 0), cap);
     return PagedSeq{lo, hi - lo, (int)len};
