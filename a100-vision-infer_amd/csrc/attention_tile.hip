@@ -43,7 +43,9 @@ namespace {
 #define RBS 1
 #endif
 constexpr int kBM = kTileRows, kBN = 64, kKeys = 16;  // kKeys: keys of a tile that a wave brings
-constexpr int kTileStart = 448;    // a unit's start and end, in keys (up to 30 us at 64 keys in 4 us, heads of 256)
+// A unit's start and end, in keys (heads of 256: up to 30 us at 64 keys in 4 us).
+template <int D>
+constexpr int kTileStart = 448 * D / 256;
 constexpr int kTileMinTiles = 4;
 
 template <int D, bool F8>
@@ -127,7 +129,7 @@ template <int D, bool F8, int RB>
 __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(PagedAttention a) {
     constexpr int W = kBM / (32 * RB);  // waves
     using L = Tile<D, F8>;
-    using Split = PagedSplit<kBM, kBN, kTileStart>;
+    using Split = PagedSplit<kBM, kBN, kTileStart<D>>;
     extern __shared__ __align__(1024) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = lane >> 5, col = lane & 31;
@@ -558,10 +560,11 @@ hipError_t launch_paged_attention(PagedAttention a, int D, bool fp8, int64_t max
     a.rows_to = INT64_MAX;
     if (max_rows <= attn::kFewRows) return attn::launch_few(a, D, fp8, (int)max_rows, stream);
     if (a.B > 1) {
-        a.rows_to = attn::kFewRows;
-        const hipError_t e = attn::launch_few(a, D, fp8, attn::kFewRows, stream);
+        constexpr int kSmall = 32;  // rows: decoding requests and drafted tokens of most head layouts
+        a.rows_to = kSmall;
+        const hipError_t e = attn::launch_few(a, D, fp8, kSmall, stream);
         if (e != hipSuccess) return e;
-        a.rows_from = attn::kFewRows;
+        a.rows_from = kSmall;
         a.rows_to = INT64_MAX;
     }
     return attn::launch_tile(a, D, fp8, stream);
