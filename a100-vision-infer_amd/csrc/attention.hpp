@@ -125,14 +125,93 @@ __device__ __forceinline__ void store4(const PagedAttention& a, int64_t tok, int
     store_bf16x4(a.out + tok * a.o_tok + head * a.o_head + d, o);
 }
 
-// The workspace: where each workgroup's piece begins (request, kv head, row
-// tile, key tile; request -1: no piece; the request's first row, the tile's
-// rows), then the partial sums of split units:
-// O (BM x D floats, the kernel's own order), m and l of the BM rows.  A
-// workgroup leaves at most two: slot 0 for the piece that begins inside a unit
-// (its first), slot 1 for the one that begins a unit (its last).
+// Whether the values of keys first, first + step, .. < last hold an infinity or
+// NaN (on the lane that sees one), by a wave.
+template <int D, bool F8>
+__device__ __forceinline__ bool odd_values(const PagedAttention& a, const int32_t* table, int hk, int first, int last, int step) {
+    constexpr int LANES = D / 4, PER = 64 / LANES;  // 4 dimensions a lane, keys at once
+    const int lane = threadIdx.x & 63, d = 4 * (lane % LANES);
+    bool odd = false;
+#pragma unroll 4
+    for (int k = first; k < last; k += step * PER) {
+        const int key = min(k + step * (lane / LANES), last - 1), id = table[key >> a.page_bits];
+        const bool there = (unsigned)id < (unsigned)a.pages;
+        const int64_t at = (int64_t)(there ? id : 0) * a.v.page + (int64_t)(key & ((1 << a.page_bits) - 1)) * a.v.slot + hk * a.v.head + d;
+        if constexpr (F8) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v.data) + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd |= there && ((w >> (8 * i)) & 0x7fu) == 0x7fu;
+        } else {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.v.data) + at);
+            odd |= there && ((w.x & 0x7f80u) == 0x7f80u || (w.x & 0x7f800000u) == 0x7f800000u || (w.y & 0x7f80u) == 0x7f80u ||
+                             (w.y & 0x7f800000u) == 0x7f800000u);
+        }
+    }
+    return odd;
+}
+
+// One row by plain FP32 sums, a key at a time, by a wave: for the rows near
+// values that only some rows may see and that are infinities or NaN, which the
+// matrix product would carry, as 0 * inf, into the other rows of its tile.
+template <int D, bool F8>
+__device__ void plain_row(const PagedAttention& a, const PagedSeq& s, int b, int hk, int flat) {
+    constexpr int LANES = D / 4;  // 4 dimensions a lane
+    const int lane = threadIdx.x & 63, d = 4 * (lane % LANES);
+    const int32_t* table = a.table + (int64_t)b * a.ldt;
+    const float c = a.scale2 * (F8 ? a.k_scale[hk] : 1.0f);
+    auto value4 = [&](const PagedCache& cache, int id, int key) {
+        f32x4 x = {0, 0, 0, 0};
+        if ((unsigned)id >= (unsigned)a.pages) return x;
+        const int64_t at = (int64_t)id * cache.page + (int64_t)(key & ((1 << a.page_bits) - 1)) * cache.slot + hk * cache.head + d;
+        if constexpr (F8) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(cache.data) + at);
+            const f32x2 lo = fp8x2_to_f32<false>(w), hi = fp8x2_to_f32<true>(w);
+            x = f32x4{lo.x, lo.y, hi.x, hi.y};
+        } else {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(cache.data) + at);
+            x = f32x4{bf16_bits_to_f32(w.x & 0xffffu), bf16_bits_to_f32(w.x >> 16), bf16_bits_to_f32(w.y & 0xffffu),
+                      bf16_bits_to_f32(w.y >> 16)};
+        }
+        return x;
+    };
+    const int tok = flat / a.G, head = hk * a.G + flat % a.G;
+    const int lim = a.causal ? min(max(s.len - s.n + tok + 1, 0), s.len) : s.len;
+    const uint16_t* q = a.q + (int64_t)(s.off + tok) * a.q_tok + (int64_t)head * a.q_head + d;
+    float m = -__builtin_inff(), l = 0.0f;
+    f32x4 qv, o = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) qv[i] = bf16_bits_to_f32(q[i]);
+    for (int key = 0; key < lim; ++key) {
+        const int id = table[key >> a.page_bits];
+        const f32x4 k = value4(a.k, id, key), v = value4(a.v, id, key);
+        float x = lane < LANES ? qv.x * k.x + qv.y * k.y + qv.z * k.z + qv.w * k.w : 0.0f;
+        x = wave_sum(x) * c;
+        const float mn = fmaxf(m, x), ms = mn == -__builtin_inff() ? 0.0f : mn;
+        const float f = m == -__builtin_inff() ? 0.0f : exp2_fast(m - ms), p = exp2_fast(x - ms);
+        l = l * f + p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = (f == 0.0f ? 0.0f : o[i] * f) + p * v[i];
+        m = mn;
+    }
+    const float inv = l == 0.0f ? 0.0f : (F8 ? a.v_scale[hk] : 1.0f) / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : o[i] * inv;
+    if (lane < LANES) store4(a, s.off + tok, head, d, o);
+}
+
+// The workspace: per workgroup where its piece begins (request, kv head, row
+// tile, key tile; request -1: no piece), the request's first row and the tile's
+// rows, and for each wave whether it met values that only some of its rows may
+// see and that are no finite numbers; then the partial sums of split units: O
+// (BM x D floats, the kernel's own order), m and l of the BM rows.  A workgroup
+// leaves at most two: slot 0 for the piece that begins inside a unit (its
+// first), slot 1 for the one that begins a unit (its last).
 typedef int i32x4v __attribute__((ext_vector_type(4)));
-constexpr int kBeginFloats = kGroups * 8;
+constexpr int kBeginInts = 16, kBeginFloats = kGroups * kBeginInts;
+__device__ __forceinline__ i32x4v* begin_of(float* ws, int group) { return reinterpret_cast<i32x4v*>(ws + group * kBeginInts); }
+__device__ __forceinline__ int* bad_of(float* ws, int group, int wave) {
+    return reinterpret_cast<int*>(ws + group * kBeginInts + 8) + wave;
+}
 template <int BM, int D>
 struct Partial {
     static constexpr int64_t kFloats = (int64_t)BM * D + 2 * BM;
@@ -150,8 +229,9 @@ hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t str
 // pieces' beginnings and takes every gridDim.x-th part of them: 64 (WAVES 4:
 // its waves share the pieces of a unit, which are many and small in a decode
 // step) or 256 (WAVES 1) groups of 4 values.  ORDER::place(e, row, d): row and
-// first dimension of the e-th 4 floats of a piece's O.
-template <int BM, int D, int WAVES, class ORDER>
+// first dimension of the e-th 4 floats of a piece's O.  The units of workgroups
+// with marked waves are computed again, row by row, instead.
+template <int BM, int D, bool F8, int WAVES, class ORDER>
 __global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
     constexpr int PER = 256 / WAVES, PARTS = BM * D / 4 / PER;
     __shared__ i32x4v begin[kGroups], rows[kGroups];
@@ -160,9 +240,15 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
     __shared__ float sm[WAVES][PER], sl[WAVES][PER];
     static_assert(kGroups == 256, "a thread per piece");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    begin[tid] = reinterpret_cast<const i32x4v*>(a.ws)[2 * tid];
-    rows[tid] = reinterpret_cast<const i32x4v*>(a.ws)[2 * tid + 1];
-    __syncthreads();
+    __shared__ uint8_t bad[kGroups];
+    {
+        const i32x4v* at = begin_of(a.ws, tid);
+        begin[tid] = at[0];
+        rows[tid] = at[1];
+        const i32x4v x = at[2], y = at[3];
+        bad[tid] = begin[tid].x >= 0 && (x.x | x.y | x.z | x.w | y.x | y.y | y.z | y.w);
+    }
+    const bool any_bad = __syncthreads_or(bad[tid]);
     auto same = [](const i32x4v& x, const i32x4v& y) { return x.x == y.x && x.y == y.y && x.z == y.z; };
     // the first boundary inside a unit
     const i32x4v mine = begin[tid];
@@ -193,6 +279,11 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
         if (a.gate) gate = load_gate4(a.gate + tok * a.g_tok + head * a.g_head + d);
         // the unit's pieces: workgroups w - 1 (slot 1), w, .. last (slot 0)
         const int last = unit_last[item / PARTS];
+        if (any_bad) {
+            bool skip = false;
+            for (int g = w - 1; g <= last; ++g) skip |= bad[g] != 0;
+            if (skip) continue;
+        }
         float M = -__builtin_inff(), l = 0.0f;
         f32x4 o = {0, 0, 0, 0};
         auto add = [&](float m1, float l1, f32x4 o1) {
@@ -242,6 +333,30 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
             for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : o[i] * inv;
             if (a.gate) apply_gate(o, gate);
             store_bf16x4(a.out + tok * a.o_tok + head * a.o_head + d, o);
+        }
+    }
+    if (any_bad) {
+        using Split = PagedSplit<BM, 16, 0>;
+        for (int g = 0; g < kGroups; ++g) {
+            if (!bad[g]) continue;
+            const i32x4v last = g + 1 < kGroups ? begin[g + 1] : i32x4v{-1, 0, 0, 0};
+            for (i32x4v u = begin[g]; u.x < a.B;) {
+                const bool end = last.x >= 0 && same(u, last);
+                if (end && last.w == 0) break;
+                const PagedSeq s = paged_seq(a, u.x);
+                const int R = Split::tiles(a, s), r0 = u.z * BM;
+                if (u.z < R)
+                    for (int r = blockIdx.x * 4 + wave; r < (int)min((int64_t)BM, (int64_t)s.n * a.G - r0); r += 4 * gridDim.x)
+                        plain_row<D, F8>(a, s, u.x, u.y, r0 + r);
+                if (end) break;
+                if (++u.z >= R) {
+                    u.z = 0;
+                    if (++u.y >= a.HK) {
+                        u.y = 0;
+                        ++u.x;
+                    }
+                }
+            }
         }
     }
 }

@@ -75,7 +75,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
     // consecutive pieces on one XCD
     const int group = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     const int64_t p0 = group * chunk, p1 = min(p0 + chunk, total);
-    i32x4v* begin = reinterpret_cast<i32x4v*>(a.ws) + 2 * group;
+    i32x4v* begin = begin_of(a.ws, group);
     if (p0 >= total) {
         if (tid == 0) begin[0] = i32x4v{-1, 0, 0, 0};
         return;
@@ -83,6 +83,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
     typename Split::Loc cur, end;
     Split::piece(a, pre, p0, p1, cur, end);
     PagedSeq s = paged_seq(a, cur.b);
+    if (lane < 2) *bad_of(a.ws, group, wave + 4 * lane) = 0;
     if (tid == 0) {
         begin[0] = i32x4v{cur.b, cur.hk, cur.r, cur.kt};
         begin[1] = i32x4v{s.off, (int)min((int64_t)BM, (int64_t)s.n * a.G - (int64_t)cur.r * BM), 0, 0};
@@ -271,6 +272,12 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                 issue(j + F::DEPTH, true);
             }
             wait_vm<0>();
+            if (a.causal) {
+                // keys that the last row may see, but not the first; a wave takes every fourth
+                const int close = min(max(s.len - s.n + (r0 + nr - 1) / a.G + 1, 0), s.len);
+                if (odd_values<D, F8>(a, table, cur.hk, max(open, k0 * KT) + wave, min(close, k1 * KT), kFewWaves))
+                    *bad_of(a.ws, group, wave) = 1;
+            }
 
             // ---- join the four waves, 16 rows at a time ----
             constexpr int LD = D + 4;
@@ -370,7 +377,7 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
     hipLaunchKernelGGL(kern, dim3(kGroups), dim3(64 * kFewWaves), LDS, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    auto* join = join_kernel<BM, D, 4, FewOrder<D>>;
+    auto* join = join_kernel<BM, D, F8, 4, FewOrder<D>>;
     hipLaunchKernelGGL(join, dim3(2 * kGroups), dim3(256), 0, stream, a);
     return hipGetLastError();
 }

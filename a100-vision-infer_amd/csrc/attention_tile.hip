@@ -139,7 +139,7 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
     const int64_t total = pre[a.B], chunk = Split::chunk(a, total, gridDim.x, kTileMinTiles);
     const int group = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     const int64_t p0 = group * chunk, p1 = min(p0 + chunk, total);
-    i32x4v* begin = reinterpret_cast<i32x4v*>(a.ws) + 2 * group;
+    i32x4v* begin = begin_of(a.ws, group);
     if (p0 >= total) {
         if (tid == 0) begin[0] = i32x4v{-1, 0, 0, 0};
         return;
@@ -147,6 +147,7 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
     typename Split::Loc cur, end;
     Split::piece(a, pre, p0, p1, cur, end);
     PagedSeq s = paged_seq(a, cur.b);
+    if (lane < 8 / W) *bad_of(a.ws, group, wave + W * lane) = 0;
     if (tid == 0) {
         begin[0] = i32x4v{cur.b, cur.hk, cur.r, cur.kt};
         begin[1] = i32x4v{s.off, (int)min((int64_t)kBM, (int64_t)s.n * a.G - (int64_t)cur.r * kBM), 0, 0};
@@ -462,6 +463,12 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
             weigh(yes, no, vb_last, sub1, 0, kb0, sub0, nothing);
             wait_vm<0>();
             drain(o);
+            if (a.causal && row0 < nr) {
+                // keys that the wave's last row may see, but not its first
+                const int close = min(max(ctx + (r0 + min(row0 + 32 * RB, nr) - 1) / a.G + 1, 0), s.len);
+                if (odd_values<D, F8>(a, table, cur.hk, max(open, k0 * kBN), min(close, k1 * kBN), 1))
+                    *bad_of(a.ws, group, wave) = 1;
+            }
 
             // A whole unit goes through its slot as well (the last piece's, not
             // yet in use): with O out of the registers its rows' gates can all
@@ -530,7 +537,7 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
     hipLaunchKernelGGL(kern, dim3(kGroups), dim3(64 * kBM / (32 * RB)), LDS, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((join_kernel<kBM, D, 1, TileOrder<D>>), dim3(8 * kGroups), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((join_kernel<kBM, D, F8, 1, TileOrder<D>>), dim3(8 * kGroups), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -188,6 +188,30 @@ def test_attention_cache_past_32_bits(fp8lin, gpu, dim, fp8):
     compare(got, b.expect())
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads", [(12, 2, 256), (8, 8, 64), (16, 1, 128)], ids=str)
+@pytest.mark.parametrize("held", [[(40, 4), (9, 9)], [(70, 70)], [(300, 100), (33, 3), (1, 1)]], ids=str)
+def test_attention_hides_what_a_row_may_not_see(fp8lin, gpu, held, heads, fp8):
+    """Infinities and NaN in keys and values of later tokens of a chunk: the rows before them are as if they were not there, the
+    rows that see them get them."""
+    b = Batch(held, *heads, page=16, fp8=fp8, gate=True, seed=13)
+    g = torch.Generator().manual_seed(14)
+    nan, inf = math.nan, math.inf
+    for r, (n, c) in enumerate(held):
+        if c < 3:
+            continue
+        for at, cache, values in ((n - 1, b.v, [nan, 3.0]), (n - c // 2, b.v, [inf, -inf]), (n - 1 - c // 4, b.k, [nan, 1.0])):
+            if cache.dtype != torch.bfloat16:
+                values = [nan, nan]  # E4M3FN has no infinities
+            row = cache[int(b.table[r, at // 16]), at % 16]
+            where = torch.randint(0, row.size(1), (row.size(0), 2), generator=g)
+            for h in range(row.size(0)):
+                for d, x in zip(where[h].tolist(), values):
+                    row[h, d] = x
+    got = fp8lin.paged_attention(max_count=b.max_count, **b.up(gpu))
+    compare(got, b.expect())
+
+
 def test_attention_is_repeatable_and_capturable(fp8lin, gpu):
     """Bit-equal calls; a captured call replayed with other lengths, queries and cache contents equals the eager one."""
     b = Batch([(300, 2), (50, 1), (90, 3)], 12, 2, 256, page=16, gate=True, seed=10)
