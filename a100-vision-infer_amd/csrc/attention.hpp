@@ -201,7 +201,7 @@ __device__ void plain_row(const PagedAttention& a, const PagedSeq& s, int b, int
 
 // The workspace: per workgroup where its piece begins (request, kv head, row
 // tile, key tile; request -1: no piece), the request's first row and the tile's
-// rows, and for each wave whether it met values that only some of its rows may
+// rows, and for each wave whether it met values that not all of its rows may
 // see and that are no finite numbers; then the partial sums of split units: O
 // (BM x D floats, the kernel's own order), m and l of the BM rows.  A workgroup
 // leaves at most two: slot 0 for the piece that begins inside a unit (its

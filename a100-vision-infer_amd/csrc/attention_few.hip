@@ -273,9 +273,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
             }
             wait_vm<0>();
             if (a.causal) {
-                // keys that the last row may see, but not the first; a wave takes every fourth
-                const int close = min(max(s.len - s.n + (r0 + nr - 1) / a.G + 1, 0), s.len);
-                if (odd_values<D, F8>(a, table, cur.hk, max(open, k0 * KT) + wave, min(close, k1 * KT), kFewWaves))
+                // keys of the piece that the first row may not see; a wave takes every fourth
+                if (odd_values<D, F8>(a, table, cur.hk, max(open, k0 * KT) + wave, min(s.len, k1 * KT), kFewWaves))
                     *bad_of(a.ws, group, wave) = 1;
             }
 

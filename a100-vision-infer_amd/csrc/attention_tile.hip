@@ -39,9 +39,6 @@ namespace fp8lin {
 namespace attn {
 namespace {
 
-#ifndef RBS
-#define RBS 1
-#endif
 constexpr int kBM = kTileRows, kBN = 64, kKeys = 16;  // kKeys: keys of a tile that a wave brings
 // A unit's start and end, in keys (heads of 256: up to 30 us at 64 keys in 4 us).
 template <int D>
@@ -464,9 +461,8 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
             wait_vm<0>();
             drain(o);
             if (a.causal && row0 < nr) {
-                // keys that the wave's last row may see, but not its first
-                const int close = min(max(ctx + (r0 + min(row0 + 32 * RB, nr) - 1) / a.G + 1, 0), s.len);
-                if (odd_values<D, F8>(a, table, cur.hk, max(open, k0 * kBN), min(close, k1 * kBN), 1))
+                // keys of the piece that the wave's first row may not see
+                if (odd_values<D, F8>(a, table, cur.hk, max(open, k0 * kBN), min(s.len, k1 * kBN), 1))
                     *bad_of(a.ws, group, wave) = 1;
             }
 
@@ -544,8 +540,8 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t stream) {
-    if (D == 64) return fp8 ? run<64, true, RBS>(a, stream) : run<64, false, RBS>(a, stream);
-    if (D == 128) return fp8 ? run<128, true, RBS>(a, stream) : run<128, false, RBS>(a, stream);
+    if (D == 64) return fp8 ? run<64, true, 1>(a, stream) : run<64, false, 1>(a, stream);
+    if (D == 128) return fp8 ? run<128, true, 1>(a, stream) : run<128, false, 1>(a, stream);
     return fp8 ? run<256, true, 2>(a, stream) : run<256, false, 2>(a, stream);
 }
 
@@ -561,7 +557,7 @@ size_t paged_attention_ws_bytes(int D, int64_t max_rows) {
 // Where some request may have more than kFewRows rows, a batch is computed in
 // two: a request of a few rows in a 256-row tile streams its keys at the pace
 // of one wave's steps (13 requests, three of them chunks of 400 to 700 tokens,
-// 32/8 heads of 128: MIXED us in two against 187).
+// 32/8 heads of 128: 161 us in two against 187).
 hipError_t launch_paged_attention(PagedAttention a, int D, bool fp8, int64_t max_rows, hipStream_t stream) {
     a.rows_from = 0;
     a.rows_to = INT64_MAX;

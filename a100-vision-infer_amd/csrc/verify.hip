@@ -68,7 +68,7 @@ __device__ __forceinline__ double slope(float t) { return 1.4426950408889634074 
 // |f| <= 1/2, 2^f = sum (f ln 2)^k / k! to k = 11, whose next term is below
 // 2^-47.  A relative error of 7e-15 moves a draw among 250 000 tokens with
 // probability 2e-9.  20 instructions without a branch, where the library's exp
-// takes 65: the rows of a batch of 48 requests (170 x 248320) 78 -> ROWS us.
+// takes 65: the rows of a batch of 48 requests (170 x 248320) 78 -> 48 us.
 // The coefficients stay in scalar registers (laundered, or the compiler would
 // load each into a vector register before every use).
 struct Exp2 {

@@ -212,6 +212,24 @@ def test_attention_hides_what_a_row_may_not_see(fp8lin, gpu, held, heads, fp8):
     compare(got, b.expect())
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads", [(12, 2, 256), (8, 8, 64), (16, 1, 128)], ids=str)
+@pytest.mark.parametrize("held", [(61, 61), (301, 193), (20, 33)], ids=str)
+def test_attention_hides_each_later_token(fp8lin, gpu, held, heads, fp8):
+    """A NaN in the values of one token of a chunk: the rows that see it have it, all others, of its tiles and of others, what
+    they have without it."""
+    n, c = held
+    b = Batch([held], *heads, page=16, fp8=fp8, gate=True, seed=15)
+    up = b.up(gpu)
+    out, bound = b.expect()
+    for at in range(max(n - c, 0), n, 3):
+        v, dim = up["v_cache"].clone(), at % heads[2]
+        v[int(b.table[0, at // 16]), at % 16, :, dim] = math.nan
+        want = out.clone()
+        want[at - (n - c):, :, dim] = math.nan
+        compare(fp8lin.paged_attention(max_count=c, **{**up, "v_cache": v}), (want, bound), f"token {at}")
+
+
 def test_attention_is_repeatable_and_capturable(fp8lin, gpu):
     """Bit-equal calls; a captured call replayed with other lengths, queries and cache contents equals the eager one."""
     b = Batch([(300, 2), (50, 1), (90, 3)], 12, 2, 256, page=16, gate=True, seed=10)
