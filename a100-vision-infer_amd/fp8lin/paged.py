@@ -154,7 +154,8 @@ def paged_attention(q, k_cache, v_cache, block_table, offsets, lengths, max_coun
     gate (as q) is given; scale defaults to head_dim ** -0.5.  max_count: the most
     rows that a request has (a hint that picks the kernel; by default the
     tokens beyond one per request).  Returns BF16 [tokens, heads, head_dim]:
-    `out` if given, whose rows behind the last request stay as they were."""
+    `out` if given, which overlaps no input and whose rows behind the last
+    request stay as they were."""
     rec = _cache(k_cache, v_cache, k_scale, v_scale)
     device, kv_heads, dim = k_cache.device, rec.kv_heads, rec.head_dim
     if not (isinstance(q, torch.Tensor) and q.dim() == 3 and q.dtype is _bf16 and q.stride(2) == 1 and q.device == device and
@@ -162,7 +163,7 @@ def paged_attention(q, k_cache, v_cache, block_table, offsets, lengths, max_coun
         _fail(ERR_ARGUMENT, "Paged attention expects BF16 queries [tokens, heads, head_dim]")
     shape = q.shape
     tokens, heads, _ = shape
-    if heads == 0 or heads % kv_heads:
+    if heads == 0 or kv_heads == 0 or heads % kv_heads:
         _fail(ERR_SHAPE, "Paged attention: heads must be a multiple of kv_heads")
     if not (isinstance(block_table, torch.Tensor) and block_table.dtype is _i32 and block_table.dim() == 2 and
             block_table.device == device and block_table.stride(1) == 1):

@@ -462,6 +462,96 @@ def test_verify_draws_the_distribution(fp8lin, gpu):
     assert float((share - torch.softmax(x[0].double().cpu(), 0) * n).abs().max()) <= 1.0 + 1e-6
 
 
+def test_verify_numbers_outside_the_interval(fp8lin, gpu):
+    """Numbers that are no uniforms stay inside the row: the first token with weight, or the last one."""
+    x = torch.randn(6, 700)
+    x[:, :3], x[:, 690:] = -math.inf, -math.inf
+    u = torch.tensor([-1.0, -math.inf, 1.0, 7.0, math.inf, math.nan])
+    offsets = torch.arange(7, dtype=torch.int32, device=gpu)
+    out = fp8lin.verify_drafts(x.to(gpu), torch.zeros(6, dtype=torch.int64, device=gpu), u.to(gpu), offsets)[1].tolist()
+    assert out[:5] == [3, 3, 689, 689, 689] and 3 <= out[5] <= 689
+
+
+def test_verify_past_32_bits(fp8lin, gpu):
+    """Logits of more than 2^31 values: the last rows as by themselves."""
+    rows, vocab = 9000, 248320
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    x = torch.zeros(rows, vocab, dtype=torch.bfloat16, device=gpu)
+    x[-300:].normal_(0, 3)
+    tokens, u = torch.randint(0, vocab, (rows,), device=gpu), torch.rand(rows, device=gpu)
+    tokens[-299:] = x[-300:-1].argmax(1)
+    offsets = torch.arange(0, rows + 1, 3, dtype=torch.int32, device=gpu)
+    taken, out = fp8lin.verify_drafts(x, tokens, u, offsets)
+    last = fp8lin.verify_drafts(x[-300:], tokens[-300:], u[-300:], (offsets[-101:] - offsets[-101]))
+    assert torch.equal(taken[-100:], last[0]) and torch.equal(out[-300:], last[1]) and int(taken[-100:].sum()) > 0
+
+
+# ---- refusals on the device -----------------------------------------------------
+
+
+def test_refused_tensors(fp8lin, gpu):
+    """Each tensor of another type, shape, place or stride than a call takes raises; nothing reaches a kernel."""
+    def alike(t):
+        yield t.cpu()
+        yield t.double() if t.is_floating_point() else t.to(torch.int16)
+        yield t[:-1] if t.dim() == 1 else t[..., :-1]
+        yield t.unsqueeze(0)
+        if t.dim() == 1 and t.numel() > 1:
+            yield torch.stack([t, t], 1)[:, 0]
+        elif t.dim() > 1:
+            yield t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+    b = Batch([(40, 3), (20, 2)], 4, 2, 64, page=16, gate=True, fp8=True)
+    ints = dict(dtype=torch.int32, device=gpu)
+    attention = dict(b.up(gpu), out=torch.empty(5, 4, 64, dtype=torch.bfloat16, device=gpu))
+    append = dict(k=attention["q"][:, :2], v=attention["q"][:, 2:], slots=torch.full((5,), -1, dtype=torch.int64, device=gpu),
+                  **{n: attention[n] for n in ("k_cache", "v_cache", "k_scale", "v_scale")})
+    layout = dict(lengths=torch.tensor([40, 20], **ints), counts=torch.tensor([1, 2], **ints), block_table=attention["block_table"],
+                  free_pages=torch.arange(3, **ints), cursor=torch.zeros(1, **ints), out=torch.empty_like(attention["block_table"]))
+    verify = dict(logits=torch.zeros(5, 90, device=gpu), tokens=torch.zeros(5, dtype=torch.int64, device=gpu),
+                  uniforms=torch.zeros(5, device=gpu), offsets=torch.tensor([0, 3, 5], **ints),
+                  draft_probs=torch.zeros(3, 90, device=gpu), temperature=torch.ones(2, device=gpu))
+    calls = [(fp8lin.paged_attention, attention, {}), (fp8lin.paged_append, append, {}),
+             (fp8lin.paged_layout, layout, dict(tokens=5, page_size=16)), (fp8lin.verify_drafts, verify, {})]
+    # of any length or width, of which a shorter one is as good
+    free = {("paged_layout", "free_pages"): (2,), ("paged_attention", "block_table"): (2,)}
+    for call, good, plain in calls:
+        call(**good, **plain)
+        for name, t in good.items():
+            for i, bad in enumerate(alike(t)):
+                if i in free.get((call.__name__, name), ()):
+                    continue
+                with pytest.raises(fp8lin.Fp8linError):
+                    call(**{**good, name: bad}, **plain)
+                    pytest.fail(f"{call.__name__}: {name} {i}")
+    for plain in (dict(tokens=-1, page_size=16), dict(tokens=5, page_size=24), dict(tokens=5, page_size=8)):
+        with pytest.raises(fp8lin.Fp8linError):
+            fp8lin.paged_layout(**layout, **plain)
+    for change in (dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(k_scale=None), dict(v_scale=None)):
+        with pytest.raises(fp8lin.Fp8linError):
+            fp8lin.paged_attention(**{**attention, **change})
+    none = attention["k_cache"][:, :, :0]
+    with pytest.raises(fp8lin.Fp8linError):
+        fp8lin.paged_attention(**{**attention, "k_cache": none, "v_cache": none, "k_scale": attention["k_scale"][:0],
+                                  "v_scale": attention["v_scale"][:0]})
+    torch.cuda.synchronize()
+
+
+def test_calls_without_tokens(fp8lin, gpu):
+    b = Batch([(40, 3), (20, 2)], 4, 2, 64, page=16)
+    up = b.up(gpu)
+    none = up["q"][:0]
+    out = fp8lin.paged_attention(**{**up, "q": none, "offsets": torch.zeros_like(up["offsets"])})
+    assert out.shape == none.shape
+    before = up["k_cache"].clone()
+    fp8lin.paged_append(none[:, :2], none[:, :2], torch.zeros(0, dtype=torch.int64, device=gpu), up["k_cache"], up["v_cache"])
+    assert torch.equal(before.view(torch.int16), up["k_cache"].view(torch.int16))
+    taken, out = fp8lin.verify_drafts(torch.zeros(0, 50, device=gpu), torch.zeros(0, dtype=torch.int64, device=gpu),
+                                      torch.zeros(0, device=gpu), torch.zeros(3, dtype=torch.int32, device=gpu))
+    assert taken.tolist() == [0, 0] and out.numel() == 0
+
+
 def test_verify_captured(fp8lin, gpu):
     rng = random.Random(7)
     logits, tokens, u, offsets, q = _drafted(rng, 6, 3, 9000, True, torch.bfloat16, 5)
