@@ -125,29 +125,27 @@ __device__ __forceinline__ void store4(const PagedAttention& a, int64_t tok, int
     store_bf16x4(a.out + tok * a.o_tok + head * a.o_head + d, o);
 }
 
-// Whether the values of keys first, first + step, .. < last hold an infinity or
-// NaN (on the lane that sees one), by a wave.
+// Whether the values of keys first, first + 1, .. < last hold an infinity or
+// NaN (on the lane that sees one), by wave `wave` of `waves` that share them.
 template <int D, bool F8>
-__device__ __forceinline__ bool odd_values(const PagedAttention& a, const int32_t* table, int hk, int first, int last, int step) {
-    constexpr int LANES = D / 4, PER = 64 / LANES;  // 4 dimensions a lane, keys at once
-    const int lane = threadIdx.x & 63, d = 4 * (lane % LANES);
-    bool odd = false;
-#pragma unroll 4
-    for (int k = first; k < last; k += step * PER) {
-        const int key = min(k + step * (lane / LANES), last - 1), id = table[key >> a.page_bits];
+__device__ __forceinline__ bool odd_values(const PagedAttention& a, const int32_t* table, int hk, int first, int last, int wave,
+                                           int waves) {
+    constexpr int ES = F8 ? 1 : 2, LANES = D * ES / 16, PER = 64 / LANES;  // 16 bytes a lane, keys at once
+    // an exponent of all ones (E4M3FN: all bits but the sign) carries into the bit above it
+    constexpr uint32_t BITS = F8 ? 0x7f7f7f7fu : 0x7f807f80u, ONE = F8 ? 0x01010101u : 0x00800080u;
+    const int lane = threadIdx.x & 63;
+    const char* base = static_cast<const char*>(a.v.data) + hk * a.v.head * ES + 16 * (lane % LANES);
+    uint32_t odd = 0;
+#pragma unroll 8
+    for (int k = first + PER * wave; k < last; k += PER * waves) {
+        const int key = min(k + lane / LANES, last - 1), id = table[key >> a.page_bits];
         const bool there = (unsigned)id < (unsigned)a.pages;
-        const int64_t at = (int64_t)(there ? id : 0) * a.v.page + (int64_t)(key & ((1 << a.page_bits) - 1)) * a.v.slot + hk * a.v.head + d;
-        if constexpr (F8) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v.data) + at);
+        const int64_t at = (int64_t)(there ? id : 0) * a.v.page + (int64_t)(key & ((1 << a.page_bits) - 1)) * a.v.slot;
+        const u32x4 w = *reinterpret_cast<const u32x4*>(base + at * ES);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) odd |= there && ((w >> (8 * i)) & 0x7fu) == 0x7fu;
-        } else {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(a.v.data) + at);
-            odd |= there && ((w.x & 0x7f80u) == 0x7f80u || (w.x & 0x7f800000u) == 0x7f800000u || (w.y & 0x7f80u) == 0x7f80u ||
-                             (w.y & 0x7f800000u) == 0x7f800000u);
-        }
+        for (int i = 0; i < 4; ++i) odd |= there ? (w[i] & BITS) + ONE : 0;
     }
-    return odd;
+    return (odd & (F8 ? 0x80808080u : 0x80008000u)) != 0;
 }
 
 // One row by plain FP32 sums, a key at a time, by a wave: for the rows near

@@ -273,8 +273,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
             }
             wait_vm<0>();
             if (a.causal) {
-                // keys of the piece that the first row may not see; a wave takes every fourth
-                if (odd_values<D, F8>(a, table, cur.hk, max(open, k0 * KT) + wave, min(s.len, k1 * KT), kFewWaves))
+                // keys of the piece that the first row may not see, by all waves
+                if (odd_values<D, F8>(a, table, cur.hk, max(open, k0 * KT), min(s.len, k1 * KT), wave, kFewWaves))
                     *bad_of(a.ws, group, wave) = 1;
             }
 

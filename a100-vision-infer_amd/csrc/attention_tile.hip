@@ -460,9 +460,10 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
             weigh(yes, no, vb_last, sub1, 0, kb0, sub0, nothing);
             wait_vm<0>();
             drain(o);
-            if (a.causal && row0 < nr) {
-                // keys of the piece that the wave's first row may not see
-                if (odd_values<D, F8>(a, table, cur.hk, max(open, k0 * kBN), min(s.len, k1 * kBN), 1))
+            if (a.causal) {
+                // keys of the piece that the tile's first row may not see, by all waves
+                const int open0 = min(max(ctx + r0 / a.G + 1, 0), s.len);
+                if (odd_values<D, F8>(a, table, cur.hk, max(open0, k0 * kBN), min(s.len, k1 * kBN), wave, W))
                     *bad_of(a.ws, group, wave) = 1;
             }
 
