@@ -381,11 +381,14 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// Tiles of 32 rows at the most: requests of 33 to 64 rows read their keys twice.
+// Tiles of 64 rows keep 256 registers of O for heads of 256 and spilled the rest
+// (48 rows, 8000 keys, 12/2 heads: 60 us against 26); for smaller heads they
+// gained 15 % on one long request (64 rows, 60000 8-bit keys, 32/8 heads of 128:
+// 57 us against 66) and lost 27 % on a batch (16 x 4000 keys: 85 against 67).
 template <int D, bool F8>
 hipError_t run_rows(const PagedAttention& a, int rows, hipStream_t stream) {
-    if (rows <= 16) return run<D, F8, 1>(a, stream);
-    if (rows <= 32) return run<D, F8, 2>(a, stream);
-    return run<D, F8, 4>(a, stream);
+    return rows <= 16 ? run<D, F8, 1>(a, stream) : run<D, F8, 2>(a, stream);
 }
 
 }  // namespace

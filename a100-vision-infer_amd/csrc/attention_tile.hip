@@ -550,25 +550,27 @@ hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t str
 
 size_t paged_attention_ws_bytes(int D, int64_t max_rows) {
     using namespace attn;
-    const int64_t bm = max_rows <= 16 ? 16 : max_rows <= 32 ? 32 : max_rows <= kFewRows ? 64 : kTileRows;
+    const int64_t bm = max_rows <= 16 ? 16 : max_rows <= kFewRows ? 32 : kTileRows;
     return (size_t)(4 * (kBeginFloats + 2 * kGroups * (bm * D + 2 * bm)));
 }
 
-// Either kernel computes any number of rows; the rule is what each is fast at.
-// Where some request may have more than kFewRows rows, a batch is computed in
-// two: a request of a few rows in a 256-row tile streams its keys at the pace
-// of one wave's steps (13 requests, three of them chunks of 400 to 700 tokens,
-// 32/8 heads of 128: 161 us in two against 187).
+// Either kernel computes any number of rows; the rule is what each is fast at
+// (heads of 256, 12/2, BF16 cache; few against tile, us: 60000 keys, 48 rows 57
+// and 81, 96 rows 78 and 83, 192 rows 128 and 85; 16 requests of 4000 keys, 48
+// rows 61 and 65, 66 rows 89 and 67).  Where some request may have more than
+// kFewRows rows, a batch is computed in two: a request of a few rows in a
+// 256-row tile streams its keys at the pace of one wave's steps (13 requests,
+// three of them chunks of 400 to 700 tokens, 32/8 heads of 128: 161 us in two
+// against 187).
 hipError_t launch_paged_attention(PagedAttention a, int D, bool fp8, int64_t max_rows, hipStream_t stream) {
     a.rows_from = 0;
     a.rows_to = INT64_MAX;
     if (max_rows <= attn::kFewRows) return attn::launch_few(a, D, fp8, (int)max_rows, stream);
     if (a.B > 1) {
-        constexpr int kSmall = 32;  // rows: decoding requests and drafted tokens of most head layouts
-        a.rows_to = kSmall;
-        const hipError_t e = attn::launch_few(a, D, fp8, kSmall, stream);
+        a.rows_to = attn::kFewRows;
+        const hipError_t e = attn::launch_few(a, D, fp8, attn::kFewRows, stream);
         if (e != hipSuccess) return e;
-        a.rows_from = kSmall;
+        a.rows_from = attn::kFewRows;
         a.rows_to = INT64_MAX;
     }
     return attn::launch_tile(a, D, fp8, stream);
