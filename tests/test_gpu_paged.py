@@ -230,6 +230,43 @@ def test_attention_hides_each_later_token(fp8lin, gpu, held, heads, fp8):
         compare(fp8lin.paged_attention(max_count=c, **{**up, "v_cache": v}), (want, bound), f"token {at}")
 
 
+@pytest.mark.parametrize("count", [1, 400])
+@pytest.mark.parametrize("held", ["all", "last"])
+def test_attention_of_the_most_requests(fp8lin, gpu, held, count):
+    """4096 requests, most of a few keys, or none but the last of any length; both kernels."""
+    rng = random.Random(held)
+    n = 4096
+    sizes = [(0, rng.choice([0, 1]))] * (n - 1) + [(3000, 2)]
+    if held == "all":
+        sizes = [(rng.choice([0, 1, 15, 16, 17, 40]), rng.choice([0, 1, 1, 2, 9])) for _ in range(n - 1)] + [(2000, 3)]
+    b = Batch(sizes, 2, 1, 64, page=16, seed=21)
+    compare(fp8lin.paged_attention(max_count=count, **b.up(gpu)), b.expect(), held)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads", [(128, 1, 64), (96, 1, 256), (65, 1, 128), (40, 40, 64), (64, 16, 128)], ids=str)
+def test_attention_many_heads(fp8lin, gpu, heads, fp8):
+    """More rows of one token than the few-rows kernel takes, many kv heads."""
+    b = Batch([(130, 1), (77, 3), (1, 1)], *heads, page=64, fp8=fp8, gate=True, seed=22)
+    want = b.expect()
+    for count in (1, 3, 300):
+        compare(fp8lin.paged_attention(max_count=count, **b.up(gpu)), want, str(count))
+
+
+def test_attention_one_page(fp8lin, gpu):
+    """The largest page: a request's keys in a row."""
+    g = torch.Generator().manual_seed(23)
+    k, v = [torch.randn(1, 1 << 20, 1, 64, generator=g).to(torch.bfloat16) for _ in range(2)]
+    q = torch.randn(4, 2, 64, generator=g).to(torch.bfloat16)
+    table, offsets, lengths = torch.zeros(2, 1, dtype=torch.int32), [0, 1, 4], [70001, 333]
+    want = PO.attention(q, k, v, table, offsets, lengths)
+    ints = dict(dtype=torch.int32, device=gpu)
+    for count in (1, 500):
+        got = fp8lin.paged_attention(q.to(gpu), k.to(gpu), v.to(gpu), table.to(gpu), torch.tensor(offsets, **ints),
+                                     torch.tensor(lengths, **ints), max_count=count)
+        compare(got, want, str(count))
+
+
 def test_attention_is_repeatable_and_capturable(fp8lin, gpu):
     """Bit-equal calls; a captured call replayed with other lengths, queries and cache contents equals the eager one."""
     b = Batch([(300, 2), (50, 1), (90, 3)], 12, 2, 256, page=16, gate=True, seed=10)
