@@ -219,8 +219,11 @@ struct Partial {
     }
 };
 
-hipError_t launch_few(const PagedAttention& a, int D, bool fp8, int rows, hipStream_t stream);
-hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t stream);
+// `rows`: the most of a request.  Without `join` the units' partial sums are
+// left to launch_tile's `few`, which joins both kernels' in one launch.
+hipError_t launch_few(const PagedAttention& a, int D, bool fp8, int rows, bool join, hipStream_t stream);
+hipError_t launch_tile(const PagedAttention& a, const PagedAttention* few, int D, bool fp8, hipStream_t stream);
+constexpr int kMixedRows = 32;  // rows of a few-rows tile of a mixed batch
 
 // Joins the pieces of the units that the boundaries between workgroups cut,
 // and writes their rows.  Every workgroup lists the split units from the
@@ -230,7 +233,7 @@ hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t str
 // first dimension of the e-th 4 floats of a piece's O.  The units of workgroups
 // with marked waves are computed again, row by row, instead.
 template <int BM, int D, bool F8, int WAVES, class ORDER>
-__global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
+__device__ __forceinline__ void join(const PagedAttention& a, int block, int blocks) {
     constexpr int PER = 256 / WAVES, PARTS = BM * D / 4 / PER;
     __shared__ i32x4v begin[kGroups], rows[kGroups];
     __shared__ int unit[kGroups], unit_last[kGroups], wave_units[4];
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
         unit_last[at + (first ? 0 : -1)] = tid;
     __syncthreads();
     const int q = WAVES > 1 ? wave : 0, et = WAVES > 1 ? lane : tid;
-    for (int item = blockIdx.x; item < units * PARTS; item += gridDim.x) {
+    for (int item = block; item < units * PARTS; item += blocks) {
         const int w = unit[item / PARTS], e = (item % PARTS) * PER + et;
         const i32x4v u = begin[w];
         const int r0 = u.z * BM, off = rows[w].x, nr = rows[w].y;
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
                 const PagedSeq s = paged_seq(a, u.x);
                 const int R = Split::tiles(a, s), r0 = u.z * BM;
                 if (u.z < R)
-                    for (int r = blockIdx.x * 4 + wave; r < (int)min((int64_t)BM, (int64_t)s.n * a.G - r0); r += 4 * gridDim.x)
+                    for (int r = block * 4 + wave; r < (int)min((int64_t)BM, (int64_t)s.n * a.G - r0); r += 4 * blocks)
                         plain_row<D, F8>(a, s, u.x, u.y, r0 + r);
                 if (end) break;
                 if (++u.z >= R) {
@@ -358,8 +361,21 @@ __global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
         }
     }
 }
+template <int BM, int D, bool F8, int WAVES, class ORDER>
+__global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
+    join<BM, D, F8, WAVES, ORDER>(a, blockIdx.x, gridDim.x);
+}
 
-// The order of O in the partial sums of the kernels with 32 rows per MFMA tile:
+// The order of O in the partial sums of the few-rows kernel: by row.
+template <int D>
+struct FewOrder {
+    static __device__ __forceinline__ void place(int e, int& row, int& d) {
+        row = e / (D / 4);
+        d = 4 * (e % (D / 4));
+    }
+};
+
+// The order of O in the partial sums of the kernel with 32 rows per MFMA tile:
 // as their registers hold it.
 template <int D>
 struct TileOrder {

@@ -357,16 +357,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
     }
 }
 
-template <int D>
-struct FewOrder {
-    static __device__ __forceinline__ void place(int e, int& row, int& d) {
-        row = e / (D / 4);
-        d = 4 * (e % (D / 4));
-    }
-};
-
 template <int D, bool F8, int NT>
-hipError_t run(const PagedAttention& a, hipStream_t stream) {
+hipError_t run(const PagedAttention& a, bool with_join, hipStream_t stream) {
     constexpr int BM = 16 * NT, LDS = Few<D, F8>::LDS;
     static_assert(LDS >= PagedSplit<BM, 16, 0>::lds_bytes(kPagedMaxRequests), "the prefix of the requests' costs fits");
     static_assert(LDS >= kFewWaves * 16 * (D + 6) * 4, "the waves' sums fit");
@@ -376,9 +368,9 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
     if (attr != hipSuccess) return attr;
     hipLaunchKernelGGL(kern, dim3(kGroups), dim3(64 * kFewWaves), LDS, stream, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    auto* join = join_kernel<BM, D, F8, 4, FewOrder<D>>;
-    hipLaunchKernelGGL(join, dim3(2 * kGroups), dim3(256), 0, stream, a);
+    if (e != hipSuccess || !with_join) return e;
+    auto* kern_join = join_kernel<BM, D, F8, 4, FewOrder<D>>;
+    hipLaunchKernelGGL(kern_join, dim3(2 * kGroups), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
@@ -388,16 +380,17 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
 // gained 15 % on one long request (64 rows, 60000 8-bit keys, 32/8 heads of 128:
 // 57 us against 66) and lost 27 % on a batch (16 x 4000 keys: 85 against 67).
 template <int D, bool F8>
-hipError_t run_rows(const PagedAttention& a, int rows, hipStream_t stream) {
-    return rows <= 16 ? run<D, F8, 1>(a, stream) : run<D, F8, 2>(a, stream);
+hipError_t run_rows(const PagedAttention& a, int rows, bool join, hipStream_t stream) {
+    static_assert(kMixedRows == 32);
+    return rows <= 16 ? run<D, F8, 1>(a, join, stream) : run<D, F8, 2>(a, join, stream);
 }
 
 }  // namespace
 
-hipError_t launch_few(const PagedAttention& a, int D, bool fp8, int rows, hipStream_t stream) {
-    if (D == 64) return fp8 ? run_rows<64, true>(a, rows, stream) : run_rows<64, false>(a, rows, stream);
-    if (D == 128) return fp8 ? run_rows<128, true>(a, rows, stream) : run_rows<128, false>(a, rows, stream);
-    return fp8 ? run_rows<256, true>(a, rows, stream) : run_rows<256, false>(a, rows, stream);
+hipError_t launch_few(const PagedAttention& a, int D, bool fp8, int rows, bool join, hipStream_t stream) {
+    if (D == 64) return fp8 ? run_rows<64, true>(a, rows, join, stream) : run_rows<64, false>(a, rows, join, stream);
+    if (D == 128) return fp8 ? run_rows<128, true>(a, rows, join, stream) : run_rows<128, false>(a, rows, join, stream);
+    return fp8 ? run_rows<256, true>(a, rows, join, stream) : run_rows<256, false>(a, rows, join, stream);
 }
 
 }  // namespace attn

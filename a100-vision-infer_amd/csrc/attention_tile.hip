@@ -528,8 +528,19 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
 
 namespace {
 
+constexpr int kFewJoin = 2 * kGroups, kTileJoin = 8 * kGroups;  // workgroups
+
+// The joins of a mixed batch: the first workgroups the few-rows kernel's.
+template <int D, bool F8>
+__global__ __launch_bounds__(256) void join_mixed_kernel(PagedAttention few, PagedAttention a) {
+    if (blockIdx.x < kFewJoin)
+        join<kMixedRows, D, F8, 4, FewOrder<D>>(few, blockIdx.x, kFewJoin);
+    else
+        join<kBM, D, F8, 1, TileOrder<D>>(a, blockIdx.x - kFewJoin, kTileJoin);
+}
+
 template <int D, bool F8, int RB>
-hipError_t run(const PagedAttention& a, hipStream_t stream) {
+hipError_t run(const PagedAttention& a, const PagedAttention* few, hipStream_t stream) {
     constexpr int LDS = std::max<int>(Tile<D, F8>::LDS, PagedSplit<kBM, kBN, 0>::lds_bytes(kPagedMaxRequests));
     auto* kern = tile_kernel<D, F8, RB>;
     static const hipError_t attr =
@@ -538,24 +549,30 @@ hipError_t run(const PagedAttention& a, hipStream_t stream) {
     hipLaunchKernelGGL(kern, dim3(kGroups), dim3(64 * kBM / (32 * RB)), LDS, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((join_kernel<kBM, D, F8, 1, TileOrder<D>>), dim3(8 * kGroups), dim3(256), 0, stream, a);
+    if (few)
+        hipLaunchKernelGGL((join_mixed_kernel<D, F8>), dim3(kFewJoin + kTileJoin), dim3(256), 0, stream, *few, a);
+    else
+        hipLaunchKernelGGL((join_kernel<kBM, D, F8, 1, TileOrder<D>>), dim3(kTileJoin), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_tile(const PagedAttention& a, int D, bool fp8, hipStream_t stream) {
-    if (D == 64) return fp8 ? run<64, true, 1>(a, stream) : run<64, false, 1>(a, stream);
-    if (D == 128) return fp8 ? run<128, true, 1>(a, stream) : run<128, false, 1>(a, stream);
-    return fp8 ? run<256, true, 2>(a, stream) : run<256, false, 2>(a, stream);
+hipError_t launch_tile(const PagedAttention& a, const PagedAttention* few, int D, bool fp8, hipStream_t stream) {
+    if (D == 64) return fp8 ? run<64, true, 1>(a, few, stream) : run<64, false, 1>(a, few, stream);
+    if (D == 128) return fp8 ? run<128, true, 1>(a, few, stream) : run<128, false, 1>(a, few, stream);
+    return fp8 ? run<256, true, 2>(a, few, stream) : run<256, false, 2>(a, few, stream);
 }
+
+static int64_t ws_floats(int D, int64_t bm) { return kBeginFloats + 2 * kGroups * (bm * D + 2 * bm); }
 
 }  // namespace attn
 
 size_t paged_attention_ws_bytes(int D, int64_t max_rows) {
     using namespace attn;
-    const int64_t bm = max_rows <= 16 ? 16 : max_rows <= kFewRows ? 32 : kTileRows;
-    return (size_t)(4 * (kBeginFloats + 2 * kGroups * (bm * D + 2 * bm)));
+    return (size_t)4 * (max_rows <= 16         ? ws_floats(D, 16)
+                        : max_rows <= kFewRows ? ws_floats(D, 32)
+                                               : ws_floats(D, kTileRows) + ws_floats(D, kMixedRows));
 }
 
 // Either kernel computes any number of rows; the rule is what each is fast at
@@ -564,20 +581,20 @@ size_t paged_attention_ws_bytes(int D, int64_t max_rows) {
 // rows 61 and 65, 66 rows 89 and 67).  Where some request may have more than
 // kFewRows rows, a batch is computed in two: a request of a few rows in a
 // 256-row tile streams its keys at the pace of one wave's steps (13 requests,
-// three of them chunks of 400 to 700 tokens, 32/8 heads of 128: 161 us in two
-// against 187).
+// three of them chunks of 400 to 700 tokens, 32/8 heads of 128: 162 us in two
+// against 187).  One launch joins both kernels' partial sums (168 us with two).
 hipError_t launch_paged_attention(PagedAttention a, int D, bool fp8, int64_t max_rows, hipStream_t stream) {
     a.rows_from = 0;
     a.rows_to = INT64_MAX;
-    if (max_rows <= attn::kFewRows) return attn::launch_few(a, D, fp8, (int)max_rows, stream);
-    if (a.B > 1) {
-        a.rows_to = attn::kFewRows;
-        const hipError_t e = attn::launch_few(a, D, fp8, attn::kFewRows, stream);
-        if (e != hipSuccess) return e;
-        a.rows_from = attn::kFewRows;
-        a.rows_to = INT64_MAX;
-    }
-    return attn::launch_tile(a, D, fp8, stream);
+    if (max_rows <= attn::kFewRows) return attn::launch_few(a, D, fp8, (int)max_rows, true, stream);
+    if (a.B == 1) return attn::launch_tile(a, nullptr, D, fp8, stream);
+    PagedAttention few = a;
+    few.rows_to = attn::kFewRows;
+    few.ws = a.ws + attn::ws_floats(D, attn::kTileRows);
+    const hipError_t e = attn::launch_few(few, D, fp8, attn::kFewRows, false, stream);
+    if (e != hipSuccess) return e;
+    a.rows_from = attn::kFewRows;
+    return attn::launch_tile(a, &few, D, fp8, stream);
 }
 
 }  // namespace fp8lin
