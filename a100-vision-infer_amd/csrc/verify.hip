@@ -14,10 +14,14 @@
 //
 //   1. verify_rows_kernel: slices of every row -> maximum, sum of exponentials;
 //   2. verify_weigh_kernel: kept drafts per request; the sums of the weights of
-//      its deciding row by slices;
+//      its deciding row by slices.  Without draft probabilities (q = 1 at the
+//      draft) those are the first kernel's, which leaves the row's draft out of
+//      its sums then, and this one is not run;
 //   3. verify_draw_kernel: the slice, then the token, that the number falls on.
-// 48 requests, 170 rows of 248320: 48 us (FP64 exponentials; 84 MB), 28 us and
-// 12 us; one request's 4 rows: 6, 8 and 8 us (latency).
+// 48 requests, 170 rows of 248320, with probabilities: 48 us (FP64 exponentials;
+// 84 MB), 28 us and 12 us.  Without: 192 rows 71 us a call (83 with the second
+// kernel), one row of each of 256 requests 82 (162), 4 rows of one request 6 and
+// 11 us (latency; 17 us a call, 22).
 #include <algorithm>
 
 #include "device.hpp"
@@ -45,7 +49,7 @@ struct Args {
     int64_t T;
     int32_t* accepted;
     int64_t* out;
-    double* row_sum;    // [T][slices]
+    double* row_sum;    // [T][slices]; without draft probabilities: without the row's draft
     float* row_max;     // [T][slices]
     int32_t* row_at;    // [T][slices] first column of the maximum
     double* weight;     // [B][cuts][2] sums of max(p - q, 0) and of p
@@ -167,14 +171,17 @@ __device__ __forceinline__ void load8(const T* row, int j, int end, float fill, 
     }
 }
 
-// Workgroup (row, slice).
-template <class T, bool VEC>
+// Workgroup (row, slice).  DIRECT: without draft probabilities.
+template <class T, bool VEC, bool DIRECT>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(Args g) {
     __shared__ Stat part[kThreads / 64];
     const int64_t row = blockIdx.x;
     const int slice = blockIdx.y, tid = threadIdx.x;
     if (row >= g.offsets[g.B]) return;  // behind the last request
-    const double s = slope(temperature(g, owner_of(g, row)));
+    const int b = owner_of(g, row);
+    const double s = slope(temperature(g, b));
+    const int64_t draft = DIRECT && row + 1 < g.offsets[b + 1] ? g.tokens[min(row + 1, g.T - 1)] : -1;
+    const int x_col = draft >= 0 && draft < g.V ? (int)draft : -1;
     const int lo = slice * g.per, hi = min(lo + g.per, g.V);
     const T* logits = static_cast<const T*>(g.logits) + row * g.ld;
     const Exp2 e;
@@ -195,10 +202,13 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(Args g) {
         }
         const float m = v.m == -__builtin_inff() ? 0.0f : v.m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            bad |= x[i] != x[i];
-            v.sum += weigh(e, x[i], m, s);
-        }
+        for (int i = 0; i < 8; ++i) bad |= x[i] != x[i];
+        if (DIRECT && (unsigned)(x_col - j) < 8u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (j + i == x_col) x[i] = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v.sum += weigh(e, x[i], m, s);
     }
     if (bad || v.m == __builtin_inff()) v.sum = __builtin_nan("");
     v = wave_join(e, v, s);
@@ -229,7 +239,8 @@ __device__ __forceinline__ bool valid(const Stat& v) { return v.sum > 0.0 && v.s
 
 struct Decision {
     int64_t kept;   // accepted drafts; row a + kept decides the next token
-    Stat stat;      // that row's
+    Stat stat;      // that row's, the sum of all columns
+    double draft;   // the exponential of its draft
     int64_t probs;  // row of the draft's probabilities for the request's first draft
 };
 
@@ -250,6 +261,7 @@ __device__ Decision decide(const Args& g, int b, const Request& r) {
     constexpr int kWaves = kThreads / 64;
     __shared__ int first;
     __shared__ Stat stats[kWaves];
+    __shared__ double drafts[kWaves];
     const int tid = threadIdx.x, wave = tid >> 6;
     const float t = temperature(g, b);
     const double s = slope(t);
@@ -271,18 +283,21 @@ __device__ Decision decide(const Args& g, int b, const Request& r) {
             const bool q_in = g.probs && in && qr >= 0 && qr < g.prob_rows;
             const double q = q_in ? (double)g.probs[qr * g.ldp + x] : g.probs ? 0.0 : 1.0;
             const double u = (double)g.u[row];
-            const Stat v = row_stat(g, e, row, s);
-            const double p = greedy(t) ? (v.at == x ? 1.0 : 0.0) : weigh(e, at, v.m, s) / v.sum;
+            Stat v = row_stat(g, e, row, s);
+            const double at_x = in ? weigh(e, at, v.m == -__builtin_inff() ? 0.0f : v.m, s) : 0.0;
+            if (!g.probs) v.sum += at_x;
+            const double p = greedy(t) ? (v.at == x ? 1.0 : 0.0) : at_x / v.sum;
             const bool keep = in && valid(v) && u * q < p;
             if ((tid & 63) == 0) {
                 stats[wave] = v;
+                drafts[wave] = at_x;
                 if (!keep) atomicMin(&first, (int)i);
             }
         }
         __syncthreads();
         if (first < i0 + kWaves) break;
     }
-    return Decision{first, stats[first % kWaves], probs};
+    return Decision{first, stats[first % kWaves], drafts[first % kWaves], probs};
 }
 
 // The weights of 8 columns in the deciding row: max(p - q, 0) in w, and p.
@@ -374,7 +389,8 @@ __device__ __forceinline__ double wave_scan64(double v) {
 }
 
 // One workgroup per request; the last one also clears the rows behind them.
-template <class T, bool VEC>
+// DIRECT: without draft probabilities; the slices are the rows'.
+template <class T, bool VEC, bool DIRECT>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(Args g) {
     __shared__ double wave_total[kThreads / 64], target_s;
     __shared__ int slice_s, pick_s, last_s;
@@ -386,11 +402,32 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(Args g) {
         if (tid == 0) g.accepted[b] = 0;
         return;
     }
+    Decision c;
+    if constexpr (DIRECT) c = decide<T>(g, b, r);
+    else c = g.decision[b];
+    const Weights<T, VEC> weights(g, b, r, c);
+    const int cuts = DIRECT ? g.slices : g.cuts, per = DIRECT ? g.per : g.cut_per;
     if (wave == 0) {
         // a lane per slice; p itself where the target is nowhere above the draft
-        const double* weight = g.weight + ((int64_t)b * g.cuts + min(lane, g.cuts - 1)) * 2;
-        double w = lane < g.cuts ? weight[0] : 0.0;
-        const double p = lane < g.cuts ? weight[1] : 0.0;
+        double w = 0.0, p = 0.0;
+        if constexpr (DIRECT) {
+            const int64_t at = (r.a + c.kept) * cuts + min(lane, cuts - 1);
+            const double sum = g.row_sum[at];
+            const float top = g.row_max[at];
+            const int64_t lo = (int64_t)lane * per;
+            auto holds = [&](int64_t j) { return j >= lo && j < lo + per; };
+            if (weights.at >= 0) {
+                p = holds(weights.at) ? 1.0 : 0.0;
+                w = weights.at == weights.x ? 0.0 : p;
+            } else if (lane < cuts) {
+                w = sum == 0.0 ? 0.0 : sum * weigh(weights.e, top, weights.m, weights.s) * weights.scale;
+                p = weights.x >= 0 && holds(weights.x) ? w + c.draft * weights.scale : w;
+            }
+        } else if (lane < cuts) {
+            const double* weight = g.weight + ((int64_t)b * cuts + lane) * 2;
+            w = weight[0];
+            p = weight[1];
+        }
         const int of = __ballot(w > 0.0) ? 0 : 1;
         if (of) w = p;
         const double run = wave_scan64(w), target = (double)g.u[r.a + r.n - 1] * __shfl(run, 63, 64);
@@ -404,12 +441,10 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(Args g) {
             last_s = -1;
         }
     }
-    const Decision c = g.decision[b];
-    const Weights<T, VEC> weights(g, b, r, c);
     __syncthreads();
     const int slice = slice_s >> 1, of = slice_s & 1;
     const double target = target_s;
-    const int lo = min(slice * g.cut_per, g.V), hi = min(lo + g.cut_per, g.V);
+    const int lo = min(slice * per, g.V), hi = min(lo + per, g.V);
     double base = 0.0;
     int pick = INT32_MAX, last = -1;
     for (int j0 = lo; j0 < hi; j0 += 8 * kThreads) {
@@ -453,30 +488,36 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(Args g) {
 
 // Columns of a slice of one of `rows` rows: enough slices to fill the chip, few
 // enough to be joined by one wave in one go (64).
-int slice_columns(int64_t rows, int64_t V) {
-    const int64_t want = std::min<int64_t>(64, std::max<int64_t>(1, 2048 / std::max<int64_t>(rows, 1)));
+int slice_columns(int64_t rows, int64_t V, int64_t least = 1) {
+    const int64_t want = std::min<int64_t>(64, std::max<int64_t>(least, 2048 / std::max<int64_t>(rows, 1)));
     const int64_t per = std::max<int64_t>((V + want - 1) / want, 2048);
     return (int)((per + 7) / 8 * 8);
 }
+// Without draft probabilities one workgroup goes through a slice of a row in
+// the draw: 24 at the least (192 rows of 248320: 84 us a call with 11, 71 with
+// 24, 72 with 48; with probabilities more than the chip holds only cost).
+constexpr int64_t kDirectSlices = 24;
 int64_t slices_of(int64_t V, int per) { return (V + per - 1) / per; }
 
 template <class T, bool VEC>
 hipError_t run(const Args& g, hipStream_t stream) {
     const dim3 block(kThreads);
     if (g.T) {
-        hipLaunchKernelGGL((verify_rows_kernel<T, VEC>), dim3((unsigned)g.T, g.slices), block, 0, stream, g);
-        hipLaunchKernelGGL((verify_weigh_kernel<T, VEC>), dim3(g.B, g.cuts), block, 0, stream, g);
+        if (g.probs) hipLaunchKernelGGL((verify_rows_kernel<T, VEC, false>), dim3((unsigned)g.T, g.slices), block, 0, stream, g);
+        else hipLaunchKernelGGL((verify_rows_kernel<T, VEC, true>), dim3((unsigned)g.T, g.slices), block, 0, stream, g);
+        if (g.probs) hipLaunchKernelGGL((verify_weigh_kernel<T, VEC>), dim3(g.B, g.cuts), block, 0, stream, g);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((verify_draw_kernel<T, VEC>), dim3(g.B), block, 0, stream, g);
+    if (g.probs) hipLaunchKernelGGL((verify_draw_kernel<T, VEC, false>), dim3(g.B), block, 0, stream, g);
+    else hipLaunchKernelGGL((verify_draw_kernel<T, VEC, true>), dim3(g.B), block, 0, stream, g);
     return hipGetLastError();
 }
 
 }  // namespace
 
 size_t verify_ws_bytes(int64_t T, int64_t B, int64_t V) {
-    return (size_t)(T * slices_of(V, slice_columns(T, V)) * 16 + B * slices_of(V, slice_columns(B, V)) * 16 +
+    return (size_t)(T * slices_of(V, slice_columns(T, V, kDirectSlices)) * 16 + B * slices_of(V, slice_columns(B, V)) * 16 +
                     B * (int64_t)sizeof(Decision));
 }
 
@@ -487,7 +528,7 @@ hipError_t launch_verify(const void* logits, bool bf16, int64_t ld, const float*
     g.logits = logits, g.ld = ld, g.probs = probs, g.ldp = ldp, g.prob_rows = prob_rows;
     g.tokens = tokens, g.u = u, g.offsets = offsets, g.temperature = temperature;
     g.B = B, g.V = V, g.T = T, g.accepted = accepted, g.out = out;
-    g.per = slice_columns(T, V), g.slices = (int)slices_of(V, g.per);
+    g.per = slice_columns(T, V, probs ? 1 : kDirectSlices), g.slices = (int)slices_of(V, g.per);
     g.cut_per = slice_columns(B, V), g.cuts = (int)slices_of(V, g.cut_per);
     g.row_sum = static_cast<double*>(ws);
     g.weight = g.row_sum + T * g.slices;

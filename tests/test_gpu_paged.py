@@ -487,6 +487,29 @@ def test_verify_masked_and_broken_rows(fp8lin, gpu):
             assert got[0].tolist() == want[0] and got[1].tolist() == want[1]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [40, 9001, 248320])
+def test_verify_refuses_likely_drafts(fp8lin, gpu, vocab, dtype):
+    """Drafts of nearly all probability that the largest number below 1 refuses, and certain ones that it does not: the token is
+    drawn from what little is left."""
+    g = torch.Generator().manual_seed(vocab)
+    rows = 24
+    x = torch.randn(rows, vocab, generator=g)
+    tokens = torch.randint(0, vocab, (rows,), generator=g)
+    for i in range(0, rows, 2):  # row i decides on the draft tokens[i + 1]
+        x[i, tokens[i + 1]] = math.log(vocab) + 4 + i / 2
+    x[22, :] = -math.inf
+    x[22, tokens[23]] = 1.0
+    x = x.to(dtype)
+    u = torch.rand(rows, generator=g)
+    u[::2] = 1 - 2.0 ** -24
+    offsets = list(range(0, rows + 1, 2))
+    want = PO.verify(x, tokens, u, offsets, None, None)
+    got = fp8lin.verify_drafts(x.to(gpu), tokens.to(gpu), u.to(gpu), torch.tensor(offsets, dtype=torch.int32, device=gpu))
+    assert got[0].tolist() == want[0] and got[1].tolist() == want[1]
+    assert 0 < sum(want[0]) < 12
+
+
 def test_verify_draws_the_distribution(fp8lin, gpu):
     """Over an even grid of numbers every token is drawn as often as its share of the residual weight says, to one draw."""
     v, n = 300, 4096
