@@ -631,6 +631,54 @@ def test_verify_captured(fp8lin, gpu):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_calls_at_once_and_graphs_of_one_pool(fp8lin, gpu):
+    """Layout, a mixed batch's attention and verification without probabilities: on two streams at once, and in two captured graphs
+    that share a memory pool, replayed in turn with eager calls between, as by themselves."""
+    rng = random.Random(31)
+    sets = []
+    for seed in (1, 2):
+        b = Batch([(300, 90), (50, 1), (90, 30), (7, 0)], 12, 2, 256, page=16, gate=True, seed=seed)
+        up = b.up(gpu)
+        logits, tokens, u, offsets, _ = _drafted(rng, 6, 3, 9000, False, torch.bfloat16, seed)
+        ints = dict(dtype=torch.int32, device=gpu)
+        verify = [logits.to(gpu), tokens.to(gpu), u.to(gpu), torch.tensor(offsets, **ints)]
+        layout = [torch.tensor([3, 40, 16, 0], **ints), torch.tensor([2, 1, 17, 5], **ints),
+                  torch.where(torch.arange(8, device=gpu)[None] < torch.tensor([1, 3, 1, 0], device=gpu)[:, None], 9, -1).int(),
+                  torch.randperm(20, device=gpu).int(), 25, 16]
+
+        def call(up=up, verify=verify, layout=layout):
+            return (*fp8lin.paged_layout(*layout), fp8lin.paged_attention(max_count=90, **up), *fp8lin.verify_drafts(*verify))
+        sets.append((call, [x.clone() for x in call()], up, verify))
+
+    def same(got, want):
+        return all(torch.equal(x.view(torch.int16) if x.dtype == torch.bfloat16 else x, y.view(torch.int16) if y.dtype == torch.bfloat16 else y)
+                   for x, y in zip(got, want))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = []
+        for s, (call, *_rest) in zip(streams, sets):
+            with torch.cuda.stream(s):
+                got.append(call())
+        torch.cuda.synchronize()
+        assert all(same(x, w) for x, (_, w, *_rest) in zip(got, sets))
+    graphs, outs = [], []
+    for call, *_rest in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append(call())
+        graphs.append(graph)
+    for i in range(4):
+        for graph, out, (call, _, up, verify) in zip(graphs, outs, sets):
+            up["q"].mul_(0.9)
+            verify[2].copy_(torch.rand(verify[2].shape, generator=torch.Generator().manual_seed(i)))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [x.clone() for x in out]
+            assert same(got, call()), i
+
+
 # ---- a run of them together -----------------------------------------------------
 
 
