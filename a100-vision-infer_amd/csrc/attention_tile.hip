@@ -45,6 +45,8 @@ namespace {
 
 constexpr int kBM = kTileRows, kBN = 64, kKeys = 16;  // kKeys: keys of a tile that a wave brings
 // A unit's start and end, in keys (heads of 256: up to 30 us at 64 keys in 4 us).
+// With 192, 320, 448 and 640 at 256 a prompt of 3913 tokens takes 196, 161, 150
+// and 157 us, a chunk of 512 85, 86, 86 and 88.
 template <int D>
 constexpr int kTileStart = 448 * D / 256;
 constexpr int kTileMinTiles = 4;

@@ -111,8 +111,8 @@ struct PagedSplit {
         return max((limit + BN - 1) / BN, 1);
     }
 
-    // floor(x / y) for 0 <= x, 0 < y, both below 2^52: by the FP64 quotient,
-    // whose error of under half a unit of the result the two checks take back.
+    // floor(x / y) for 0 <= x < 2^62, 0 < y, x / y below 2^31: by the FP64
+    // quotient, whose error of under half a unit the two checks take back.
     static __device__ __forceinline__ int64_t div(int64_t x, int64_t y) {
         int64_t q = (int64_t)((double)x / (double)y);
         if (q * y > x) --q;
@@ -177,7 +177,7 @@ struct PagedSplit {
         int64_t q = p - pre[lo];
         Loc l;
         l.b = lo;
-        l.hk = (int)div(q, per_head);
+        l.hk = (int)min(max(div(q, per_head), (int64_t)0), (int64_t)a.HK - 1);
         q -= l.hk * per_head;
         int rl = 0, rh = tiles(a, s);
         while (rh - rl > 1) {
@@ -187,7 +187,10 @@ struct PagedSplit {
         l.r = rl;
         const int64_t start = (int64_t)START * a.G;
         q = max(q - first(a, s, rl) - start, (int64_t)0);
-        l.kt = (int)div(q * key_tiles(a, s, rl), tile(a, s, rl) - start);
+        // in FP64, as the product may pass 64 bits: a piece's end and the next
+        // one's begin are the same computation, which grows with q
+        const int kts = key_tiles(a, s, rl);
+        l.kt = min(max((int)((double)q * kts / (double)(tile(a, s, rl) - start)), 0), kts - 1);
         return l;
     }
     // The pieces [p0, p1) of every wave's workgroup: even lanes find where it
@@ -202,9 +205,9 @@ struct PagedSplit {
                   __builtin_amdgcn_readlane(l.kt, 1)};
     }
     // Length of a piece: an even share, but no shorter than min_tiles key
-    // tiles of a unit.
+    // tiles of a unit.  groups: a power of two.
     static __device__ __forceinline__ int64_t chunk(const PagedAttention& a, int64_t total, int groups, int min_tiles) {
-        return max(div(total + groups - 1, groups), (int64_t)min_tiles * BN * a.G);
+        return max((total + groups - 1) >> (31 - __builtin_clz(groups)), (int64_t)min_tiles * BN * a.G);
     }
 };
 

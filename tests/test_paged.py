@@ -47,7 +47,7 @@ def test_bad_caches(fp8lin, change, code):
     (dict(heads=3), 1), (dict(heads=0), 1), (dict(heads=-2), 1), (dict(tokens=-1), 1), (dict(tokens=1 << 30), 1), (dict(requests=0), 1),
     (dict(requests=8193), 1), (dict(width=0), 1), (dict(width=(1 << 26) + 1), 1), (dict(table_ld=7), 1), (dict(scale=0.0), 2),
     (dict(scale=-1.0), 2), (dict(scale=float("nan")), 2), (dict(scale=float("inf")), 2), (dict(scale=1e-60), 2),
-    (dict(workspace_bytes=64), 4), (dict(workspace=None), 4), (dict(workspace=ctypes.c_void_p(0x10008)), 4),
+    (dict(tokens=1 << 10, heads=1 << 20, width=1 << 24), 1), (dict(workspace_bytes=64), 4), (dict(workspace=None), 4), (dict(workspace=ctypes.c_void_p(0x10008)), 4),
     (dict(tokens=0, q=None, out=None, workspace=None, workspace_bytes=0), 0),
 ], ids=str)
 def test_attention_validation(fp8lin, change, code):
