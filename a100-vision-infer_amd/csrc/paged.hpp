@@ -1,4 +1,4 @@
-// Host-side arguments of the paged-cache kernels (paged.hip, attention.hip)
+// Host-side arguments of the paged-cache kernels (paged.hip, attention_*.hip)
 // and the device-side arithmetic that the attention kernels share: which part
 // of which request a workgroup computes.
 #pragma once
