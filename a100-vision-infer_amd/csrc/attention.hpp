@@ -188,7 +188,7 @@ __device__ void plain_row(const PagedAttention& a, const PagedSeq& s, int b, int
         const float f = m == -__builtin_inff() ? 0.0f : exp2_fast(m - ms), p = exp2_fast(x - ms);
         l = l * f + p;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = (f == 0.0f ? 0.0f : o[i] * f) + p * v[i];
+        for (int i = 0; i < 4; ++i) o[i] = o[i] * f + p * v[i];
         m = mn;
     }
     const float inv = l == 0.0f ? 0.0f : (F8 ? a.v_scale[hk] : 1.0f) / l;
@@ -287,13 +287,16 @@ __device__ __forceinline__ void join(const PagedAttention& a, int block, int blo
         }
         float M = -__builtin_inff(), l = 0.0f;
         f32x4 o = {0, 0, 0, 0};
+        // A factor of 0 is multiplied in like any other: a part whose scores are
+        // all NaN has m = -inf and l = NaN, and a NaN stays one however little
+        // its part weighs; a part of nothing adds l = 0, O = 0.
         auto add = [&](float m1, float l1, f32x4 o1) {
             const float mn = fmaxf(M, m1);
             const float f0 = M == -__builtin_inff() ? 0.0f : exp2_fast(M - mn);
             const float f1 = m1 == -__builtin_inff() ? 0.0f : exp2_fast(m1 - mn);
-            l = (f0 == 0.0f ? 0.0f : l * f0) + (f1 == 0.0f ? 0.0f : l1 * f1);
+            l = l * f0 + l1 * f1;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = (f0 == 0.0f ? 0.0f : o[i] * f0) + (f1 == 0.0f ? 0.0f : o1[i] * f1);
+            for (int i = 0; i < 4; ++i) o[i] = o[i] * f0 + o1[i] * f1;
             M = mn;
         };
         if (ok) {
@@ -312,7 +315,11 @@ __device__ __forceinline__ void join(const PagedAttention& a, int block, int blo
                     m1[i] = part[(int64_t)BM * D + row];
                     l1[i] = part[(int64_t)BM * D + BM + row];
                     o1[i] = *reinterpret_cast<const f32x4*>(part + 4 * (int64_t)e);
-                    if (!there) m1[i] = -__builtin_inff();
+                    if (!there) {
+                        m1[i] = -__builtin_inff();
+                        l1[i] = 0.0f;
+                        o1[i] = f32x4{0, 0, 0, 0};
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < UN; ++i) add(m1[i], l1[i], o1[i]);

@@ -324,7 +324,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                         for (int w = 0; w < kFewWaves; ++w) {
                             const f32x4 x = *reinterpret_cast<const f32x4*>(so + (w * 16 + row) * LD + d);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) t[i] += f[w] == 0.0f ? 0.0f : x[i] * f[w];
+                            for (int i = 0; i < 4; ++i) t[i] += x[i] * f[w];
                         }
                         if (whole) {
 #pragma unroll

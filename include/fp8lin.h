@@ -593,7 +593,9 @@ int fp8lin_paged_append(const fp8lin_paged_cache* cache, const uint16_t* k, int6
  * over the keys up to each row's own token (causal), or all lengths[b] keys.
  * gate [tokens, heads, head_dim] may be null.  FP32 sums, one rounding of the
  * result; the weights are rounded to BF16 for the product with V.  A row
- * without keys (or whose every score is -inf) gives 0; a page id outside
+ * without keys (or whose every score is -inf) gives 0; a NaN or +inf among a
+ * row's scores makes its head NaN, a NaN in a value that it sees that element,
+ * and what a row may not see does not reach it.  A page id outside
  * [0, pages) reads as keys and values of 0; lengths are cut to the table's
  * width; rows from offsets[requests] on are left as they are.
  * max_count: the most rows that a request is expected to have; more give the
