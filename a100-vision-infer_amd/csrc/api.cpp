@@ -539,6 +539,39 @@ void check_cache(const fp8lin_paged_cache* c, fp8lin::PagedCache& k, fp8lin::Pag
     v = fp8lin::PagedCache{c->v, c->v_page, c->v_slot, c->v_head};
 }
 
+constexpr int64_t kMaxStride = (int64_t)1 << 56;  // elements; bytes of it stay in 64 bits
+
+// Memory of an operand: `rows` rows of `width` bytes, `stride` bytes apart
+// (stride >= width).
+struct Extent {
+    const void* at;
+    int64_t rows, width, stride;
+};
+Extent extent(const void* at, int64_t elements, int64_t size) { return Extent{at, 1, elements * size, elements * size}; }
+
+// Whether the two have a byte in common.
+bool overlap(const Extent& a, const Extent& b) {
+    if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+    if (a.rows > b.rows) return overlap(b, a);
+    const __int128 a0 = (intptr_t)a.at, b0 = (intptr_t)b.at, stride = b.rows > 1 ? b.stride : b.width;
+    if (a0 >= b0 + (b.rows - 1) * stride + b.width || b0 >= a0 + (a.rows - 1) * (__int128)a.stride + a.width) return false;
+    for (int64_t i = 0; i < a.rows; ++i) {
+        const __int128 lo = a0 + i * (__int128)a.stride, hi = lo + a.width;
+        if (hi <= b0) continue;
+        // the last row of b that begins before hi
+        const __int128 last = std::min<__int128>((hi - 1 - b0) / stride, b.rows - 1);
+        if (b0 + last * stride + b.width > lo) return true;
+    }
+    return false;
+}
+
+void require_apart(std::initializer_list<Extent> outputs, std::initializer_list<Extent> inputs, const char* what) {
+    for (auto o = outputs.begin(); o != outputs.end(); ++o) {
+        for (const Extent& i : inputs) require(!overlap(*o, i), FP8LIN_ERR_ARGUMENT, what);
+        for (auto p = o + 1; p != outputs.end(); ++p) require(!overlap(*o, *p), FP8LIN_ERR_ARGUMENT, what);
+    }
+}
+
 // Rows of a request per kv head.
 int64_t paged_rows(int64_t heads, int64_t kv_heads, int64_t max_count) {
     return heads / kv_heads * std::min<int64_t>(std::max<int64_t>(max_count, 1), kMaxDim);
@@ -1064,11 +1097,22 @@ int fp8lin_paged_layout(const int32_t* lengths, const int32_t* counts, const int
                 FP8LIN_ERR_ARGUMENT, "paged layout: null pointer");
         check_requests(requests, tokens);
         check_pages(width, page_size);
-        require(free_count >= 0 && free_count < kMaxDim && table_ld >= width && new_table_ld >= width, FP8LIN_ERR_SHAPE,
-                "paged layout: invalid table strides or free list");
+        require(free_count >= 0 && free_count < kMaxDim && table_ld >= width && new_table_ld >= width && table_ld < kMaxStride &&
+                    new_table_ld < kMaxStride,
+                FP8LIN_ERR_SHAPE, "paged layout: invalid table strides or free list");
         require(new_table != table || new_table_ld == table_ld, FP8LIN_ERR_ARGUMENT,
                 "paged layout: a table written in place keeps its stride");
-        check_workspace(workspace, workspace_bytes, fp8lin::paged_layout_ws_bytes(requests, new_table == table), "paged layout: workspace too small");
+        const size_t need = fp8lin::paged_layout_ws_bytes(requests, new_table == table);
+        check_workspace(workspace, workspace_bytes, need, "paged layout: workspace too small");
+        // workgroups read every request's lengths and table entries and the
+        // cursor while others write theirs
+        const Extent old_rows{table, requests, 4 * width, 4 * table_ld}, new_rows{new_table, requests, 4 * width, 4 * new_table_ld};
+        const Extent held = new_table == table ? Extent{} : old_rows;
+        require_apart({extent(offsets, requests + 1, 4), extent(new_lengths, requests, 4), extent(slots, tokens, 8),
+                       extent(positions, tokens, 8), new_rows, extent(new_cursor, 1, 4), extent(workspace, (int64_t)need, 1)},
+                      {extent(lengths, requests, 4), extent(counts, requests, 4), held, extent(free_pages, free_count, 4),
+                       extent(cursor, 1, 4)},
+                      "paged layout: an output overlaps an input or another output (only new_table may be table)");
         ensure_device();
         check_hip(fp8lin::launch_paged_layout(lengths, counts, table, table_ld, free_pages, free_count, cursor, (int)requests,
                                               (int)width, page_bits(page_size), tokens, offsets, new_lengths, slots, positions,

@@ -60,9 +60,9 @@ def paged_layout(lengths, counts, block_table, free_pages, tokens, page_size, cu
     from index cursor[0] on, in the order of the requests.  tokens: rows of the
     step's token tensors, at least the sum of the counts; rows behind the last
     request get slot -1 and position 0.  Returns a PagedLayout: its block_table
-    is a new tensor, or `out`, which may be block_table itself; its cursor goes
-    into the next call and is above len(free_pages) when pages were short (their
-    tokens have slot -1)."""
+    is a new tensor, or `out`, which may be block_table itself (and overlap no
+    other input); its cursor goes into the next call and is above
+    len(free_pages) when pages were short (their tokens have slot -1)."""
     if not (_is_dev(block_table) and block_table.dtype is _i32 and block_table.dim() == 2 and block_table.stride(1) == 1):
         _fail(ERR_ARGUMENT, "Invalid block table")
     device, (requests, width) = block_table.device, block_table.shape

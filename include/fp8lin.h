@@ -561,8 +561,10 @@ typedef struct fp8lin_paged_cache {
  *       page (none left, a negative id, a position past the table); rows from
  *       offsets[requests] on: slot -1, position 0; rows past `tokens` are dropped;
  *   new_table [requests, width]  the table with the pages taken, which may be
- *       `table` itself (in_place; it may overlap no other argument);
+ *       `table` itself (in_place);
  *   new_cursor [1]  cursor + pages wanted: above free_count, the list was short.
+ * No output may overlap an input or another output, but new_table == table:
+ * FP8LIN_ERR_ARGUMENT (lengths and cursor are advanced by a copy afterwards).
  * Page ids are not checked here; fp8lin_paged_append and
  * fp8lin_paged_attention check them.  0 < requests <= 4096; width * page_size
  * <= 2^30.
