@@ -1206,13 +1206,20 @@ int fp8lin_verify_drafts(const void* logits, int logits_f32, int64_t logits_ld, 
                          fp8lin_stream_t stream) {
     return guarded([&] {
         check_requests(requests, rows);
-        require(vocab > 0 && vocab < kMaxDim - 65536 && logits_ld >= vocab && (!draft_probs || draft_ld >= vocab) &&
-                    prob_rows >= 0,
+        require(vocab > 0 && vocab < kMaxDim - 65536 && logits_ld >= vocab && logits_ld < kMaxStride &&
+                    (!draft_probs || (draft_ld >= vocab && draft_ld < kMaxStride)) && prob_rows >= 0 && prob_rows < kMaxDim,
                 FP8LIN_ERR_SHAPE, "verify drafts: invalid vocabulary or row strides");
         require(offsets && accepted && (rows == 0 || (logits && tokens && uniforms && out)), FP8LIN_ERR_ARGUMENT,
                 "verify drafts: null pointer");
-        check_workspace(workspace, workspace_bytes, fp8lin::verify_ws_bytes(rows, requests, vocab),
-                        "verify drafts: workspace too small");
+        const size_t need = fp8lin::verify_ws_bytes(rows, requests, vocab);
+        check_workspace(workspace, workspace_bytes, need, "verify drafts: workspace too small");
+        // a row's token is written while others are read
+        const int64_t size = logits_f32 ? 4 : 2;
+        require_apart({extent(accepted, requests, 4), extent(out, rows, 8), extent(workspace, (int64_t)need, 1)},
+                      {Extent{logits, rows, size * vocab, size * logits_ld},
+                       Extent{draft_probs, prob_rows, 4 * vocab, 4 * draft_ld}, extent(tokens, rows, 8), extent(uniforms, rows, 4),
+                       extent(offsets, requests + 1, 4), extent(temperature, requests, 4)},
+                      "verify drafts: an output or the workspace overlaps an input or another output");
         ensure_device();
         check_hip(fp8lin::launch_verify(logits, logits_f32 == 0, logits_ld, draft_probs, draft_ld, prob_rows, tokens, uniforms,
                                         offsets, temperature, rows, (int)requests, (int)vocab, accepted, out, workspace,

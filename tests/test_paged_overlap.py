@@ -51,3 +51,38 @@ def test_layout_takes_what_is_apart(fp8lin, change):
 @pytest.mark.parametrize("change", [dict(table_ld=1 << 62), dict(new_table_ld=1 << 62), dict(table_ld=1 << 56)], ids=str)
 def test_layout_refuses_strides_past_64_bits(fp8lin, change):
     assert layout(fp8lin, **change) == 1
+
+
+VERIFY = "logits logits_f32 logits_ld draft_probs draft_ld prob_rows tokens uniforms offsets temperature requests rows vocab accepted " \
+         "out workspace workspace_bytes stream".split()
+
+
+def verify(fp8lin, **kw):
+    d = dict(zip(VERIFY, [A, 0, 100, A + 0x10000, 100, 5, A + 0x20000, A + 0x21000, A + 0x22000, A + 0x23000, 2, 7, 100, A + 0x24000,
+                          A + 0x25000, A + 0x30000, 1 << 30, None]))
+    d.update(kw)
+    return fp8lin.lib().fp8lin_verify_drafts(*[d[k] for k in VERIFY])
+
+
+@pytest.mark.parametrize("change", [
+    dict(out=A + 0x20000), dict(out=A + 0x20000 + 8), dict(out=A + 0x20000 - 8), dict(out=A + 0x21000), dict(out=A + 0x22000 - 48),
+    dict(out=A), dict(out=A + 0x10000 + 1992), dict(accepted=A + 0x20000 + 52), dict(accepted=A + 0x22000 + 8), dict(accepted=A + 0x23000),
+    dict(accepted=A + 0x25000), dict(out=A + 0x30000), dict(workspace=A + 0x20000), dict(workspace=A),
+], ids=str)
+def test_verify_refuses_shared_memory(fp8lin, change):
+    assert verify(fp8lin, **change) == 2
+    assert b"overlaps" in fp8lin.lib().fp8lin_last_error()
+
+
+@pytest.mark.parametrize("change", [{}, dict(out=A + 0x20000 + 56), dict(accepted=A + 0x22000 + 12), dict(temperature=None),
+                                    dict(draft_probs=None, out=A + 0x10000), dict(logits_ld=200, out=A + 216)], ids=str)
+def test_verify_takes_what_is_apart(fp8lin, change):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the call would launch")
+    assert accepted(verify(fp8lin, **change))
+
+
+@pytest.mark.parametrize("change", [dict(logits_ld=1 << 62), dict(draft_ld=1 << 61), dict(prob_rows=1 << 40)], ids=str)
+def test_verify_refuses_strides_past_64_bits(fp8lin, change):
+    assert verify(fp8lin, **change) == 1
