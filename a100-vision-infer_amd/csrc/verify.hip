@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(Args g) {
     __shared__ Stat part[kThreads / 64];
     const int64_t row = blockIdx.x;
     const int slice = blockIdx.y, tid = threadIdx.x;
-    if (row >= g.offsets[g.B]) return;  // behind the last request
+    if (row < g.offsets[0] || row >= g.offsets[g.B]) return;  // of no request
     const int b = owner_of(g, row);
     const double s = slope(temperature(g, b));
     const int64_t draft = DIRECT && row + 1 < g.offsets[b + 1] ? g.tokens[min(row + 1, g.T - 1)] : -1;
@@ -245,14 +245,15 @@ struct Decision {
 };
 
 // The draft model's rows are those of all requests but their last ones: the
-// request's first is a less the requests before it that have rows.
+// request's first is a, less the rows before the first request and the requests
+// before it that have rows.
 __device__ int64_t probs_row(const Args& g, int b, const Request& r) {
     int64_t before = 0;
     for (int i0 = 0; i0 < b; i0 += kThreads) {
         const int i = i0 + threadIdx.x;
         before += __syncthreads_count(i < b && request(g, i).n > 0);
     }
-    return r.a - before;
+    return r.a - request(g, 0).a - before;
 }
 
 // By all threads of a workgroup: wave w tests drafts w, w + 4, ...
@@ -388,7 +389,8 @@ __device__ __forceinline__ double wave_scan64(double v) {
     return v;
 }
 
-// One workgroup per request; the last one also clears the rows behind them.
+// One workgroup per request; the first and last ones also clear the rows before
+// and behind them.
 // DIRECT: without draft probabilities; the slices are the rows'.
 template <class T, bool VEC, bool DIRECT>
 __global__ __launch_bounds__(kThreads) void verify_draw_kernel(Args g) {
@@ -396,6 +398,8 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(Args g) {
     __shared__ int slice_s, pick_s, last_s;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Request r = request(g, b);
+    if (b == 0)
+        for (int64_t i = tid; i < r.a; i += kThreads) g.out[i] = -1;
     if (b == g.B - 1)
         for (int64_t i = r.a + r.n + tid; i < g.T; i += kThreads) g.out[i] = -1;
     if (r.n == 0) {

@@ -630,7 +630,8 @@ int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, i
  * from p of the last row: the first index whose running sum of weights exceeds
  * the number times their sum.
  *   accepted [requests]: drafts kept; out [rows]: the kept drafts, the next
- *   token, then -1 (as in rows behind the last request).
+ *   token, then -1 (as in rows of no request, before the first or behind the
+ *   last one).
  * A row without a distribution (NaN, +inf, all -inf) keeps no draft and draws
  * -1; a draft outside [0, vocab) is refused.  64-bit sums.  0 < requests <=
  * 4096; vocab < 2^31 - 65536.  No output may overlap an input or another output:

@@ -1,7 +1,12 @@
 """Calls of the paged-cache operators on the GPU that a server makes beside the plain ones: operands that share memory, batches
 with rows of no request, prompts beside drafted requests."""
+import random
+
 import pytest
 import torch
+
+import paged_oracle as PO
+from test_gpu_paged import _drafted
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +25,35 @@ def test_layout_refuses_a_table_over_its_inputs(fp8lin, gpu):
     # one page for position 3, then entry 2 for positions 40 and 41
     assert got.block_table.tolist() == [[0] + [-1] * 7, [-1, -1, 1] + [-1] * 5] and got.slots.tolist() == [3, 24, 25]
     assert (wide[:, :8] == -1).all()
+
+
+def _verify(fp8lin, logits, tokens, u, offsets, q=None, temperature=None):
+    """fp8lin_verify_drafts into memory that holds other numbers."""
+    rows, vocab = logits.shape
+    dev, requests = logits.device, len(offsets) - 1
+    off = torch.tensor(offsets, dtype=torch.int32, device=dev)
+    accepted, out = torch.full((requests,), 77, dtype=torch.int32, device=dev), torch.full((rows,), 77, dtype=torch.int64, device=dev)
+    need = fp8lin.lib().fp8lin_verify_drafts_workspace_bytes(requests, rows, vocab)
+    ws = torch.full((need,), 0x7f, dtype=torch.uint8, device=dev)
+    rc = fp8lin.lib().fp8lin_verify_drafts(
+        logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), None if q is None else q.data_ptr(), vocab,
+        0 if q is None else q.size(0), tokens.data_ptr(), u.data_ptr(), off.data_ptr(),
+        None if temperature is None else temperature.data_ptr(), requests, rows, vocab, accepted.data_ptr(), out.data_ptr(),
+        ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    return accepted.tolist(), out.tolist()
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("before,behind", [(0, 3), (1, 0), (5, 2), (200, 1)])
+def test_verify_rows_of_no_request(fp8lin, gpu, before, behind, probs):
+    """Rows before the first request and behind the last one: token -1, and the draft model's rows are those of the requests."""
+    rng = random.Random(before)
+    logits, tokens, u, offsets, q = _drafted(rng, 6, 3, 700, probs, torch.float32, 40 + before)
+    g = torch.Generator().manual_seed(3)
+    pad = lambda x, n: torch.rand(n, *x.shape[1:], generator=g).to(x.dtype)
+    logits, tokens, u = [torch.cat([pad(x, before), x, pad(x, behind)]) for x in (logits, tokens, u)]
+    offsets = [before + o for o in offsets]
+    want = PO.verify(logits, tokens, u, offsets, q, None)
+    got = _verify(fp8lin, logits.to(gpu), tokens.to(gpu), u.to(gpu), offsets, None if q is None else q.to(gpu))
+    assert got == want
