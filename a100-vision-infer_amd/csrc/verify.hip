@@ -180,7 +180,8 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(Args g) {
     if (row < g.offsets[0] || row >= g.offsets[g.B]) return;  // of no request
     const int b = owner_of(g, row);
     const double s = slope(temperature(g, b));
-    const int64_t draft = DIRECT && row + 1 < g.offsets[b + 1] ? g.tokens[min(row + 1, g.T - 1)] : -1;
+    const Request r = request(g, b);
+    const int64_t draft = DIRECT && row + 1 < r.a + r.n ? g.tokens[row + 1] : -1;
     const int x_col = draft >= 0 && draft < g.V ? (int)draft : -1;
     const int lo = slice * g.per, hi = min(lo + g.per, g.V);
     const T* logits = static_cast<const T*>(g.logits) + row * g.ld;

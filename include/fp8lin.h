@@ -617,9 +617,10 @@ int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, i
                            fp8lin_stream_t stream);
 
 /* Verification of drafted tokens.  Request b has rows offsets[b] ..
- * offsets[b+1] of logits [rows, vocab] (BF16, or FP32 with logits_f32): the
- * target's after its last token and after each draft; tokens [rows] are the
- * tokens that were fed in, so draft i of the request is tokens[offsets[b] + i].
+ * offsets[b+1] (cut to `rows`) of logits [rows, vocab] (BF16, or FP32 with
+ * logits_f32): the target's after its last token and after each draft; tokens
+ * [rows] are the tokens that were fed in, so draft i of the request is
+ * tokens[offsets[b] + i].
  * With p = softmax(logits / temperature[b]) (null: 1; 0: the most likely token,
  * lowest index of equal ones) and q the draft model's distribution,
  * draft_probs [prob_rows, vocab] (FP32; the rows of all requests but each one's

@@ -57,3 +57,24 @@ def test_verify_rows_of_no_request(fp8lin, gpu, before, behind, probs):
     want = PO.verify(logits, tokens, u, offsets, q, None)
     got = _verify(fp8lin, logits.to(gpu), tokens.to(gpu), u.to(gpu), offsets, None if q is None else q.to(gpu))
     assert got == want
+
+
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_offsets_past_the_rows(fp8lin, gpu, probs):
+    """A last request that is cut by the number of rows (a layout of fewer token rows than new tokens) is one of the rows that are
+    there: its last row draws, over all columns."""
+    vocab, rows = 5000, 7
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(rows, vocab, generator=g)
+    tokens = torch.randint(0, vocab, (rows,), generator=g)
+    for i in range(rows):  # each row's own token is likely: where it is taken for the row's draft, its weight is missing
+        x[i, tokens[i]] = 12.0
+    x[[3, 4, 5], tokens[4:7]] = 30.0
+    q = torch.softmax(torch.randn(rows - 2, vocab, generator=g), 1) if probs else None
+    for i in range(8):
+        u = torch.rand(rows, generator=g)
+        want = PO.verify(x, tokens, u, [0, 3, rows], q, None)
+        for end in (rows + 1, rows + 5, 1 << 30):
+            got = _verify(fp8lin, x.to(gpu), tokens.to(gpu), u.to(gpu), [0, 3, end], None if q is None else q.to(gpu))
+            assert got == want, (i, end)
+        assert want[0][1] == 3 or probs
