@@ -282,14 +282,14 @@ __device__ Decision decide(const Args& g, int b, const Request& r) {
             if constexpr (sizeof(T) == 2) at = bf16_bits_to_f32(logits[in ? x : 0]);
             else at = logits[in ? x : 0];
             const int64_t qr = probs + i;
-            const bool q_in = g.probs && in && qr >= 0 && qr < g.prob_rows;
-            const double q = q_in ? (double)g.probs[qr * g.ldp + x] : g.probs ? 0.0 : 1.0;
+            const bool given = !g.probs || (qr >= 0 && qr < g.prob_rows);
+            const double q = g.probs && in && given ? (double)g.probs[qr * g.ldp + x] : 1.0;
             const double u = (double)g.u[row];
             Stat v = row_stat(g, e, row, s);
             const double at_x = in ? weigh(e, at, v.m == -__builtin_inff() ? 0.0f : v.m, s) : 0.0;
             if (!g.probs) v.sum += at_x;
             const double p = greedy(t) ? (v.at == x ? 1.0 : 0.0) : at_x / v.sum;
-            const bool keep = in && valid(v) && u * q < p;
+            const bool keep = in && given && valid(v) && u * q < p;
             if ((tid & 63) == 0) {
                 stats[wave] = v;
                 drafts[wave] = at_x;

@@ -199,8 +199,8 @@ def verify_drafts(logits, tokens, uniforms, offsets, draft_probs=None, temperatu
     its drafts; tokens (int64 [rows]) were fed in, so its drafts are tokens but
     its first row's.  uniforms (float32 [rows], in [0, 1)): a row's number
     decides its draft, a request's last one draws its next token.
-    draft_probs (float32 [rows - requests, vocab]): the draft model's
-    distributions, the rows of all requests but each one's last; None: drafts
+    draft_probs (float32 [drafts, vocab]): the draft model's distributions, the
+    rows of all requests but each one's last, in order; None (or no row): drafts
     without probabilities.  temperature (float32 [requests], 0: the most likely
     token).  Returns (accepted int32 [requests], out int64 [rows]: per request
     the drafts kept, the next token, then -1)."""

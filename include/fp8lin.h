@@ -634,7 +634,8 @@ int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, i
  *   token, then -1 (as in rows of no request, before the first or behind the
  *   last one).
  * A row without a distribution (NaN, +inf, all -inf) keeps no draft and draws
- * -1; a draft outside [0, vocab) is refused.  64-bit sums.  0 < requests <=
+ * -1; a draft outside [0, vocab) is refused, and one whose row of draft_probs is
+ * missing (the token is drawn from p then).  64-bit sums.  0 < requests <=
  * 4096; vocab < 2^31 - 65536.  No output may overlap an input or another output:
  * FP8LIN_ERR_ARGUMENT.  Workspace: the bytes below, 16-byte aligned, any content.
  */

@@ -78,3 +78,22 @@ def test_verify_offsets_past_the_rows(fp8lin, gpu, probs):
             got = _verify(fp8lin, x.to(gpu), tokens.to(gpu), u.to(gpu), [0, 3, end], None if q is None else q.to(gpu))
             assert got == want, (i, end)
         assert want[0][1] == 3 or probs
+
+
+@pytest.mark.parametrize("rows,given", [(4, 1), (4, 2), (6, 3), (2, 1)])
+def test_verify_drafts_without_a_row(fp8lin, gpu, rows, given):
+    """Fewer rows of draft probabilities than drafts: a draft without one is refused and the token drawn from p, as if the request
+    ended there."""
+    vocab = 900
+    g = torch.Generator().manual_seed(rows)
+    for i in range(12):
+        x = torch.randn(rows, vocab, generator=g)
+        tokens, u = torch.randint(0, vocab, (rows,), generator=g), torch.rand(rows, generator=g)
+        x[torch.arange(rows - 1), tokens[1:]] = 9.0
+        q = torch.softmax(x[:-1] + 0.5 * torch.randn(rows - 1, vocab, generator=g), 1)
+        short = u[:given + 1].clone()
+        short[given] = u[-1]
+        kept, out = PO.verify(x[:given + 1], tokens[:given + 1], short, [0, given + 1], q, None)
+        want = kept, out + [-1] * (rows - given - 1)
+        got = _verify(fp8lin, x.to(gpu), tokens.to(gpu), u.to(gpu), [0, rows], q[:given].contiguous().to(gpu))
+        assert got == want, i
