@@ -215,7 +215,8 @@ class LinearEngine:
         linear(o_proj); the cross-rank reduce is the caller's.  layout: the
         step's PagedLayout (paged_layout).  positions int64 [3, tokens]: the
         mRoPE positions (default: layout.positions on every axis).  The gate
-        and the values are read where the projection wrote them."""
+        and the values are read where the projection wrote them.  Rows of no
+        request (behind the last one) come out as o_proj of zeros."""
         projected = self.linear(x, prefix + ".qkv_gate")
         T, H, HK, D = projected.size(0), heads, kv_heads, head_dim
         if projected.size(-1) != 2 * (H + HK) * D:
@@ -228,8 +229,9 @@ class LinearEngine:
         gate = projected[:, :2 * H * D].view(T, H, 2 * D)[..., D:]
         v = projected[:, (2 * H + HK) * D:].view(T, HK, D)
         paged_append(k, v, layout.slots, k_cache, v_cache, k_scale=k_scale, v_scale=v_scale)
+        # the attention leaves rows of no request as they are: zeros, not what the memory held
         core = paged_attention(q, k_cache, v_cache, layout.block_table, layout.offsets, layout.lengths, max_count=max_count,
-                               gate=gate, k_scale=k_scale, v_scale=v_scale)
+                               gate=gate, k_scale=k_scale, v_scale=v_scale, out=torch.zeros_like(q))
         return self.linear(core.view(T, H * D), prefix + ".o_proj")
 
     # -- steps -----------------------------------------------------------------

@@ -1,12 +1,14 @@
 """Calls of the paged-cache operators on the GPU that a server makes beside the plain ones: operands that share memory, batches
 with rows of no request, prompts beside drafted requests."""
+import math
 import random
 
 import pytest
 import torch
 
 import paged_oracle as PO
-from test_gpu_paged import _drafted
+import paged_values as PV
+from test_gpu_paged import _drafted, _Server
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +99,57 @@ def test_verify_drafts_without_a_row(fp8lin, gpu, rows, given):
         want = kept, out + [-1] * (rows - given - 1)
         got = _verify(fp8lin, x.to(gpu), tokens.to(gpu), u.to(gpu), [0, rows], q[:given].contiguous().to(gpu))
         assert got == want, i
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_full_attention_is_its_parts(fp8lin, gpu, fp8):
+    """LinearEngine.full_attention of prompts, then of drafted tokens with rows of no request, against q, gate, k and v from
+    full_attention_inputs: the cache's contents, 64-bit attention and a 64-bit product with o_proj's weights; rows of no request
+    give zeros, whatever the memory held."""
+    s = _Server(fp8lin, gpu, 3, fp8)
+    H, HK, D = s.H, s.HK, s.D
+    ints = dict(dtype=torch.int32, device=gpu)
+    g = torch.Generator().manual_seed(8)
+    codes, scale = s.eng.weights[s.P + ".o_proj.weight"].data, s.eng.weights[s.P + ".o_proj.weight"].scale
+    w = codes.cpu().view(torch.float8_e4m3fn).double() * scale.cpu().double().view(codes.size(0), -1).repeat_interleave(128, 1)[:, :H * D] \
+        if scale.dim() == 2 else codes.cpu().view(torch.float8_e4m3fn).double() * scale.cpu().double()[:, None]
+    slots = {}
+    for counts, extra in (([40, 17, 5], 0), ([3, 1, 4], 6), ([0, 1, 1], 30)):
+        tokens = torch.randint(0, s.V, (sum(counts) + extra,), generator=g).to(gpu)
+        x = s.embed[tokens]
+        lay = fp8lin.paged_layout(s.lengths, torch.tensor(counts, **ints), s.table, s.free, tokens.numel(), s.PAGE, cursor=s.cursor, out=s.table)
+        s.cursor.copy_(lay.cursor)
+        junk = [torch.full((tokens.numel(), H, D), math.nan, dtype=torch.bfloat16, device=gpu) for _ in range(8)]
+        del junk  # what the next tensors of this size hold
+        args = (lay, *s.caches, *s.norms, H, HK, D, s.ROPE, 1e-6)
+        y = s.eng.full_attention(x, s.P, *args, max_count=max(counts), **s.scales)
+        pos = lay.positions.repeat(3, 1)
+        again = s.eng.full_attention(x, s.P, *args, max_count=max(counts), positions=pos, **s.scales)
+        assert torch.equal(y.view(torch.int16), again.view(torch.int16))
+        q, gate, k, v = [t.cpu() for t in s.eng.full_attention_inputs(x, s.P, pos, *s.norms, H, HK, D, s.ROPE, 1e-6)]
+        total = sum(counts)
+        for i, slot in enumerate(lay.slots.tolist()[:total]):
+            slots[slot] = k[i], v[i]
+        caches = [c.cpu() for c in s.caches]
+        for slot, rows in slots.items():
+            for cache, row, name in zip(caches, rows, ("k_scale", "v_scale")):
+                if fp8:
+                    row = (row.float() / s.scales[name].cpu()[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+                assert torch.equal(cache[slot // s.PAGE, slot % s.PAGE].float(), row.float())
+        sc = {n: t.cpu() for n, t in s.scales.items()}
+        core, bound, rows = PV.attention(q, *caches, lay.block_table.cpu(), lay.offsets.tolist(), lay.lengths.tolist(),
+                                         gate=gate.view(-1, H, D), **sc)
+        assert rows.tolist() == [True] * total + [False] * extra
+        core, bound = core.flatten(1), bound.flatten(1)
+        # the operand's own bound; weights rounded to BF16 by some paths, FP32 sums, the result's rounding
+        mass = core.abs() @ w.abs().t()
+        off = bound @ w.abs().t() + (PO.BF16_HALF + 2 * PO.F32_HALF * H * D) * mass * 1.01
+
+        def beyond(core):
+            want = core @ w.t()
+            return float(((y.double().cpu() - want).abs() - off - PO.BF16_HALF * want.abs() * 1.02)[:total].max())
+        assert beyond(core) <= 0
+        # a mistake of the heads' order, or of the dimensions', would show
+        assert beyond(core.view(-1, H, D).roll(1, 1).flatten(1)) > 0 and beyond(core.view(-1, H, D).roll(1, 2).flatten(1)) > 0
+        assert (y[total:] == 0).all()
+        s.lengths.copy_(lay.lengths)
