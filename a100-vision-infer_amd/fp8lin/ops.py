@@ -308,7 +308,8 @@ def qk_norm_rope(projected, q_norm, k_norm, positions, heads, kv_heads, head_dim
     [T, H, D] = rope(rms(query heads, q_norm)) and k [T, HK, D] =
     rope(rms(key heads, k_norm)) with the centered RMSNorm, in one launch.
     Equal bit for bit to fused_rms of the query (key) heads followed by
-    fused_rope."""
+    fused_rope.  Positions that are one row expanded over the three axes are
+    read as that row."""
     H, HK, D = int(heads), int(kv_heads), int(head_dim)
     ok = (_is_dev(projected) and projected.dim() == 2 and projected.dtype == torch.bfloat16 and
           projected.stride(1) == 1 and H > 0 and HK > 0 and 0 < D <= 512 and
@@ -319,8 +320,11 @@ def qk_norm_rope(projected, q_norm, k_norm, positions, heads, kv_heads, head_dim
                      w.is_contiguous() and w.numel() == D)
     if not ok:
         _fail(ERR_ARGUMENT, "Invalid Q/K norm + RoPE input")
-    positions = positions.contiguous()
     T = projected.size(0)
+    if positions.stride(0) == 0 and (T <= 1 or positions.stride(1) == 1):
+        height_section = width_section = 0  # every pair takes axis 0, the only one that is read then
+    else:
+        positions = positions.contiguous()
     q = torch.empty((T, H, D), dtype=torch.bfloat16, device=projected.device)
     k = torch.empty((T, HK, D), dtype=torch.bfloat16, device=projected.device)
     check(lib().fp8lin_qk_norm_rope(_ptr(projected), projected.stride(0), _ptr(q_norm), _ptr(k_norm),

@@ -386,7 +386,8 @@ int fp8lin_rope(const uint16_t* x, const int64_t* positions, uint16_t* y, int64_
  * the centered RMSNorm of fp8lin_rms and fp8lin_rope's rotation.  Bit-identical
  * to fp8lin_rms of the contiguous query (key) rows followed by fp8lin_rope.
  * The gate and value heads stay views of projected.  Requires H > 0, HK > 0,
- * D <= 512; eps is used as given, as by fp8lin_rms.
+ * D <= 512; eps is used as given, as by fp8lin_rms.  With height_section and
+ * width_section 0 only the first row of positions is read.
  * Replaces the optimized branch of src/engine.cpp:279-287 (norm(q_norm),
  * norm(k_norm), fused_rope(q), fused_rope(k)).
  */

@@ -153,3 +153,25 @@ def test_full_attention_is_its_parts(fp8lin, gpu, fp8):
         assert beyond(core.view(-1, H, D).roll(1, 1).flatten(1)) > 0 and beyond(core.view(-1, H, D).roll(1, 2).flatten(1)) > 0
         assert (y[total:] == 0).all()
         s.lengths.copy_(lay.lengths)
+
+
+@pytest.mark.parametrize("heads,tokens", [((4, 2, 64), 1), ((4, 2, 64), 3), ((12, 2, 256), 70), ((12, 2, 256), 2000)], ids=str)
+def test_positions_of_one_row(fp8lin, gpu, heads, tokens):
+    """Positions expanded over the axes: the same bits as three rows of them, and no copy of them is made."""
+    H, HK, D = heads
+    g = torch.Generator().manual_seed(tokens)
+    projected = torch.randn(tokens, 2 * (H + HK) * D, generator=g).to(torch.bfloat16).to(gpu)
+    norms = [(0.1 * torch.randn(D, generator=g)).to(torch.bfloat16).to(gpu) for _ in range(2)]
+    pos = torch.randint(0, 100000, (tokens,), generator=g).to(gpu)
+    rest = (H, HK, D, D // 4, 10000.0, D // 32 - 1, D // 32, 1e-6)
+    want = fp8lin.qk_norm_rope(projected, *norms, pos.repeat(3, 1), *rest)
+    got = fp8lin.qk_norm_rope(projected, *norms, pos.expand(3, tokens), *rest)
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(got, want))
+    expanded = pos.expand(3, tokens)
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    got = fp8lin.qk_norm_rope(projected, *norms, expanded, *rest)
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] - before == 2  # q and k, no positions
+    # a row that is no row of its own, strided: copied
+    two = torch.stack([pos, pos + 1], 1)
+    got = fp8lin.qk_norm_rope(projected, *norms, two[:, 0].expand(3, tokens), *rest)
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(got, want))
