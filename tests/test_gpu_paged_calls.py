@@ -175,3 +175,120 @@ def test_positions_of_one_row(fp8lin, gpu, heads, tokens):
     two = torch.stack([pos, pos + 1], 1)
     got = fp8lin.qk_norm_rope(projected, *norms, two[:, 0].expand(3, tokens), *rest)
     assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(got, want))
+
+
+class _Loop:
+    """A server's step of chunks and drafted requests together, every length on the GPU."""
+
+    def __init__(self, F, dev, requests):
+        self.s = _Server(F, dev, requests, False)
+        self.F, self.u = F, None
+
+    def step(self, tokens, counts, is_chunk, deciding, deciding_offsets, max_count):
+        s = self.s
+        layout = self.F.paged_layout(s.lengths, counts, s.table, s.free, tokens.numel(), s.PAGE, cursor=s.cursor, out=s.table)
+        x = s.eng.full_attention(s.embed[tokens], s.P, layout, *s.caches, *s.norms, s.H, s.HK, s.D, s.ROPE, 1e-6, max_count=max_count)
+        logits = s.eng.linear(x[deciding], "lm_head")
+        taken, out = self.F.verify_drafts(logits, tokens[deciding], self.u, deciding_offsets)
+        s.lengths.copy_(torch.where(is_chunk, layout.lengths, s.lengths + taken + (counts > 0)))
+        s.cursor.copy_(layout.cursor)
+        return logits, taken, out
+
+
+def test_chunks_beside_drafted_requests(fp8lin, gpu):
+    """Prompts that arrive in chunks while other requests verify drafts: every request's cache holds at the end what one prompt
+    of its tokens puts there."""
+    n, chunk = 3, 24
+    loop = _Loop(fp8lin, gpu, n)
+    s = loop.s
+    ints = dict(dtype=torch.int32, device=gpu)
+    g = torch.Generator().manual_seed(12)
+    prompts = [torch.randint(0, s.V, (c,), generator=g).tolist() for c in (100, 30, 7)]
+    fed, last, kept = [0] * n, [None] * n, [[] for _ in range(n)]
+    drafted_beside_chunk = 0
+    for i in range(10):
+        rows, deciding, parts, ends = [], [], [], []
+        for b in range(n):
+            a = sum(map(len, rows))
+            if fed[b] < len(prompts[b]):
+                new = prompts[b][fed[b]:fed[b] + chunk]
+                ends.append(fed[b] + len(new) == len(prompts[b]))
+                mine = [a + len(new) - 1] if ends[-1] else []
+            else:
+                new = [last[b]] + torch.randint(0, s.V, ((i + b) % 4,), generator=g).tolist()
+                ends.append(None)
+                mine = list(range(a, a + len(new)))
+            rows.append(new)
+            deciding += mine
+            parts.append(len(mine))
+        tokens = torch.tensor(sum(rows, []), device=gpu)
+        offsets = [sum(parts[:b]) for b in range(n + 1)]
+        counts = torch.tensor([len(r) for r in rows], **ints)
+        loop.u = torch.rand(len(deciding), generator=g).to(gpu)
+        logits, taken, out = loop.step(tokens, counts, torch.tensor([e is not None for e in ends], device=gpu),
+                                       torch.tensor(deciding, dtype=torch.int64, device=gpu), torch.tensor(offsets, **ints), chunk)
+        want = PO.verify(logits.cpu(), tokens[deciding].cpu(), loop.u.cpu(), offsets, None, None)
+        assert taken.tolist() == want[0] and out.tolist() == want[1]
+        drafted_beside_chunk += None in ends and any(e is not None for e in ends)
+        for b in range(n):
+            t, o = int(taken[b]), out.tolist()[offsets[b]:offsets[b + 1]]
+            if ends[b] is None:
+                kept[b] += [last[b]] + o[:t]
+                last[b] = o[t]
+            else:
+                kept[b] += rows[b]
+                fed[b] += len(rows[b])
+                if ends[b]:
+                    assert t == 0
+                    last[b] = o[0]
+        assert s.lengths.tolist() == [len(k) for k in kept]
+    assert drafted_beside_chunk > 2
+    t = _Server(fp8lin, gpu, n, False)
+    _, lay = t.step(torch.tensor(sum(kept, []), device=gpu), torch.tensor([len(k) for k in kept], **ints), max(map(len, kept)))
+    for b in range(n):
+        for cache, other in zip(s.caches, t.caches):
+            x, z = [PO.keys_of(c.cpu(), None, tab[b].cpu(), len(kept[b]), 1) for c, tab in ((cache, s.table), (other, lay.block_table))]
+            assert torch.isfinite(x).all()
+            assert float((x - z).norm() / z.norm()) <= torch.finfo(torch.bfloat16).eps
+
+
+def test_chunk_and_drafts_captured(fp8lin, gpu):
+    """The same step as one graph, replayed: the lengths advance by it, a chunk's by all its tokens, and equal the eager steps'."""
+    states = []
+    for form in ("eager", "graph"):
+        loop = _Loop(fp8lin, gpu, 2)
+        s = loop.s
+        ints = dict(dtype=torch.int32, device=gpu)
+        g = torch.Generator().manual_seed(5)
+        loop.u = torch.full((3,), 0.5, device=gpu)
+        tokens = torch.randint(0, s.V, (20 + 3 + 2,), generator=g).to(gpu)  # two rows of no request
+        args = (tokens, torch.tensor([20, 3], **ints), torch.tensor([True, False], device=gpu),
+                torch.tensor([20, 21, 22], device=gpu), torch.tensor([0, 0, 3], **ints), 20)
+        saved = [x.clone() for x in (s.lengths, s.cursor, s.table, *s.caches)]
+        if form == "graph":
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                loop.step(*args)
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                res = loop.step(*args)
+            for x, y in zip((s.lengths, s.cursor, s.table, *s.caches), saved):
+                x.copy_(y)
+        got = []
+        for i in range(5):
+            gi = torch.Generator().manual_seed(i)
+            loop.u.copy_(torch.rand(3, generator=gi))
+            tokens.copy_(torch.randint(0, s.V, (25,), generator=gi))
+            torch.cuda.synchronize()
+            if form == "graph":
+                graph.replay()
+            else:
+                res = loop.step(*args)
+            torch.cuda.synchronize()
+            got += [x.clone().cpu() for x in (*res, s.lengths, s.cursor, s.table)]
+            assert int(s.lengths[0]) == 20 * (i + 1) and int(s.lengths[1]) > i
+        states.append(got)
+    for x, y in zip(*states):
+        assert torch.equal(x.view(torch.int16) if x.dtype == torch.bfloat16 else x, y.view(torch.int16) if y.dtype == torch.bfloat16 else y)
