@@ -363,8 +363,8 @@ hipError_t run(const PagedAttention& a, bool with_join, hipStream_t stream) {
     static_assert(LDS >= PagedSplit<BM, 16, 0>::lds_bytes(kPagedMaxRequests), "the prefix of the requests' costs fits");
     static_assert(LDS >= kFewWaves * 16 * (D + 6) * 4, "the waves' sums fit");
     auto* kern = few_kernel<D, F8, NT>;
-    static const hipError_t attr =
-        hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    static OncePerDevice once;
+    const hipError_t attr = allow_lds(once, reinterpret_cast<const void*>(kern), LDS);
     if (attr != hipSuccess) return attr;
     hipLaunchKernelGGL(kern, dim3(kGroups), dim3(64 * kFewWaves), LDS, stream, a);
     hipError_t e = hipGetLastError();

@@ -545,8 +545,8 @@ template <int D, bool F8, int RB>
 hipError_t run(const PagedAttention& a, const PagedAttention* few, hipStream_t stream) {
     constexpr int LDS = std::max<int>(Tile<D, F8>::LDS, PagedSplit<kBM, kBN, 0>::lds_bytes(kPagedMaxRequests));
     auto* kern = tile_kernel<D, F8, RB>;
-    static const hipError_t attr =
-        hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    static OncePerDevice once;
+    const hipError_t attr = allow_lds(once, reinterpret_cast<const void*>(kern), LDS);
     if (attr != hipSuccess) return attr;
     hipLaunchKernelGGL(kern, dim3(kGroups), dim3(64 * kBM / (32 * RB)), LDS, stream, a);
     const hipError_t e = hipGetLastError();

@@ -3,7 +3,18 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "per_device.hpp"
+
 namespace fp8lin {
+
+// Dynamic LDS above the default limit needs an opt-in for each kernel (gfx950
+// has 160 KiB per workgroup), on every device that launches it.
+inline hipError_t allow_lds(OncePerDevice& once, const void* kern, int bytes) {
+    int dev = 0;
+    const hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    return (hipError_t)once(dev, [&] { return (int)hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+}
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -102,7 +102,8 @@ hipError_t run_fp8_mt(const uint16_t* x, const uint8_t* w, const float* scales, 
     using Gm = Geo<MT>;
     if (!Gm::SPLIT && plan.rtiles != 0) return hipErrorInvalidValue;
     auto kern = gemm_fp8_kernel<MT, SWIGLU>;
-    static const hipError_t attr = gemm::allow_lds(reinterpret_cast<const void*>(kern), Gm::LDS_BYTES);
+    static OncePerDevice once;
+    const hipError_t attr = allow_lds(once, reinterpret_cast<const void*>(kern), Gm::LDS_BYTES);
     if (attr != hipSuccess) return attr;
     const int grid = std::min(plan.units, G);
     hipLaunchKernelGGL(kern, dim3(grid), dim3(THREADS), Gm::LDS_BYTES, stream, x, w, scales, S, y, (int)ldy, M, N,

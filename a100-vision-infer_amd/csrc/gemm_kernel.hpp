@@ -396,12 +396,6 @@ __global__ __launch_bounds__(C::THREADS) void gemm_kernel(
     }
 }
 
-// Dynamic LDS above the default limit needs an explicit per-kernel opt-in
-// (once per process; gfx950 has 160 KiB per workgroup).
-inline hipError_t allow_lds(const void* kern, int bytes) {
-    return hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 // Whether the 16-byte loader takes these operands (raw buffers with 32-bit
 // byte offsets).
 inline bool aligned(const uint16_t* x, const void* w, bool fp8, int64_t M, int64_t N, int64_t K) {
@@ -417,7 +411,8 @@ hipError_t launch(const uint16_t* x, const void* w, const float* scales, int S, 
     const int ntiles = SWIGLU ? ((N >> 1) + C::BN / 2 - 1) / (C::BN / 2) : (N + C::BN - 1) / C::BN;
     const int per_xcd = (mtiles * ntiles + kXcds - 1) / kXcds;
     auto kern = gemm_kernel<C, FP8, GUARD, SWIGLU, GROUP_M, IGLP, PF, ST>;
-    static const hipError_t attr = allow_lds(reinterpret_cast<const void*>(kern), C::LDS_BYTES);
+    static OncePerDevice once;
+    const hipError_t attr = allow_lds(once, reinterpret_cast<const void*>(kern), C::LDS_BYTES);
     if (attr != hipSuccess) return attr;
     hipLaunchKernelGGL(kern, dim3(per_xcd * kXcds), dim3(C::THREADS), C::LDS_BYTES, stream, x, w, scales, S, bias, y,
                        ldy, M, N, K, mtiles, ntiles);

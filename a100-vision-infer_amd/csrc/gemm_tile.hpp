@@ -642,17 +642,14 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const float* __restri
     store8(dst, o, D - col, wide);
 }
 
-inline hipError_t allow_lds(const void* kern, int bytes) {
-    return hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 // The launch of config C over grid gr (part: splits > 1, gr.splits x M x
 // gr.ldp floats).
 template <class C, bool SWIGLU>
 hipError_t launch(const uint16_t* x, const void* w, const float* scales, int S, const uint16_t* bias, uint16_t* y,
                   int64_t ldy, int M, int N, int K, const Grid& gr, float* part, hipStream_t stream) {
     auto kern = gemm_tile_kernel<C, SWIGLU>;
-    static const hipError_t attr = allow_lds(reinterpret_cast<const void*>(kern), kLds);
+    static OncePerDevice once;
+    const hipError_t attr = allow_lds(once, reinterpret_cast<const void*>(kern), kLds);
     if (attr != hipSuccess) return attr;
     const int units = gr.mtiles * gr.nblocks * gr.splits;
     hipLaunchKernelGGL(kern, dim3((unsigned)((units + 7) / 8 * 8)), dim3(C::THREADS), C::LDS_BYTES, stream,

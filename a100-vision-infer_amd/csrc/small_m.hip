@@ -378,8 +378,8 @@ hipError_t launch(const uint16_t* x, const uint8_t* codes, const float* scales, 
                   int N, int K, int per, hipStream_t stream) {
     using C = SmallCfg<W, D, NBW, XA, MX, TL>;
     auto kern = small_m_kernel<W, D, NBW, XA, MX, SW, TL>;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds);
+    static OncePerDevice once;
+    const hipError_t attr = allow_lds(once, reinterpret_cast<const void*>(kern), kMaxLds);
     if (attr != hipSuccess) return attr;
     static_assert(C::KSPLIT, "rows per workgroup are set at run time only in the K-split form");
     const int tiles = SW ? (N / 2 + per - 1) / per : (N + per - 1) / per;
@@ -679,8 +679,8 @@ template <int NB, int D, bool SW, bool CAND, int T>
 hipError_t launch_stream(const uint16_t* x, const uint8_t* codes, const float* scales, uint16_t* y, int64_t ldy,
                          int M, int N, int K, int per, hipStream_t stream, uint32_t* part) {
     auto kern = small_m_stream_kernel<NB, D, SW, CAND, T>;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds);
+    static OncePerDevice once;
+    const hipError_t attr = allow_lds(once, reinterpret_cast<const void*>(kern), kMaxLds);
     if (attr != hipSuccess) return attr;
     const int units = SW ? N / 2 : N;
     const int groups = (units + per - 1) / per;
@@ -1029,8 +1029,8 @@ hipError_t launch_row_wide(const uint16_t* x, const uint8_t* codes, const float*
     auto kern = small_m_row_wide_kernel<NS, SW, NT, MX, D, KS>;
     constexpr int lds = wide_lds<NT, MX, D, KS>();
     static_assert(lds <= kMaxLds, "row-staged LDS");
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    static OncePerDevice once;
+    const hipError_t attr = allow_lds(once, reinterpret_cast<const void*>(kern), lds);
     if (attr != hipSuccess) return attr;
     hipLaunchKernelGGL(kern, dim3(groups), dim3(64 * kWideWaves), lds, stream, x, codes, scales, y, ldy, M, N, K);
     return hipGetLastError();
