@@ -1133,8 +1133,10 @@ int fp8lin_paged_append(const fp8lin_paged_cache* cache, const uint16_t* k, int6
         require(k && v && slots, FP8LIN_ERR_ARGUMENT, "paged append: null pointer");
         require(cache->head_dim % (cache->fp8 ? 16 : 8) == 0, FP8LIN_ERR_UNSUPPORTED,
                 "paged append: head_dim must be a multiple of 8 (16 in an 8-bit cache)");
-        require(tokens * (cache->kv_heads * cache->head_dim / 8) < ((int64_t)1 << 38), FP8LIN_ERR_SHAPE,
-                "paged append: too many values");
+        // a thread per 8 values of a grid below 2^32 threads, a token's values in 32 bits
+        require(cache->kv_heads * cache->head_dim < kMaxDim &&
+                    tokens <= (((int64_t)1 << 32) - 256) / (cache->kv_heads * cache->head_dim / 8),
+                FP8LIN_ERR_SHAPE, "paged append: too many values");
         ensure_device();
         check_hip(fp8lin::launch_paged_append(k, v, k_token, k_head, v_token, v_head, slots, kc, vc, cache->fp8 != 0,
                                               cache->k_scale, cache->v_scale, tokens, (int)cache->kv_heads,

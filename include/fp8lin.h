@@ -582,8 +582,10 @@ int fp8lin_paged_layout(const int32_t* lengths, const int32_t* counts, const int
  * last dimension contiguous) into their slots: BF16 as they are, 8-bit as
  * E4M3FN(x / scale), to nearest even, above 448 as 448, NaN as NaN.  A row
  * whose slot is outside [0, pages * page_size) is skipped.  Two rows of one
- * slot: it is not defined which of them each 8 values come from.  head_dim % 8
- * == 0 (16 in an 8-bit cache).
+ * slot: it is not defined which of them each 8 values come from; nor what a row
+ * of k or v gives that lies in a slot of the call.  head_dim % 8 == 0 (16 in an
+ * 8-bit cache); kv_heads * head_dim < 2^31, and times tokens / 8 at most
+ * 2^32 - 256.
  */
 int fp8lin_paged_append(const fp8lin_paged_cache* cache, const uint16_t* k, int64_t k_token, int64_t k_head,
                         const uint16_t* v, int64_t v_token, int64_t v_head, const int64_t* slots, int64_t tokens,
