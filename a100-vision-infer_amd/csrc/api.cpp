@@ -539,6 +539,7 @@ void check_cache(const fp8lin_paged_cache* c, fp8lin::PagedCache& k, fp8lin::Pag
     v = fp8lin::PagedCache{c->v, c->v_page, c->v_slot, c->v_head};
 }
 
+constexpr int64_t kMaxVerifyRows = (int64_t)1 << 24;  // 256 threads a row, a grid below 2^32
 constexpr int64_t kMaxStride = (int64_t)1 << 56;  // elements; bytes of it stay in 64 bits
 
 // Memory of an operand: `rows` rows of `width` bytes, `stride` bytes apart
@@ -1196,7 +1197,8 @@ int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, i
 }
 
 size_t fp8lin_verify_drafts_workspace_bytes(int64_t requests, int64_t rows, int64_t vocab) {
-    if (requests <= 0 || requests > FP8LIN_PAGED_MAX_REQUESTS || rows < 0 || rows >= kMaxDim || vocab <= 0 || vocab >= kMaxDim)
+    if (requests <= 0 || requests > FP8LIN_PAGED_MAX_REQUESTS || rows < 0 || rows >= kMaxVerifyRows || vocab <= 0 ||
+        vocab >= kMaxDim - 65536)
         return 0;
     return fp8lin::verify_ws_bytes(rows, requests, vocab);
 }
@@ -1208,6 +1210,7 @@ int fp8lin_verify_drafts(const void* logits, int logits_f32, int64_t logits_ld, 
                          fp8lin_stream_t stream) {
     return guarded([&] {
         check_requests(requests, rows);
+        require(rows < kMaxVerifyRows, FP8LIN_ERR_SHAPE, "verify drafts: more than 2^24-1 rows");
         require(vocab > 0 && vocab < kMaxDim - 65536 && logits_ld >= vocab && logits_ld < kMaxStride &&
                     (!draft_probs || (draft_ld >= vocab && draft_ld < kMaxStride)) && prob_rows >= 0 && prob_rows < kMaxDim,
                 FP8LIN_ERR_SHAPE, "verify drafts: invalid vocabulary or row strides");

@@ -639,8 +639,9 @@ int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, i
  * A row without a distribution (NaN, +inf, all -inf) keeps no draft and draws
  * -1; a draft outside [0, vocab) is refused, and one whose row of draft_probs is
  * missing (the token is drawn from p then).  64-bit sums.  0 < requests <=
- * 4096; vocab < 2^31 - 65536.  No output may overlap an input or another output:
- * FP8LIN_ERR_ARGUMENT.  Workspace: the bytes below, 16-byte aligned, any content.
+ * 4096; rows < 2^24; vocab < 2^31 - 65536.  No output may overlap an input or
+ * another output: FP8LIN_ERR_ARGUMENT.  Workspace: the bytes below, 16-byte
+ * aligned, any content.
  */
 size_t fp8lin_verify_drafts_workspace_bytes(int64_t requests, int64_t rows, int64_t vocab);
 int fp8lin_verify_drafts(const void* logits, int logits_f32, int64_t logits_ld, const float* draft_probs,
