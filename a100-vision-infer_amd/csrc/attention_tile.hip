@@ -18,12 +18,17 @@
 // 3913 tokens).  Heads of 256 take the whole register file: 256 accumulation
 // registers of O^T, 128 of queries, 32 of S^T, 32 of two steps' weights.
 //
-// With one wave per SIMD nothing else hides the softmax, so the steps are
-// skewed: the products of step s - 1 with V run while the weights of step s are
-// computed, a few vector instructions after each pair of MFMAs.  The MFMAs are
-// one asm statement each, in that order, with O in accumulation and S in vector
-// registers; the compiler keeps the order of the groups (sched_barrier) and
-// counts the LDS waits.
+// The steps are skewed: the products of step s - 1 with V are issued while the
+// weights of step s are computed.  The source spreads those a few vector
+// instructions behind each pair of MFMAs, in groups that sched_barrier keeps in
+// order, but nothing holds their results there: the compiler moves the 2^x, the
+// sums and the packing of a step past its MFMAs, behind the branch that rescales
+// O.  So softmax and MFMAs run one after the other in a wave (MFMAs busy in 42%
+// of the cycles of a prompt of 3913 tokens, heads of 256), and where two waves
+// share a SIMD (heads of 64 and 128) the counters show little of one's hidden
+// behind the other's (a mixed batch: MFMAs 37%, vector work some 47%).  The MFMAs
+// are one asm statement each, with O in accumulation and S in vector registers;
+// the compiler counts the LDS waits.
 //
 // K and V of a tile arrive by direct-to-LDS DMA into two buffers each, as they
 // are in the cache; the codes of an 8-bit cache are converted when a fragment
@@ -45,8 +50,9 @@ namespace {
 
 constexpr int kBM = kTileRows, kBN = 64, kKeys = 16;  // kKeys: keys of a tile that a wave brings
 // A unit's start and end, in keys (heads of 256: up to 30 us at 64 keys in 4 us).
-// With 192, 320, 448 and 640 at 256 a prompt of 3913 tokens takes 196, 161, 150
-// and 157 us, a chunk of 512 85, 86, 86 and 88.
+// With 192, 320, 448 and 640 at 256 a prompt of 3913 tokens takes 217, 173, 164
+// and 167 us, a chunk of 512 77, 78, 78 and 79, a mixed batch (heads of 128)
+// 170, 160, 153 and 150.
 template <int D>
 constexpr int kTileStart = 448 * D / 256;
 constexpr int kTileMinTiles = 4;
@@ -298,9 +304,11 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
             };
             // PV: O += P V of the last step (keys `sub` of the tile whose V is at
             // vb).  SM: the weights of this step (32 keys from key0), each stage
-            // a group behind the one before (scores less the maximum, 2^x, sums
-            // and packing), so that no instruction waits on the last one's
-            // result.  The first fragments of K's keys `ksub` at kb follow.
+            // (scores less the maximum, 2^x, sums and packing) written a group
+            // behind the one before, so that no instruction waits on the last
+            // one's result; the compiler keeps the stages' order, not their
+            // places between the MFMAs.  The first fragments of K's keys `ksub`
+            // at kb follow.
             // each(i): what else goes out with group i.
             auto weigh = [&](auto pv_, auto sm_, uint32_t vb, auto sub_, int key0, uint32_t kb, auto ksub_, auto each) {
                 constexpr bool PV = decltype(pv_)::value, SM = decltype(sm_)::value;
@@ -583,8 +591,8 @@ size_t paged_attention_ws_bytes(int D, int64_t max_rows) {
 // rows 61 and 65, 66 rows 89 and 67).  Where some request may have more than
 // kFewRows rows, a batch is computed in two: a request of a few rows in a
 // 256-row tile streams its keys at the pace of one wave's steps (13 requests,
-// three of them chunks of 400 to 700 tokens, 32/8 heads of 128: 162 us in two
-// against 187).  One launch joins both kernels' partial sums (168 us with two).
+// three of them chunks of 400 to 700 tokens, 32/8 heads of 128: 153 us in two
+// against 165).  One launch joins both kernels' partial sums: two cost 6 us more.
 hipError_t launch_paged_attention(PagedAttention a, int D, bool fp8, int64_t max_rows, hipStream_t stream) {
     a.rows_from = 0;
     a.rows_to = INT64_MAX;
