@@ -186,12 +186,13 @@ class _Loop:
 
     def step(self, tokens, counts, is_chunk, deciding, deciding_offsets, max_count):
         s = self.s
-        layout = self.F.paged_layout(s.lengths, counts, s.table, s.free, tokens.numel(), s.PAGE, cursor=s.cursor, out=s.table)
+        layout = self.F.paged_layout(s.lengths, counts, s.table, s.free, tokens.numel(), s.PAGE, cursor=s.cursor)
         x = s.eng.full_attention(s.embed[tokens], s.P, layout, *s.caches, *s.norms, s.H, s.HK, s.D, s.ROPE, 1e-6, max_count=max_count)
         logits = s.eng.linear(x[deciding], "lm_head")
         taken, out = self.F.verify_drafts(logits, tokens[deciding], self.u, deciding_offsets)
         s.lengths.copy_(torch.where(is_chunk, layout.lengths, s.lengths + taken + (counts > 0)))
         s.cursor.copy_(layout.cursor)
+        s.table.copy_(layout.block_table)
         return logits, taken, out
 
 
