@@ -28,7 +28,7 @@ def attention(q, k_cache, v_cache, table, offsets, lengths, gate=None, k_scale=N
             v = PO.keys_of(v_cache, v_scale, table[b], n, g // group)
             for i in range(a, e):
                 sees = min(max(n - (e - i) + 1, 0), n) if causal else n
-                x, sig = q[i, g].double(), 1.0 if gate is None else torch.sigmoid(gate[i, g].double())
+                x, sig = q[i, g].double(), torch.ones(d).double() if gate is None else torch.sigmoid(gate[i, g].double())
                 s = (k[:sees] * x).sum(1) * scale
                 bound[i, g] = 1e-37
                 if not sees or bool((s == -math.inf).all()):
@@ -44,10 +44,10 @@ def attention(q, k_cache, v_cache, table, offsets, lengths, gate=None, k_scale=N
                 odd = ~torch.isfinite(vi)
                 for j in odd.any(1).nonzero()[:, 0].tolist():
                     o = torch.where(odd[j], o + w[j] * vi[j], o)
-                spread = float((torch.where(torch.isfinite(s)[:, None], k[:sees], 0.0).abs() * x.abs()).sum(1).max()) * scale
+                spread = float((k[:sees].abs() * x.abs()).sum(1)[torch.isfinite(s)].max()) * scale
                 weight = BF16_HALF + 2 * F32_HALF * ((d + 2) * spread + n + 600)
                 out[i, g] = o * sig
-                o = torch.where(torch.isfinite(o), o, 0.0)
+                o, sig = torch.where(torch.isfinite(o * sig), o, 0.0), torch.where(torch.isfinite(o * sig), sig, 0.0)
                 bound[i, g] += sig * (weight * mass + 8 * F32_HALF * o.abs()) * 1.01 + BF16_HALF * (o * sig).abs() * 1.01
     return out, bound, rows
 

@@ -93,3 +93,30 @@ def test_attention_keeps_nan(fp8lin, gpu, what, count, heads, fp8):
             want = expect(b, causal=False)
         got = fp8lin.paged_attention(max_count=count, causal=causal, **b.up(gpu))
         assert PV.compare(got, want, f"causal={causal}") == odd.numel() - int(odd.sum())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads", [(12, 2, 256), (4, 4, 64), (6, 1, 128)], ids=str)
+@pytest.mark.parametrize("count", [3, 1000])
+def test_attention_of_infinite_scores_and_gates(fp8lin, gpu, count, heads, fp8):
+    """Infinities in queries, keys (BF16) and gates: +inf among a row's scores makes it NaN, -inf a weight of 0, nothing but -inf a row
+    of zeros; gates of either infinity and NaN."""
+    held = [(900, 2), (40, 3), (1, 1), (300, 1)] if count == 3 else [(900, 200), (70, 70), (5, 2)]
+    b = Batch(held, *heads, page=16, fp8=fp8, gate=True, seed=23)
+    h, hk, dim = heads
+    b.q[0, 0, 2] = INF                                   # every score an infinity of the key's sign, or NaN
+    b.q[b.offsets[1], h - 1] = 0.0
+    b.q[b.offsets[1], h - 1, 1] = -INF                   # infinities and, of the zeros, nothing else
+    if not fp8:
+        put(b, b.k, 0, 17, hk - 1, 3, INF)
+        put(b, b.k, 1, 4, 0, 1, -INF)
+        for at in range(held[-1][0]):                    # one head whose every key is infinite: scores of one sign a row
+            put(b, b.k, len(held) - 1, at, 0, 0, -INF)
+    b.gate[1, :, 0], b.gate[1, :, 1], b.gate[1, :, 2] = INF, -INF, NAN
+    want = expect(b)
+    got = fp8lin.paged_attention(max_count=count, **b.up(gpu))
+    compared = PV.compare(got, want)
+    assert 0 < compared < want[0][want[2]].numel()
+    if not fp8:
+        last = want[0][b.offsets[-2]:b.offsets[-1], :h // hk]
+        assert ((last == 0).all(-1) | torch.isnan(last).all(-1)).all()
