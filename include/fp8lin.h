@@ -604,8 +604,8 @@ int fp8lin_paged_append(const fp8lin_paged_cache* cache, const uint16_t* k, int6
  * [0, pages) reads as keys and values of 0; lengths are cut to the table's
  * width; rows from offsets[requests] on are left as they are.
  * max_count: the most rows that a request is expected to have; more are right as
- * well (in another summation order), slower.  head_dim 64, 128 or 256; scale > 0; 0 < requests <=
- * 4096; width * page_size <= 2^30; tokens * heads < 2^31, and times (heads /
+ * well (in another summation order), slower.  head_dim 64, 128 or 256; scale >
+ * 0; 0 < requests <= 4096; width * page_size <= 2^30; tokens * heads < 2^31, and times (heads /
  * kv_heads / 16 + 1) (width * page_size + 1024) < 2^61.  out may not overlap the
  * inputs.  A call's result does not depend on timing, but a row's does on
  * the lengths of the whole batch (FP32 summation order).  Where a chunk's values
