@@ -1168,7 +1168,8 @@ int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, i
                 "paged attention: head_dim must be 64, 128 or 256");
         check_pages(width, cache->page_size);
         require(table_ld >= width, FP8LIN_ERR_SHAPE, "paged attention: invalid table stride");
-        // the work of a batch is counted in 64 bits (PagedSplit), whatever the lengths on the device are
+        // the work of a batch is counted in 64 bits (PagedSplit), whatever the lengths on the device are (of
+        // offsets in order: no row in two requests)
         require((double)tokens * heads * (heads / cache->kv_heads / 16.0 + 1.0) * (double)(width * cache->page_size + 1024) < 0x1p61,
                 FP8LIN_ERR_SHAPE, "paged attention: too many tokens and heads for the table's width");
         const double scale2 = scale * 1.4426950408889634;
