@@ -15,6 +15,7 @@
 #include "../../include/fp8lin.h"
 #include "internal.hpp"
 #include "paged.hpp"
+#include "rotate.hpp"
 #include "verify.hpp"
 
 namespace {
@@ -520,7 +521,9 @@ void check_requests(int64_t requests, int64_t rows) {
     require(rows >= 0 && rows < kMaxDim, FP8LIN_ERR_SHAPE, "paged cache: invalid number of rows");
 }
 
-void check_cache(const fp8lin_paged_cache* c, fp8lin::PagedCache& k, fp8lin::PagedCache& v) {
+// blocks: scales of blocks instead of the cache's own, or null.
+void check_cache(const fp8lin_paged_cache* c, fp8lin::PagedCache& k, fp8lin::PagedCache& v,
+                 const fp8lin_block_scales* blocks = nullptr) {
     require(c != nullptr && c->k && c->v, FP8LIN_ERR_ARGUMENT, "paged cache: null pointer");
     check_pages(1, c->page_size);
     require(c->pages > 0 && c->pages < kMaxDim && c->kv_heads > 0 && c->kv_heads < kMaxDim && c->head_dim > 0 &&
@@ -533,13 +536,23 @@ void check_cache(const fp8lin_paged_cache* c, fp8lin::PagedCache& k, fp8lin::Pag
     };
     require(good(c->k, c->k_page, c->k_slot, c->k_head) && good(c->v, c->v_page, c->v_slot, c->v_head), FP8LIN_ERR_ARGUMENT,
             "paged cache: data and strides must be multiples of 16 bytes, a slot at least head_dim elements");
-    require(c->fp8 ? c->k_scale && c->v_scale : !c->k_scale && !c->v_scale, FP8LIN_ERR_ARGUMENT,
-            "paged cache: an 8-bit cache needs k_scale and v_scale, a BF16 cache has none");
+    if (blocks) {
+        require(c->fp8 && !c->k_scale && !c->v_scale && blocks->k && blocks->v, FP8LIN_ERR_ARGUMENT,
+                "paged cache: scales of blocks need an 8-bit cache without scales of heads, and two tables");
+        const int64_t b = blocks->block;
+        require((b == 16 || b == 32 || b == 64 || b == 128) && b <= c->page_size, FP8LIN_ERR_SHAPE,
+                "paged cache: a scale's block must be 16, 32, 64 or 128 tokens, at most a page");
+        require(c->pages * (c->page_size / b) < kMaxDim * 2 / c->kv_heads, FP8LIN_ERR_SHAPE, "paged cache: too many scales");
+    } else {
+        require(c->fp8 ? c->k_scale && c->v_scale : !c->k_scale && !c->v_scale, FP8LIN_ERR_ARGUMENT,
+                "paged cache: an 8-bit cache needs k_scale and v_scale, a BF16 cache has none");
+    }
     k = fp8lin::PagedCache{c->k, c->k_page, c->k_slot, c->k_head};
     v = fp8lin::PagedCache{c->v, c->v_page, c->v_slot, c->v_head};
 }
 
 constexpr int64_t kMaxVerifyRows = (int64_t)1 << 24;  // 256 threads a row, a grid below 2^32
+constexpr int64_t kMaxRotateDim = 1024;  // a wave's lanes hold a head, 16 values each
 constexpr int64_t kMaxStride = (int64_t)1 << 56;  // elements; bytes of it stay in 64 bits
 
 // Memory of an operand: `rows` rows of `width` bytes, `stride` bytes apart
@@ -571,6 +584,41 @@ void require_apart(std::initializer_list<Extent> outputs, std::initializer_list<
         for (const Extent& i : inputs) require(!overlap(*o, i), FP8LIN_ERR_ARGUMENT, what);
         for (auto p = o + 1; p != outputs.end(); ++p) require(!overlap(*o, *p), FP8LIN_ERR_ARGUMENT, what);
     }
+}
+
+// Heads [tokens, heads, dim] of BF16: a token's, from its first to its last
+// element, in a row.
+Extent heads_extent(const void* at, int64_t tokens, int64_t heads, int64_t dim, int64_t token, int64_t head) {
+    const int64_t width = 2 * ((heads - 1) * head + dim);
+    if (2 * token >= width || tokens <= 1) return Extent{at, heads ? tokens : 0, width, 2 * token};
+    // tokens side by side within a head's stride
+    const int64_t inner = 2 * ((tokens - 1) * token + dim);
+    if (2 * head >= inner) return Extent{at, heads, inner, 2 * head};
+    const int64_t all = 2 * ((tokens - 1) * token) + width;
+    return Extent{at, heads ? 1 : 0, all, all};
+}
+void check_heads(int64_t tokens, int64_t heads, int64_t token, int64_t head, const char* what) {
+    require(token >= 0 && head >= 0 && heads < kMaxDim && tokens < kMaxDim && (double)tokens * token < 0x1p56 && (double)heads * head < 0x1p56,
+            FP8LIN_ERR_SHAPE, what);
+}
+
+// The rows of an output are apart from each other.
+void check_apart_rows(int64_t tokens, int64_t heads, int64_t dim, int64_t token, int64_t head, const char* what) {
+    const bool by_token = tokens <= 1 || token >= (heads - 1) * head + dim, by_head = heads <= 1 || head >= (tokens - 1) * token + dim;
+    require((tokens <= 1 || token >= dim) && (heads <= 1 || head >= dim) && (by_token || by_head), FP8LIN_ERR_ARGUMENT, what);
+}
+
+fp8lin::Rotation check_rotary(const fp8lin_rotary* r, const int64_t* positions, int64_t axes, int64_t axis_stride, int64_t dim,
+                              bool transposed) {
+    require(r->rotary > 0 && r->rotary % 2 == 0 && r->rotary <= dim, FP8LIN_ERR_SHAPE,
+            "rotation: rotary must be even, of 2 to head_dim");
+    require(axes >= 1 && axes <= 4 && axis_stride >= 0 && axis_stride < kMaxStride, FP8LIN_ERR_SHAPE,
+            "rotation: positions have 1 to 4 axes");
+    require(r->steps && positions && reinterpret_cast<uintptr_t>(r->steps) % 8 == 0, FP8LIN_ERR_ARGUMENT,
+            "rotation: null or unaligned steps or positions");
+    require(std::isfinite(r->magnitude), FP8LIN_ERR_ARGUMENT, "rotation: the magnitude must be finite");
+    return fp8lin::Rotation{r->steps, positions, axis_stride, (int)axes, (int)(r->rotary / 2), r->neighbours != 0, r->magnitude,
+                            transposed ? -1.0f : 1.0f};
 }
 
 // Rows of a request per kv head.
@@ -1144,6 +1192,144 @@ int fp8lin_paged_append(const fp8lin_paged_cache* cache, const uint16_t* k, int6
                                               (int)cache->head_dim, page_bits(cache->page_size), cache->pages,
                                               as_stream(stream)),
                   "paged append launch");
+    });
+}
+
+int fp8lin_rotary_frequencies(int64_t rotary, double theta, int scaling, double factor, double original, double low,
+                              double high, double* frequencies, double* magnitude) {
+    return guarded([&] {
+        require(rotary > 0 && rotary % 2 == 0 && rotary < kMaxDim, FP8LIN_ERR_SHAPE, "rotary frequencies: rotary must be even and positive");
+        require(frequencies && magnitude, FP8LIN_ERR_ARGUMENT, "rotary frequencies: null pointer");
+        require(theta > 0 && std::isfinite(theta), FP8LIN_ERR_ARGUMENT, "rotary frequencies: theta must be positive");
+        require(scaling >= FP8LIN_ROTARY_PLAIN && scaling <= FP8LIN_ROTARY_WAVELENGTH, FP8LIN_ERR_ARGUMENT, "rotary frequencies: unknown scaling");
+        const bool scaled = scaling != FP8LIN_ROTARY_PLAIN, parts = scaling >= FP8LIN_ROTARY_YARN;
+        require(!scaled || (factor > 0 && std::isfinite(factor)), FP8LIN_ERR_ARGUMENT, "rotary frequencies: the factor must be positive");
+        if (low == 0) low = 1;
+        if (high == 0) high = scaling == FP8LIN_ROTARY_YARN ? 32 : 4;
+        require(!parts || (original > 0 && std::isfinite(original) && low > 0 && high > low && std::isfinite(high)), FP8LIN_ERR_ARGUMENT,
+                "rotary frequencies: need an original length and 0 < low < high");
+        require(scaling != FP8LIN_ROTARY_YARN || theta > 1, FP8LIN_ERR_ARGUMENT, "rotary frequencies: theta must be above 1");
+        const double turn = 6.283185307179586476925;
+        if (scaling == FP8LIN_ROTARY_NTK) theta *= std::pow(factor, (double)rotary / std::max<int64_t>(rotary - 2, 1));
+        // the pair (not whole) that turns so often in `original` positions
+        auto pair_of = [&](double turns) { return rotary * std::log(original / (turns * turn)) / (2 * std::log(theta)); };
+        const double from = std::max(std::floor(pair_of(high)), 0.0), to = std::min(std::ceil(pair_of(low)), rotary - 1.0);
+        for (int64_t j = 0; j < rotary / 2; ++j) {
+            const double f = std::pow(theta, -2.0 * j / rotary);
+            double kept = 1;  // the share of f that is not stretched
+            if (scaling == FP8LIN_ROTARY_LINEAR) kept = 0;
+            if (scaling == FP8LIN_ROTARY_YARN) kept = 1 - std::clamp((j - from) / std::max(to - from, 0.001), 0.0, 1.0);
+            if (scaling == FP8LIN_ROTARY_WAVELENGTH) kept = std::clamp((original * f / turn - low) / (high - low), 0.0, 1.0);
+            frequencies[j] = kept == 1 ? f : f * kept + f / factor * (1 - kept);
+        }
+        *magnitude = scaling == FP8LIN_ROTARY_YARN && factor > 1 ? 0.1 * std::log(factor) + 1 : 1.0;
+    });
+}
+
+int fp8lin_rotary_steps(const double* frequencies, const int32_t* axes, int64_t pairs, uint64_t* steps) {
+    return guarded([&] {
+        require(pairs >= 0 && pairs < kMaxDim, FP8LIN_ERR_SHAPE, "rotary steps: invalid number of pairs");
+        require(pairs == 0 || (frequencies && steps), FP8LIN_ERR_ARGUMENT, "rotary steps: null pointer");
+        for (int64_t j = 0; j < pairs; ++j) {
+            require(std::isfinite(frequencies[j]) && (!axes || (axes[j] >= 0 && axes[j] <= 3)), FP8LIN_ERR_ARGUMENT,
+                    "rotary steps: frequencies must be finite, axes 0 to 3");
+            const double turns = frequencies[j] / 6.283185307179586476925, part = turns - std::floor(turns);
+            // 2^62 units a turn, 1.0 (by rounding) being 0
+            steps[j] = ((uint64_t)std::nearbyint(part * 0x1p62) << 2) + (axes ? (uint64_t)axes[j] : 0);
+        }
+    });
+}
+
+int fp8lin_rotate(const fp8lin_rotary* rotary, const uint16_t* x, int64_t x_token, int64_t x_head, int64_t tokens,
+                  int64_t heads, int64_t head_dim, const int64_t* positions, int64_t axes, int64_t axis_stride,
+                  int transposed, uint16_t* y, int64_t y_token, int64_t y_head, fp8lin_stream_t stream) {
+    return guarded([&] {
+        require(rotary != nullptr, FP8LIN_ERR_ARGUMENT, "rotate: null pointer");
+        require(tokens >= 0 && heads >= 0 && head_dim > 0 && head_dim % 2 == 0 && head_dim <= kMaxRotateDim, FP8LIN_ERR_SHAPE,
+                "rotate: head_dim must be even, at most 1024");
+        check_heads(tokens, heads, x_token, x_head, "rotate: invalid strides");
+        check_heads(tokens, heads, y_token, y_head, "rotate: invalid strides");
+        require((double)tokens * heads * head_dim < 0x1p35, FP8LIN_ERR_SHAPE, "rotate: too many values");
+        if (tokens == 0 || heads == 0) return;
+        require(x && y, FP8LIN_ERR_ARGUMENT, "rotate: null pointer");
+        check_apart_rows(tokens, heads, head_dim, y_token, y_head, "rotate: the output's rows overlap");
+        fp8lin::Rotate a{};
+        a.r = check_rotary(rotary, positions, axes, axis_stride, head_dim, transposed != 0);
+        const Extent in = heads_extent(x, tokens, heads, head_dim, x_token, x_head),
+                     out = heads_extent(y, tokens, heads, head_dim, y_token, y_head);
+        const Extent pos = extent(positions, (axes - 1) * axis_stride + tokens, 8), steps = extent(rotary->steps, rotary->rotary / 2, 8);
+        if (x == y && x_token == y_token && x_head == y_head)
+            require_apart({out}, {pos, steps}, "rotate: the output overlaps the positions or the steps");
+        else
+            require_apart({out}, {in, pos, steps}, "rotate: the output overlaps an input");
+        ensure_device();
+        a.x = fp8lin::Heads{x, x_token, x_head, (int)heads};
+        a.y = y, a.y_tok = y_token, a.y_head = y_head, a.T = tokens, a.D = (int)head_dim;
+        check_hip(fp8lin::launch_rotate(a, as_stream(stream)), "rotate launch");
+    });
+}
+
+int fp8lin_paged_rotate_append(const fp8lin_paged_cache* cache, const fp8lin_block_scales* scales,
+                               const fp8lin_rotary* rotary, const uint16_t* q, int64_t q_token, int64_t q_head,
+                               int64_t heads, const uint16_t* k, int64_t k_token, int64_t k_head, const uint16_t* v,
+                               int64_t v_token, int64_t v_head, const uint16_t* q_norm, const uint16_t* k_norm,
+                               double eps, int centered, const int64_t* positions, int64_t axes, int64_t axis_stride,
+                               const int64_t* slots, int64_t tokens, uint16_t* q_out, int64_t out_token,
+                               int64_t out_head, fp8lin_stream_t stream) {
+    return guarded([&] {
+        const char* apart = "paged rotate append: q_out or the cache overlaps another operand";
+        fp8lin::RotateAppend a{};
+        check_cache(cache, a.kc, a.vc, scales);
+        const int64_t dim = cache->head_dim, hk = cache->kv_heads;
+        require(tokens >= 0 && tokens < kMaxDim && heads >= 0 && heads < kMaxDim, FP8LIN_ERR_SHAPE,
+                "paged rotate append: invalid number of tokens or heads");
+        require(dim % 16 == 0 && dim <= kMaxRotateDim, FP8LIN_ERR_UNSUPPORTED,
+                "paged rotate append: head_dim must be a multiple of 16, at most 1024");
+        require((double)tokens * (heads + 2.0 * hk) * dim < 0x1p35, FP8LIN_ERR_SHAPE, "paged rotate append: too many values");
+        require(eps >= 0 && std::isfinite((float)eps), FP8LIN_ERR_ARGUMENT, "paged rotate append: eps must be finite, 0 or more");
+        check_heads(tokens, heads, q_token, q_head, "paged rotate append: invalid strides");
+        check_heads(tokens, heads, out_token, out_head, "paged rotate append: invalid strides");
+        check_heads(tokens, hk, k_token, k_head, "paged rotate append: invalid strides");
+        check_heads(tokens, hk, v_token, v_head, "paged rotate append: invalid strides");
+        if (rotary) a.r = check_rotary(rotary, positions, axes, axis_stride, dim, false);
+        if (tokens == 0) return;
+        require(k && v && slots && (heads == 0 || (q && q_out)), FP8LIN_ERR_ARGUMENT, "paged rotate append: null pointer");
+        if (heads) check_apart_rows(tokens, heads, dim, out_token, out_head, "paged rotate append: the output's rows overlap");
+        const Extent in = heads_extent(q, tokens, heads, dim, q_token, q_head),
+                     out = heads_extent(heads ? q_out : nullptr, tokens, heads, dim, out_token, out_head);
+        const Extent nothing = extent(nullptr, 0, 1);
+        const bool in_place = q == q_out && q_token == out_token && q_head == out_head;
+        require((double)cache->pages * std::max(cache->k_page, cache->v_page) < 0x1p56 && (double)hk * std::max(cache->k_head, cache->v_head) < 0x1p56,
+                FP8LIN_ERR_SHAPE, "paged rotate append: invalid cache strides");
+        // a cache's memory from its first to its last element: all that lies between its pages counts
+        const int64_t size = cache->fp8 ? 1 : 2;
+        auto cache_extent = [&](const void* at, int64_t page, int64_t slot, int64_t head) {
+            return extent(at, (cache->pages - 1) * page + (cache->page_size - 1) * slot + (hk - 1) * head + dim, size);
+        };
+        const int64_t powers = scales ? cache->pages * (cache->page_size / scales->block) * hk : 0;
+        const Extent keys = cache_extent(cache->k, cache->k_page, cache->k_slot, cache->k_head),
+                     values = cache_extent(cache->v, cache->v_page, cache->v_slot, cache->v_head),
+                     key_powers = extent(scales ? scales->k : nullptr, powers, 1), value_powers = extent(scales ? scales->v : nullptr, powers, 1);
+        const std::initializer_list<Extent> read = {
+            in_place ? nothing : in, heads_extent(k, tokens, hk, dim, k_token, k_head), heads_extent(v, tokens, hk, dim, v_token, v_head),
+            extent(q_norm, dim, 2), extent(k_norm, dim, 2), extent(cache->k_scale, hk, 4), extent(cache->v_scale, hk, 4),
+            extent(slots, tokens, 8), rotary ? extent(positions, (axes - 1) * axis_stride + tokens, 8) : nothing,
+            rotary ? extent(rotary->steps, rotary->rotary / 2, 8) : nothing};
+        // the caches of keys and values may lie between each other's pages
+        require_apart({out, key_powers, value_powers}, read, apart);
+        require_apart({out, key_powers, value_powers}, {keys, values}, apart);
+        for (const Extent& c : {keys, values}) require_apart({c}, read, apart);
+        ensure_device();
+        a.q = fp8lin::Heads{q, q_token, q_head, (int)heads};
+        a.k = fp8lin::Heads{k, k_token, k_head, (int)hk};
+        a.v = fp8lin::Heads{v, v_token, v_head, (int)hk};
+        a.y = q_out, a.y_tok = out_token, a.y_head = out_head;
+        a.q_norm = q_norm, a.k_norm = k_norm, a.eps = (float)eps, a.center = centered ? 1.0f : 0.0f;
+        a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
+        if (scales) a.k_pow = scales->k, a.v_pow = scales->v, a.block_bits = page_bits(scales->block);
+        a.slots = slots, a.T = tokens, a.limit = cache->pages * cache->page_size;
+        a.D = (int)dim, a.page_bits = page_bits(cache->page_size), a.fp8 = cache->fp8 != 0;
+        check_hip(fp8lin::launch_rotate_append(a, as_stream(stream)), "paged rotate append launch");
     });
 }
 

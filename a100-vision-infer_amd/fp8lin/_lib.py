@@ -49,6 +49,7 @@ EXPORTED = [
     "fp8lin_paged_layout_workspace_bytes", "fp8lin_paged_layout", "fp8lin_paged_append",
     "fp8lin_paged_attention_workspace_bytes", "fp8lin_paged_attention",
     "fp8lin_verify_drafts_workspace_bytes", "fp8lin_verify_drafts",
+    "fp8lin_rotary_frequencies", "fp8lin_rotary_steps", "fp8lin_rotate", "fp8lin_paged_rotate_append",
 ]
 
 
@@ -85,6 +86,16 @@ class PagedCacheRecord(ctypes.Structure):
                 ("v_scale", ctypes.c_void_p)]
 
 
+class RotaryRecord(ctypes.Structure):
+    """struct fp8lin_rotary"""
+    _fields_ = [("steps", ctypes.c_void_p), ("rotary", ctypes.c_int64), ("neighbours", ctypes.c_int),
+                ("magnitude", ctypes.c_float)]
+
+
+class BlockScalesRecord(ctypes.Structure):
+    """struct fp8lin_block_scales"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("block", ctypes.c_int64)]
+
 
 class LinearOptions(ctypes.Structure):
     """struct fp8lin_linear_options (the EngineOptions linear flags,
@@ -116,7 +127,7 @@ def lib():
     L = ctypes.CDLL(LIB_PATH)
     vp, i64, i32, u64, u32 = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
                               ctypes.c_uint64, ctypes.c_uint32)
-    sz = ctypes.c_size_t
+    sz, dbl = ctypes.c_size_t, ctypes.c_double
     sig = {
         "fp8lin_version": (i32, []),
         "fp8lin_last_error": (ctypes.c_char_p, []),
@@ -175,6 +186,12 @@ def lib():
         "fp8lin_paged_attention_workspace_bytes": (sz, [i64, i64, i64, i64]),
         "fp8lin_paged_attention": (i32, [ctypes.POINTER(PagedCacheRecord), vp, i64, i64, vp, i64, i64, vp, i64, i64, vp,
                                          vp, i64, i64, i64, i64, i32, ctypes.c_double, vp, i64, i64, vp, sz, vp]),
+        "fp8lin_rotary_frequencies": (i32, [i64, dbl, i32, dbl, dbl, dbl, dbl, vp, vp]),
+        "fp8lin_rotary_steps": (i32, [vp, vp, i64, vp]),
+        "fp8lin_rotate": (i32, [ctypes.POINTER(RotaryRecord), vp, i64, i64, i64, i64, i64, vp, i64, i64, i32, vp, i64, i64, vp]),
+        "fp8lin_paged_rotate_append": (i32, [ctypes.POINTER(PagedCacheRecord), ctypes.POINTER(BlockScalesRecord),
+                                             ctypes.POINTER(RotaryRecord), vp, i64, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp,
+                                             dbl, i32, vp, i64, i64, vp, i64, vp, i64, i64, vp]),
         "fp8lin_verify_drafts_workspace_bytes": (sz, [i64, i64, i64]),
         "fp8lin_verify_drafts": (i32, [vp, i32, i64, vp, i64, i64, vp, vp, vp, vp, i64, i64, i64, vp, vp, vp, sz, vp]),
     }

@@ -14,8 +14,9 @@ from collections import namedtuple
 
 import torch
 
-from ._lib import ERR_ARGUMENT, ERR_SHAPE, PagedCacheRecord, check, lib
+from ._lib import ERR_ARGUMENT, ERR_SHAPE, BlockScalesRecord, PagedCacheRecord, check, lib
 from .ops import _fail, _is_dev, _ready_devices, _stream
+from .rotary import plan_record, positions_of
 
 PagedLayout = namedtuple("PagedLayout", "offsets lengths slots positions block_table cursor")
 PagedLayout.__doc__ = """What paged_layout returns: offsets int32 [requests + 1], lengths int32 [requests] after the step, slots and
@@ -29,6 +30,7 @@ _FP8 = (torch.float8_e4m3fn, torch.uint8)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current = torch._C._cuda_getDevice
 _byref, _i32, _i64, _f32, _bf16 = ctypes.byref, torch.int32, torch.int64, torch.float32, torch.bfloat16
+_e8m0 = torch.float8_e8m0fnu
 
 
 def _call(name, device, *args):
@@ -96,9 +98,11 @@ def _row_stride(t, width):
 
 
 def _cache(k_cache, v_cache, k_scale, v_scale):
-    """The library's record of a cache [pages, page_size, kv_heads, head_dim]
+    """The library's records of a cache [pages, page_size, kv_heads, head_dim]
     (any strides, the last dimension contiguous), BF16 or E4M3FN codes
-    (torch.float8_e4m3fn or uint8) with a float32 scale per kv head."""
+    (torch.float8_e4m3fn or uint8) with a float32 scale per kv head or E8M0
+    scales [pages, blocks, kv_heads] (torch.float8_e8m0fnu, contiguous) of
+    page_size / blocks tokens each: the cache's, and the blocks' or None."""
     if not (_is_dev(k_cache) and isinstance(v_cache, torch.Tensor) and k_cache.dim() == 4 and
             k_cache.shape == v_cache.shape and k_cache.dtype is v_cache.dtype and k_cache.device == v_cache.device):
         _fail(ERR_ARGUMENT, "Paged caches must be equal device tensors [pages, page_size, kv_heads, head_dim]")
@@ -109,14 +113,24 @@ def _cache(k_cache, v_cache, k_scale, v_scale):
     if ks[3] != 1 or vs[3] != 1:
         _fail(ERR_ARGUMENT, "Paged caches need a contiguous last dimension")
     pages, page_size, kv_heads, head_dim = k_cache.shape
-    if fp8:
+    blocks = None
+    if fp8 and isinstance(k_scale, torch.Tensor) and k_scale.dtype is _e8m0:
+        if not (isinstance(v_scale, torch.Tensor) and v_scale.dtype is _e8m0 and k_scale.dim() == 3 and k_scale.shape == v_scale.shape and
+                k_scale.is_contiguous() and v_scale.is_contiguous() and k_scale.device == v_scale.device == k_cache.device):
+            _fail(ERR_ARGUMENT, "Scales of blocks must be equal contiguous E8M0 tensors [pages, blocks, kv_heads] on the cache's device")
+        n = k_scale.size(1)
+        if not (k_scale.size(0) == pages and k_scale.size(2) == kv_heads and n > 0 and page_size % n == 0):
+            _fail(ERR_SHAPE, "Scales of blocks do not match the cache")
+        blocks = BlockScalesRecord(k_scale.data_ptr(), v_scale.data_ptr(), page_size // n)
+    elif fp8:
         if not (_vector(k_scale, kv_heads, _f32, k_cache.device) and _vector(v_scale, kv_heads, _f32, k_cache.device)):
             _fail(ERR_ARGUMENT, "An 8-bit cache needs float32 k_scale and v_scale [kv_heads]")
     elif k_scale is not None or v_scale is not None:
         _fail(ERR_ARGUMENT, "A BF16 cache has no scales")
+    own = fp8 and blocks is None
     return PagedCacheRecord(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages, page_size,
-                            kv_heads, head_dim, int(fp8), k_scale.data_ptr() if fp8 else None,
-                            v_scale.data_ptr() if fp8 else None)
+                            kv_heads, head_dim, int(fp8), k_scale.data_ptr() if own else None,
+                            v_scale.data_ptr() if own else None), blocks
 
 
 def _heads(t, shape, device):
@@ -127,8 +141,10 @@ def _heads(t, shape, device):
 def paged_append(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     """k and v (BF16 [tokens, kv_heads, head_dim], last dimension contiguous)
     into their slots (int64 [tokens]) of the caches, in place
-    (fp8lin_paged_append); rows whose slot is outside the cache are skipped."""
-    rec = _cache(k_cache, v_cache, k_scale, v_scale)
+    (fp8lin_paged_append); rows whose slot is outside the cache are skipped.
+    A cache with scales of blocks (see _cache) is written as paged_rotate_append
+    writes it."""
+    rec, blocks = _cache(k_cache, v_cache, k_scale, v_scale)
     device = k_cache.device
     tokens = k.size(0) if isinstance(k, torch.Tensor) and k.dim() == 3 else -1
     shape = (tokens, rec.kv_heads, rec.head_dim)
@@ -139,8 +155,57 @@ def paged_append(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     if tokens == 0:
         return
     ks, vs = k.stride(), v.stride()
+    if blocks is not None:
+        _call("fp8lin_paged_rotate_append", device, _byref(rec), _byref(blocks), None, None, 0, 0, 0, k.data_ptr(), ks[0], ks[1],
+              v.data_ptr(), vs[0], vs[1], None, None, 0.0, 1, None, 1, 0, slots.data_ptr(), tokens, None, 0, 0)
+        return
     _call("fp8lin_paged_append", device, _byref(rec), k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], slots.data_ptr(),
           tokens)
+
+
+def paged_rotate_append(q, k, v, positions, slots, k_cache, v_cache, plan, q_norm=None, k_norm=None, eps=1e-6, centered=True,
+                        k_scale=None, v_scale=None, out=None):
+    """The end of a projection and the append in one launch
+    (fp8lin_paged_rotate_append): q (BF16 [tokens, heads, head_dim]) and k
+    ([tokens, kv_heads, head_dim]) normed per head (q_norm, k_norm BF16
+    [head_dim] or None; centered: weights are offsets from 1) and rotated by the
+    RotaryPlan `plan` (None: not rotated) at positions (int64 [tokens] or [axes,
+    tokens]), then k and v into their slots (int64 [tokens]) of the caches, in
+    place; rows whose slot is outside the cache are skipped.  Returns the
+    queries: `out` if given, which may be q and overlaps nothing else.
+    Caches are BF16, E4M3FN with a float32 scale per kv head, or E4M3FN with E8M0
+    scales [pages, blocks, kv_heads], which the call sets: the rows of one block
+    stand side by side, as paged_layout numbers them, and a block whose first
+    slot is written starts anew."""
+    rec, blocks = _cache(k_cache, v_cache, k_scale, v_scale)
+    device = k_cache.device
+    dim = rec.head_dim
+    if not (isinstance(q, torch.Tensor) and q.dim() == 3):
+        _fail(ERR_ARGUMENT, "Paged rotate append expects BF16 queries [tokens, heads, head_dim]")
+    tokens, heads = q.shape[:2]
+    shape, kv_shape = (tokens, heads, dim), (tokens, rec.kv_heads, dim)
+    if not (_heads(q, shape, device) and _heads(k, kv_shape, device) and _heads(v, kv_shape, device)):
+        _fail(ERR_ARGUMENT, "Paged rotate append expects BF16 queries, keys and values [tokens, heads, head_dim]")
+    if not _vector(slots, tokens, _i64, device):
+        _fail(ERR_ARGUMENT, "Paged rotate append expects int64 slots [tokens]")
+    for w in (q_norm, k_norm):
+        if w is not None and not _vector(w, dim, _bf16, device):
+            _fail(ERR_ARGUMENT, "Paged rotate append expects BF16 norms [head_dim]")
+    rotary, axes, axis, at = None, 1, 0, None
+    if plan is not None:
+        rotary = _byref(plan_record(plan, device))
+        axes, axis, at = positions_of(positions, tokens, device)
+    if out is None:
+        out = q.new_empty(shape)
+    elif not _heads(out, shape, device):
+        _fail(ERR_ARGUMENT, "Paged rotate append expects a BF16 output as the queries")
+    if tokens:
+        qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+        _call("fp8lin_paged_rotate_append", device, _byref(rec), None if blocks is None else _byref(blocks), rotary, q.data_ptr(),
+              qs[0], qs[1], heads, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+              None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), float(eps), int(bool(centered)),
+              at, axes, axis, slots.data_ptr(), tokens, out.data_ptr(), os[0], os[1])
+    return out
 
 
 def paged_attention(q, k_cache, v_cache, block_table, offsets, lengths, max_count=None, gate=None, k_scale=None, v_scale=None,
@@ -156,7 +221,9 @@ def paged_attention(q, k_cache, v_cache, block_table, offsets, lengths, max_coun
     tokens beyond one per request).  Returns BF16 [tokens, heads, head_dim]:
     `out` if given, which overlaps no input and whose rows behind the last
     request stay as they were."""
-    rec = _cache(k_cache, v_cache, k_scale, v_scale)
+    rec, blocks = _cache(k_cache, v_cache, k_scale, v_scale)
+    if blocks is not None:
+        _fail(ERR_ARGUMENT, "Paged attention does not take scales of blocks")
     device, kv_heads, dim = k_cache.device, rec.kv_heads, rec.head_dim
     if not (isinstance(q, torch.Tensor) and q.dim() == 3 and q.dtype is _bf16 and q.stride(2) == 1 and q.device == device and
             q.size(2) == dim):

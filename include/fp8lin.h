@@ -654,6 +654,102 @@ int fp8lin_verify_drafts(const void* logits, int logits_f32, int64_t logits_ld, 
                          fp8lin_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Rotary positions.  Pair j of a head's first `rotary` dimensions, (x_2j,
+ * x_2j+1) with `neighbours`, else (x_j, x_j+rotary/2), at position p:
+ *   x_a' = magnitude (x_a cos a - x_b sin a),  x_b' = magnitude (x_b cos a + x_a sin a),
+ *   a = p frequency_j (radians);
+ * the dimensions behind stay.  FP32 with one rounding of the result, the angle
+ * exact modulo a turn to 2^-33 turns at any 64-bit position (fp8lin_rope and
+ * fp8lin_qk_norm_rope are the reference's form: FP32 angles, BF16 in between).
+ *
+ * steps[j] holds frequency_j as the part of a turn per position in units of
+ * 2^-64, modulo a turn, and in its two lowest bits the axis whose position the
+ * pair takes: 4 * round(frequency_j / (2 pi) * 2^62) + axis.  positions
+ * [axes, tokens] (int64, `axis_stride` elements between the axes, 1 to 4 of
+ * them): a pair whose axis is not there takes the last one.
+ */
+typedef struct fp8lin_rotary {
+    const uint64_t* steps; /* device [rotary / 2] */
+    int64_t rotary;        /* even */
+    int neighbours;
+    float magnitude;       /* of the cosines and sines, 1 without scaling for long contexts */
+} fp8lin_rotary;
+
+enum fp8lin_rotary_scaling {
+    FP8LIN_ROTARY_PLAIN = 0,     /* f_j = theta^(-2j / rotary) */
+    FP8LIN_ROTARY_LINEAR = 1,    /* f_j / factor: positions interpolated */
+    FP8LIN_ROTARY_NTK = 2,       /* theta times factor^(rotary / (rotary - 2)) */
+    FP8LIN_ROTARY_YARN = 3,      /* f_j kept where a pair turns `high` times or more in `original` positions, f_j / factor where
+                                  * it turns `low` times or less, between them linear in j (from floor to ceil of the two
+                                  * borders); magnitude 0.1 ln(factor) + 1 */
+    FP8LIN_ROTARY_WAVELENGTH = 4 /* the same borders, linear in the turns original f_j / (2 pi); magnitude 1 */
+};
+/* Host functions (no device is touched).  Frequencies [rotary / 2] in radians
+ * per position and the magnitude of a scaling; `low`, `high`: 0 for the usual
+ * borders, 1 and 32 (YARN) or 1 and 4 (WAVELENGTH).  And the steps of
+ * frequencies (finite) and axes (0..3; null: all 0).
+ */
+int fp8lin_rotary_frequencies(int64_t rotary, double theta, int scaling, double factor, double original, double low,
+                              double high, double* frequencies, double* magnitude);
+int fp8lin_rotary_steps(const double* frequencies, const int32_t* axes, int64_t pairs, uint64_t* steps);
+
+/* y = x rotated, heads [tokens, heads, head_dim] (BF16, strides in elements, the
+ * last dimension contiguous, any alignment); transposed: by the transposed
+ * matrix, which turns back (magnitude times) and takes a gradient of y to x's.
+ * y may be x itself (the same pointer and strides); other memory in common is
+ * FP8LIN_ERR_ARGUMENT.  head_dim even, at most 1024; rotary <= head_dim; tokens *
+ * heads * head_dim below 2^35.
+ */
+int fp8lin_rotate(const fp8lin_rotary* rotary, const uint16_t* x, int64_t x_token, int64_t x_head, int64_t tokens,
+                  int64_t heads, int64_t head_dim, const int64_t* positions, int64_t axes, int64_t axis_stride,
+                  int transposed, uint16_t* y, int64_t y_token, int64_t y_head, fp8lin_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * An 8-bit paged cache with a scale for each block of `block` tokens of a page
+ * and kv head: codes that stand for code * 2^(b - 127), b = k[page][slot /
+ * block][head] (v), bytes 7 .. 247 of E8M0 [pages, page_size / block, kv_heads].
+ * block: 16, 32, 64 or 128, at most page_size.  The cache's record has fp8 and
+ * null scales then.  A power of two: codes keep their value when a block's
+ * scale grows, and the matrix cores' operands are converted with it.
+ */
+typedef struct fp8lin_block_scales {
+    uint8_t* k;
+    uint8_t* v;
+    int64_t block;
+} fp8lin_block_scales;
+
+/* The end of the projection and the append in one launch:
+ *   q_out = rotate(norm(q, q_norm)), k slot = rotate(norm(k, k_norm)), v slot = v,
+ * norm(x, w) = x / sqrt(mean(x^2) + eps) * (centered ? 1 + w : w) over a head's
+ * head_dim values (null weights: no norm; rotary null: no rotation), all in FP32
+ * with one rounding into q_out (BF16) and into the cache: BF16; with scales
+ * null in an 8-bit cache E4M3FN(x / scale) as fp8lin_paged_append's; else block
+ * scales:
+ *   A block's scale is the least 2^e, e from -120 on, with |x| <= 448 2^e for
+ *   the finite values of the call's rows in it, and no less than the scale
+ *   that the block had, unless the rows write the block's first slot: then it
+ *   starts anew, and what its slots hold that the call does not write is lost.
+ *   Where the scale grows, the codes of the block's other slots are multiplied by
+ *   old / new (rounded, to nearest even, where they fall below 2^-6).  Values
+ *   beyond 448 2^e (infinities) become 448 2^e, NaN stays NaN.
+ *   The rows of one block stand side by side, as fp8lin_paged_layout numbers
+ *   them: of a block that comes twice, other rows (of another block, or
+ *   without a slot) between, it is not defined what it holds.
+ * A row whose slot is outside [0, pages * page_size) is not written; its query
+ * is rotated.  Two rows of one slot: either's values.  q may be null with heads
+ * 0; its strides and q_out's as fp8lin_rotate's, q_out may be q.  q_out and the
+ * cache may not overlap another operand: FP8LIN_ERR_ARGUMENT.  head_dim % 16 ==
+ * 0, at most 1024; tokens * (heads + 2 kv_heads) * head_dim below 2^35.
+ */
+int fp8lin_paged_rotate_append(const fp8lin_paged_cache* cache, const fp8lin_block_scales* scales,
+                               const fp8lin_rotary* rotary, const uint16_t* q, int64_t q_token, int64_t q_head,
+                               int64_t heads, const uint16_t* k, int64_t k_token, int64_t k_head, const uint16_t* v,
+                               int64_t v_token, int64_t v_head, const uint16_t* q_norm, const uint16_t* k_norm,
+                               double eps, int centered, const int64_t* positions, int64_t axes, int64_t axis_stride,
+                               const int64_t* slots, int64_t tokens, uint16_t* q_out, int64_t out_token,
+                               int64_t out_head, fp8lin_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Deterministic synthetic inputs (no reference counterpart; used by the
  * benchmark and tests so that the device and a host checker see the same
  * bits).  Element i of stream `tag` is a standard normal from Philox4x32-10
