@@ -626,6 +626,55 @@ int64_t paged_rows(int64_t heads, int64_t kv_heads, int64_t max_count) {
     return heads / kv_heads * std::min<int64_t>(std::max<int64_t>(max_count, 1), kMaxDim);
 }
 
+// fp8lin_paged_attention; scales: of blocks, or null.
+int attend(const fp8lin_paged_cache* cache, const fp8lin_block_scales* scales, const uint16_t* q, int64_t q_token, int64_t q_head,
+                           const uint16_t* gate, int64_t gate_token, int64_t gate_head, const int32_t* table,
+                           int64_t table_ld, int64_t width, const int32_t* offsets, const int32_t* lengths,
+                           int64_t requests, int64_t tokens, int64_t heads, int64_t max_count, int causal, double scale,
+                           uint16_t* out, int64_t out_token, int64_t out_head, void* workspace, size_t workspace_bytes,
+                           fp8lin_stream_t stream) {
+    return guarded([&] {
+        fp8lin::PagedAttention a{};
+        check_cache(cache, a.k, a.v, scales);
+        check_requests(requests, tokens);
+        require(heads > 0 && heads % cache->kv_heads == 0 && heads < kMaxDim && tokens * heads < kMaxDim - 1024,
+                FP8LIN_ERR_SHAPE, "paged attention: heads must be a multiple of kv_heads, tokens * heads below 2^31");
+        require(cache->head_dim == 64 || cache->head_dim == 128 || cache->head_dim == 256, FP8LIN_ERR_UNSUPPORTED,
+                "paged attention: head_dim must be 64, 128 or 256");
+        check_pages(width, cache->page_size);
+        require(table_ld >= width, FP8LIN_ERR_SHAPE, "paged attention: invalid table stride");
+        // the work of a batch is counted in 64 bits (PagedSplit), whatever the lengths on the device are (of
+        // offsets in order: no row in two requests)
+        require((double)tokens * heads * (heads / cache->kv_heads / 16.0 + 1.0) * (double)(width * cache->page_size + 1024) < 0x1p61,
+                FP8LIN_ERR_SHAPE, "paged attention: too many tokens and heads for the table's width");
+        const double scale2 = scale * 1.4426950408889634;
+        require(scale > 0.0 && std::isfinite((float)scale2) && (float)scale2 > 0.0f, FP8LIN_ERR_ARGUMENT,
+                "paged attention: scale must be positive");
+        if (tokens == 0) return;
+        require(q && table && offsets && lengths && out, FP8LIN_ERR_ARGUMENT, "paged attention: null pointer");
+        const int64_t rows = paged_rows(heads, cache->kv_heads, max_count);
+        check_workspace(workspace, workspace_bytes, fp8lin::paged_attention_ws_bytes((int)cache->head_dim, rows),
+                        "paged attention: workspace too small");
+        ensure_device();
+        a.q = q, a.gate = gate, a.out = out;
+        a.q_tok = q_token, a.q_head = q_head, a.g_tok = gate_token, a.g_head = gate_head;
+        a.o_tok = out_token, a.o_head = out_head;
+        a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
+        if (scales) a.k_pow = scales->k, a.v_pow = scales->v, a.block_bits = page_bits(scales->block);
+        a.table = table, a.offsets = offsets, a.lengths = lengths, a.ldt = table_ld;
+        a.width = (int)width, a.page_bits = page_bits(cache->page_size), a.pages = (int)cache->pages;
+        a.B = (int)requests, a.T = (int)tokens, a.H = (int)heads, a.HK = (int)cache->kv_heads;
+        a.G = a.H / a.HK;
+        a.causal = causal != 0;
+        a.scale2 = (float)scale2;
+        a.ws = static_cast<float*>(workspace);
+        check_hip(fp8lin::launch_paged_attention(a, (int)cache->head_dim,
+                                                 scales ? fp8lin::kCacheBlocks : cache->fp8 ? fp8lin::kCacheHeads : fp8lin::kCacheBf16, rows,
+                                                 as_stream(stream)),
+                  "paged attention launch");
+    });
+}
+
 }  // namespace
 
 extern "C" {
@@ -1344,43 +1393,19 @@ int fp8lin_paged_attention(const fp8lin_paged_cache* cache, const uint16_t* q, i
                            int64_t requests, int64_t tokens, int64_t heads, int64_t max_count, int causal, double scale,
                            uint16_t* out, int64_t out_token, int64_t out_head, void* workspace, size_t workspace_bytes,
                            fp8lin_stream_t stream) {
-    return guarded([&] {
-        fp8lin::PagedAttention a{};
-        check_cache(cache, a.k, a.v);
-        check_requests(requests, tokens);
-        require(heads > 0 && heads % cache->kv_heads == 0 && heads < kMaxDim && tokens * heads < kMaxDim - 1024,
-                FP8LIN_ERR_SHAPE, "paged attention: heads must be a multiple of kv_heads, tokens * heads below 2^31");
-        require(cache->head_dim == 64 || cache->head_dim == 128 || cache->head_dim == 256, FP8LIN_ERR_UNSUPPORTED,
-                "paged attention: head_dim must be 64, 128 or 256");
-        check_pages(width, cache->page_size);
-        require(table_ld >= width, FP8LIN_ERR_SHAPE, "paged attention: invalid table stride");
-        // the work of a batch is counted in 64 bits (PagedSplit), whatever the lengths on the device are (of
-        // offsets in order: no row in two requests)
-        require((double)tokens * heads * (heads / cache->kv_heads / 16.0 + 1.0) * (double)(width * cache->page_size + 1024) < 0x1p61,
-                FP8LIN_ERR_SHAPE, "paged attention: too many tokens and heads for the table's width");
-        const double scale2 = scale * 1.4426950408889634;
-        require(scale > 0.0 && std::isfinite((float)scale2) && (float)scale2 > 0.0f, FP8LIN_ERR_ARGUMENT,
-                "paged attention: scale must be positive");
-        if (tokens == 0) return;
-        require(q && table && offsets && lengths && out, FP8LIN_ERR_ARGUMENT, "paged attention: null pointer");
-        const int64_t rows = paged_rows(heads, cache->kv_heads, max_count);
-        check_workspace(workspace, workspace_bytes, fp8lin::paged_attention_ws_bytes((int)cache->head_dim, rows),
-                        "paged attention: workspace too small");
-        ensure_device();
-        a.q = q, a.gate = gate, a.out = out;
-        a.q_tok = q_token, a.q_head = q_head, a.g_tok = gate_token, a.g_head = gate_head;
-        a.o_tok = out_token, a.o_head = out_head;
-        a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
-        a.table = table, a.offsets = offsets, a.lengths = lengths, a.ldt = table_ld;
-        a.width = (int)width, a.page_bits = page_bits(cache->page_size), a.pages = (int)cache->pages;
-        a.B = (int)requests, a.T = (int)tokens, a.H = (int)heads, a.HK = (int)cache->kv_heads;
-        a.G = a.H / a.HK;
-        a.causal = causal != 0;
-        a.scale2 = (float)scale2;
-        a.ws = static_cast<float*>(workspace);
-        check_hip(fp8lin::launch_paged_attention(a, (int)cache->head_dim, cache->fp8 != 0, rows, as_stream(stream)),
-                  "paged attention launch");
-    });
+    return attend(cache, nullptr, q, q_token, q_head, gate, gate_token, gate_head, table, table_ld, width, offsets, lengths, requests,
+                  tokens, heads, max_count, causal, scale, out, out_token, out_head, workspace, workspace_bytes, stream);
+}
+
+int fp8lin_paged_attention_blocks(const fp8lin_paged_cache* cache, const fp8lin_block_scales* scales, const uint16_t* q, int64_t q_token, int64_t q_head,
+                           const uint16_t* gate, int64_t gate_token, int64_t gate_head, const int32_t* table,
+                           int64_t table_ld, int64_t width, const int32_t* offsets, const int32_t* lengths,
+                           int64_t requests, int64_t tokens, int64_t heads, int64_t max_count, int causal, double scale,
+                           uint16_t* out, int64_t out_token, int64_t out_head, void* workspace, size_t workspace_bytes,
+                           fp8lin_stream_t stream) {
+    if (!scales) return guarded([] { fail(FP8LIN_ERR_ARGUMENT, "paged attention: null scales of blocks"); });
+    return attend(cache, scales, q, q_token, q_head, gate, gate_token, gate_head, table, table_ld, width, offsets, lengths, requests,
+                  tokens, heads, max_count, causal, scale, out, out_token, out_head, workspace, workspace_bytes, stream);
 }
 
 size_t fp8lin_verify_drafts_workspace_bytes(int64_t requests, int64_t rows, int64_t vocab) {

@@ -63,14 +63,36 @@ __device__ __forceinline__ u32x4 read16(uint32_t addr) {
     return *(lds_t*)(uintptr_t)addr;
 }
 
-// Two E4M3FN codes to BF16, exactly (every code has 4 significant bits).
+// Two E4M3FN codes times a power of two to BF16, exactly (every code has 4
+// significant bits; the instruction takes the scale's exponent): the scales of
+// a cache's blocks cost no instruction here.
 template <bool HI>
-__device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
 }
-__device__ __forceinline__ bf16x8 codes8_bf16(uint32_t lo, uint32_t hi) {
-    return __builtin_bit_cast(bf16x8, u32x4{codes_bf16<false>(lo), codes_bf16<true>(lo), codes_bf16<false>(hi),
-                                            codes_bf16<true>(hi)});
+__device__ __forceinline__ bf16x8 codes8_bf16(uint32_t lo, uint32_t hi, float scale_lo = 1.0f, float scale_hi = 1.0f) {
+    return __builtin_bit_cast(bf16x8, u32x4{codes_bf16<false>(lo, scale_lo), codes_bf16<true>(lo, scale_lo),
+                                            codes_bf16<false>(hi, scale_hi), codes_bf16<true>(hi, scale_hi)});
+}
+
+// E8M0 powers of two of a cache's blocks, a byte each.  As long as a block is
+// 16 tokens or more, the 16 keys of one page that a DMA brings have one.
+__device__ __forceinline__ uint32_t power_index(const PagedAttention& a, int id, int64_t key, int hk) {
+    const int in_page = (int)(key & ((1 << a.page_bits) - 1));
+    return (((uint32_t)id << (a.page_bits - a.block_bits)) + (uint32_t)(in_page >> a.block_bits)) * (uint32_t)a.HK + (uint32_t)hk;
+}
+// The bytes of all blocks, below 2^32; other offsets read 0.
+__device__ __forceinline__ i32x4 power_desc(const PagedAttention& a, const uint8_t* bytes) {
+    return make_desc(bytes, ((uint32_t)a.pages << (a.page_bits - a.block_bits)) * (uint32_t)a.HK);
+}
+constexpr uint32_t kNoPower = 0xffffffffu;
+// A byte a lane from global (voff, bounds-checked), as 32 bits into LDS [m0v, m0v + 256).
+__device__ __forceinline__ void dma_byte(uint32_t m0v, uint32_t voff, i32x4 desc) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_ubyte %1, %2, 0 offen lds" ::"s"(m0v), "v"(voff), "s"(desc) : "memory", "m0");
+}
+__device__ __forceinline__ float power_at(uint32_t lds) {
+    typedef __attribute__((address_space(3))) uint32_t lds_t;
+    return __builtin_bit_cast(float, *(lds_t*)(uintptr_t)lds << 23);
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -151,13 +173,14 @@ __device__ __forceinline__ bool odd_values(const PagedAttention& a, const int32_
 // One row by plain FP32 sums, a key at a time, by a wave: for the rows near
 // values that only some rows may see and that are infinities or NaN, which the
 // matrix product would carry, as 0 * inf, into the other rows of its tile.
-template <int D, bool F8>
+template <int D, int KIND>
 __device__ void plain_row(const PagedAttention& a, const PagedSeq& s, int b, int hk, int flat) {
+    constexpr bool F8 = KIND != kCacheBf16;
     constexpr int LANES = D / 4;  // 4 dimensions a lane
     const int lane = threadIdx.x & 63, d = 4 * (lane % LANES);
     const int32_t* table = a.table + (int64_t)b * a.ldt;
-    const float c = a.scale2 * (F8 ? a.k_scale[hk] : 1.0f);
-    auto value4 = [&](const PagedCache& cache, int id, int key) {
+    const float c = a.scale2 * (KIND == kCacheHeads ? a.k_scale[hk] : 1.0f);
+    auto value4 = [&](const PagedCache& cache, const uint8_t* powers, int id, int key) {
         f32x4 x = {0, 0, 0, 0};
         if ((unsigned)id >= (unsigned)a.pages) return x;
         const int64_t at = (int64_t)id * cache.page + (int64_t)(key & ((1 << a.page_bits) - 1)) * cache.slot + hk * cache.head + d;
@@ -165,6 +188,11 @@ __device__ void plain_row(const PagedAttention& a, const PagedSeq& s, int b, int
             const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(cache.data) + at);
             const f32x2 lo = fp8x2_to_f32<false>(w), hi = fp8x2_to_f32<true>(w);
             x = f32x4{lo.x, lo.y, hi.x, hi.y};
+            if constexpr (KIND == kCacheBlocks) {
+                const float f = __builtin_bit_cast(float, (uint32_t)powers[power_index(a, id, key, hk)] << 23);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] *= f;
+            }
         } else {
             const u32x2 w = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(cache.data) + at);
             x = f32x4{bf16_bits_to_f32(w.x & 0xffffu), bf16_bits_to_f32(w.x >> 16), bf16_bits_to_f32(w.y & 0xffffu),
@@ -181,7 +209,7 @@ __device__ void plain_row(const PagedAttention& a, const PagedSeq& s, int b, int
     for (int i = 0; i < 4; ++i) qv[i] = bf16_bits_to_f32(q[i]);
     for (int key = 0; key < lim; ++key) {
         const int id = table[key >> a.page_bits];
-        const f32x4 k = value4(a.k, id, key), v = value4(a.v, id, key);
+        const f32x4 k = value4(a.k, a.k_pow, id, key), v = value4(a.v, a.v_pow, id, key);
         float x = lane < LANES ? qv.x * k.x + qv.y * k.y + qv.z * k.z + qv.w * k.w : 0.0f;
         x = wave_sum(x) * c;
         const float mn = fmaxf(m, x), ms = mn == -__builtin_inff() ? 0.0f : mn;
@@ -191,7 +219,7 @@ __device__ void plain_row(const PagedAttention& a, const PagedSeq& s, int b, int
         for (int i = 0; i < 4; ++i) o[i] = o[i] * f + p * v[i];
         m = mn;
     }
-    const float inv = l == 0.0f ? 0.0f : (F8 ? a.v_scale[hk] : 1.0f) / l;
+    const float inv = l == 0.0f ? 0.0f : (KIND == kCacheHeads ? a.v_scale[hk] : 1.0f) / l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : o[i] * inv;
     if (lane < LANES) store4(a, s.off + tok, head, d, o);
@@ -221,8 +249,8 @@ struct Partial {
 
 // `rows`: the most of a request.  Without `join` the units' partial sums are
 // left to launch_tile's `few`, which joins both kernels' in one launch.
-hipError_t launch_few(const PagedAttention& a, int D, bool fp8, int rows, bool join, hipStream_t stream);
-hipError_t launch_tile(const PagedAttention& a, const PagedAttention* few, int D, bool fp8, hipStream_t stream);
+hipError_t launch_few(const PagedAttention& a, int D, CacheKind kind, int rows, bool join, hipStream_t stream);
+hipError_t launch_tile(const PagedAttention& a, const PagedAttention* few, int D, CacheKind kind, hipStream_t stream);
 constexpr int kMixedRows = 32;  // rows of a few-rows tile of a mixed batch
 
 // Joins the pieces of the units that the boundaries between workgroups cut,
@@ -232,7 +260,7 @@ constexpr int kMixedRows = 32;  // rows of a few-rows tile of a mixed batch
 // step) or 256 (WAVES 1) groups of 4 values.  ORDER::place(e, row, d): row and
 // first dimension of the e-th 4 floats of a piece's O.  The units of workgroups
 // with marked waves are computed again, row by row, instead.
-template <int BM, int D, bool F8, int WAVES, class ORDER>
+template <int BM, int D, int KIND, int WAVES, class ORDER>
 __device__ __forceinline__ void join(const PagedAttention& a, int block, int blocks) {
     constexpr int PER = 256 / WAVES, PARTS = BM * D / 4 / PER;
     __shared__ i32x4v begin[kGroups], rows[kGroups];
@@ -355,7 +383,7 @@ __device__ __forceinline__ void join(const PagedAttention& a, int block, int blo
                 const int R = Split::tiles(a, s), r0 = u.z * BM;
                 if (u.z < R)
                     for (int r = block * 4 + wave; r < (int)min((int64_t)BM, (int64_t)s.n * a.G - r0); r += 4 * blocks)
-                        plain_row<D, F8>(a, s, u.x, u.y, r0 + r);
+                        plain_row<D, KIND>(a, s, u.x, u.y, r0 + r);
                 if (end) break;
                 if (++u.z >= R) {
                     u.z = 0;
@@ -368,9 +396,9 @@ __device__ __forceinline__ void join(const PagedAttention& a, int block, int blo
         }
     }
 }
-template <int BM, int D, bool F8, int WAVES, class ORDER>
+template <int BM, int D, int KIND, int WAVES, class ORDER>
 __global__ __launch_bounds__(256) void join_kernel(PagedAttention a) {
-    join<BM, D, F8, WAVES, ORDER>(a, blockIdx.x, gridDim.x);
+    join<BM, D, KIND, WAVES, ORDER>(a, blockIdx.x, gridDim.x);
 }
 
 // The order of O in the partial sums of the few-rows kernel: by row.

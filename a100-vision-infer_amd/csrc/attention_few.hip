@@ -16,6 +16,8 @@
 // permuted by row so that the reads hit distinct banks; each DMA lane fetches
 // the chunk that its LDS place holds.  Rows past the request's keys, and pages
 // whose id is out of range, are read as zeros by the buffer's bounds check.
+#include <type_traits>
+
 #include "attention.hpp"
 
 namespace fp8lin {
@@ -36,6 +38,7 @@ struct Few {
     static constexpr int DEPTH = 16384 / SLOT;        // tiles of a wave's ring
     static constexpr int WAVE = 2 * DEPTH * SLOT;     // 32 KB per wave
     static constexpr int LDS = kFewWaves * WAVE;      // 128 KB
+    static constexpr int POWERS = 2 * 2 * 256;        // of block scales, per wave
     // What a unit's start and end cost, as keys that stream in that time: 5 us
     // (its queries and first tiles, the join) at a CU's 30 KB per us.
     static constexpr int START = 160 * 1024 / (2 * ROWB);
@@ -61,8 +64,9 @@ struct Few {
     }
 };
 
-template <int D, bool F8, int NT>
+template <int D, int KIND, int NT>
 __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a) {
+    constexpr bool F8 = KIND != kCacheBf16, BLOCKS = KIND == kCacheBlocks;
     using F = Few<D, F8>;
     constexpr int BM = 16 * NT, KT = F::KT, SUB = KT / 16, ES = F8 ? 1 : 2;
     using Split = PagedSplit<BM, KT, F::START>;
@@ -92,6 +96,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
     __syncthreads();
 
     const uint32_t ring = (uint32_t)(uintptr_t)lds + wave * F::WAVE;
+    // BLOCKS: the powers of two of the wave's tiles, two batches of K's and V's
+    const uint32_t powers = (uint32_t)(uintptr_t)lds + F::LDS + wave * F::POWERS;
     // this lane's place in a DMA instruction: key lr of RPI, chunk lc
     const int lr = lane / F::LPR, lc = lane % F::LPR;
 
@@ -112,9 +118,16 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                 const int64_t key = ((int64_t)k0 + wave + (int64_t)kFewWaves * (j0 + lane / SUB)) * KT + 16 * (lane % SUB);
                 const int id = table[min(key, (int64_t)s.len - 1 + (s.len == 0)) >> a.page_bits];
                 ids = key < s.len ? id : -1;
+                if constexpr (BLOCKS) {
+                    // older than the tiles' DMAs, so the wait for a tile covers them
+                    const uint32_t at = (unsigned)ids < (unsigned)a.pages ? power_index(a, ids, key, cur.hk) : kNoPower;
+                    const uint32_t m0 = __builtin_amdgcn_readfirstlane(powers + (j0 / BATCH & 1) * 512);
+                    dma_byte(m0, at, power_desc(a, a.k_pow));
+                    dma_byte(m0 + 256, at, power_desc(a, a.v_pow));
+                }
             };
             load_ids(0);
-            const float c = a.scale2 * (F8 ? a.k_scale[cur.hk] : 1.0f);
+            const float c = a.scale2 * (KIND == kCacheHeads ? a.k_scale[cur.hk] : 1.0f);
             // queries (B operand: row col, dimensions 64 t + 16 quad + 8 e ..)
             bf16x8 qf[NT][D / 32];
             int lim[NT];  // keys that the lane's row may see
@@ -174,6 +187,16 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                 const int key0 = (k0 + wave + kFewWaves * j) * KT;
                 if ((j + F::DEPTH) % BATCH == 0) load_ids(j + F::DEPTH);
                 wait_vm<F::IN_FLIGHT>();
+                float kp[SUB], vp[SUB];  // powers of two of K and V
+#pragma unroll
+                for (int sub = 0; sub < SUB; ++sub) {
+                    kp[sub] = vp[sub] = 1.0f;
+                    if constexpr (BLOCKS) {
+                        const uint32_t at = powers + (j / BATCH & 1) * 512 + ((j % BATCH) * SUB + sub) * 4;
+                        kp[sub] = power_at(at);
+                        vp[sub] = power_at(at + 256);
+                    }
+                }
                 f32x4 st[NT][SUB];
 #pragma unroll
                 for (int sub = 0; sub < SUB; ++sub) {
@@ -185,8 +208,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                         bf16x8 kf[2];
                         if constexpr (F8) {
                             const u32x4 w = read16(ks + row * F::ROWB + (((4 * t + quad) ^ F::xk(row)) << 4));
-                            kf[0] = codes8_bf16(w.x, w.y);
-                            kf[1] = codes8_bf16(w.z, w.w);
+                            kf[0] = codes8_bf16(w.x, w.y, kp[sub], kp[sub]);
+                            kf[1] = codes8_bf16(w.z, w.w, kp[sub], kp[sub]);
                         } else {
 #pragma unroll
                             for (int e = 0; e < 2; ++e)
@@ -252,7 +275,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
                         // 8 keys of dimension 16 dt + col: 4 quad + 0..3 and 16 + 4 quad + 0..3
                         const int rr = col >> 1, row = (rr & 3) + 4 * quad + 16 * (rr >> 2);
                         const i32x2 w = read_tr8(vs + row * F::ROWB + ((dt ^ F::xv(row)) << 4) + 8 * (col & 1));
-                        const bf16x8 vf = codes8_bf16((uint32_t)w.x, (uint32_t)w.y);
+                        const bf16x8 vf = codes8_bf16((uint32_t)w.x, (uint32_t)w.y, vp[0], vp[SUB - 1]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             const u32x4 pb = {pw[nt][0].x, pw[nt][0].y, pw[nt][SUB - 1].x, pw[nt][SUB - 1].y};
@@ -286,7 +309,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
             float* sl = sm + kFewWaves * 16;
             const bool whole = k0 == 0 && k1 == nkt;
             float* part = Partial<BM, D>::at(a.ws, group, k0 == 0);
-            const float vscale = F8 ? a.v_scale[cur.hk] : 1.0f;
+            const float vscale = KIND == kCacheHeads ? a.v_scale[cur.hk] : 1.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 __syncthreads();
@@ -357,19 +380,20 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void few_kernel(PagedAttention a
     }
 }
 
-template <int D, bool F8, int NT>
+template <int D, int KIND, int NT>
 hipError_t run(const PagedAttention& a, bool with_join, hipStream_t stream) {
-    constexpr int BM = 16 * NT, LDS = Few<D, F8>::LDS;
+    using F = Few<D, KIND != kCacheBf16>;
+    constexpr int BM = 16 * NT, LDS = F::LDS + (KIND == kCacheBlocks ? kFewWaves * F::POWERS : 0);
     static_assert(LDS >= PagedSplit<BM, 16, 0>::lds_bytes(kPagedMaxRequests), "the prefix of the requests' costs fits");
     static_assert(LDS >= kFewWaves * 16 * (D + 6) * 4, "the waves' sums fit");
-    auto* kern = few_kernel<D, F8, NT>;
+    auto* kern = few_kernel<D, KIND, NT>;
     static OncePerDevice once;
     const hipError_t attr = allow_lds(once, reinterpret_cast<const void*>(kern), LDS);
     if (attr != hipSuccess) return attr;
     hipLaunchKernelGGL(kern, dim3(kGroups), dim3(64 * kFewWaves), LDS, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !with_join) return e;
-    auto* kern_join = join_kernel<BM, D, F8, 4, FewOrder<D>>;
+    auto* kern_join = join_kernel<BM, D, KIND, 4, FewOrder<D>>;
     hipLaunchKernelGGL(kern_join, dim3(2 * kGroups), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
@@ -379,18 +403,24 @@ hipError_t run(const PagedAttention& a, bool with_join, hipStream_t stream) {
 // (48 rows, 8000 keys, 12/2 heads: 60 us against 26); for smaller heads they
 // gained 15 % on one long request (64 rows, 60000 8-bit keys, 32/8 heads of 128:
 // 57 us against 66) and lost 27 % on a batch (16 x 4000 keys: 85 against 67).
-template <int D, bool F8>
-hipError_t run_rows(const PagedAttention& a, int rows, bool join, hipStream_t stream) {
+template <int D>
+hipError_t run_rows(const PagedAttention& a, CacheKind kind, int rows, bool join, hipStream_t stream) {
     static_assert(kMixedRows == 32);
-    return rows <= 16 ? run<D, F8, 1>(a, join, stream) : run<D, F8, 2>(a, join, stream);
+    auto go = [&](auto kind_) {
+        constexpr int KIND = decltype(kind_)::value;
+        return rows <= 16 ? run<D, KIND, 1>(a, join, stream) : run<D, KIND, 2>(a, join, stream);
+    };
+    if (kind == kCacheBlocks) return go(std::integral_constant<int, kCacheBlocks>{});
+    if (kind == kCacheHeads) return go(std::integral_constant<int, kCacheHeads>{});
+    return go(std::integral_constant<int, kCacheBf16>{});
 }
 
 }  // namespace
 
-hipError_t launch_few(const PagedAttention& a, int D, bool fp8, int rows, bool join, hipStream_t stream) {
-    if (D == 64) return fp8 ? run_rows<64, true>(a, rows, join, stream) : run_rows<64, false>(a, rows, join, stream);
-    if (D == 128) return fp8 ? run_rows<128, true>(a, rows, join, stream) : run_rows<128, false>(a, rows, join, stream);
-    return fp8 ? run_rows<256, true>(a, rows, join, stream) : run_rows<256, false>(a, rows, join, stream);
+hipError_t launch_few(const PagedAttention& a, int D, CacheKind kind, int rows, bool join, hipStream_t stream) {
+    if (D == 64) return run_rows<64>(a, kind, rows, join, stream);
+    if (D == 128) return run_rows<128>(a, kind, rows, join, stream);
+    return run_rows<256>(a, kind, rows, join, stream);
 }
 
 }  // namespace attn

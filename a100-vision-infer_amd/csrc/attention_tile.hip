@@ -134,8 +134,9 @@ __device__ __forceinline__ void finish_row(const PagedAttention& a, const f32x4*
     }
 }
 
-template <int D, bool F8, int RB>
+template <int D, int KIND, int RB>
 __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(PagedAttention a) {
+    constexpr bool F8 = KIND != kCacheBf16, BLOCKS = KIND == kCacheBlocks;
     constexpr int W = kBM / (32 * RB);  // waves
     using L = Tile<D, F8>;
     using Split = PagedSplit<kBM, kBN, kTileStart<D>>;
@@ -174,6 +175,16 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
     const int vi = lane & 15, vr = F8 ? 4 * half + ((vi >> 1) & 3) + 8 * (vi >> 3) : 4 * half + (vi >> 2);
     const int vc = F8 ? (lane >> 4) & 1 : 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);
     const uint32_t v_lane = lds0 + 2 * L::HALF + vr * L::ROWB + ((vc ^ L::xv(vr)) << 4) + 8 * (lane & 1);
+    // BLOCKS: the powers of two of each tile's 4 times 16 keys (256 bytes each, a
+    // copy a lane), two buffers of K's, then of V's.  K's of the tile at kb for this lane's
+    // fragments, V's of the tile at vb.
+    const uint32_t powers = lds0 + L::LDS;
+    auto k_power = [&](uint32_t kb, int sub) {
+        return power_at(powers + (kb - k_lane) / L::HALF * 1024 + (2 * sub + (col >> 4)) * 256 + 4 * lane);
+    };
+    auto v_power = [&](uint32_t vb, int sub, int ks) {
+        return power_at(powers + 2048 + (vb - v_lane) / L::HALF * 1024 + (2 * sub + ks) * 256 + 4 * lane);
+    };
 
     for (;;) {
         const int R = Split::tiles(a, s);
@@ -182,7 +193,7 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
         const int k0 = cur.kt, k1 = last ? end.kt : nkt;
         if (R && k1 > k0) {
             const int r0 = cur.r * kBM, nr = (int)min((int64_t)kBM, (int64_t)s.n * a.G - r0);
-            const float c = a.scale2 * (F8 ? a.k_scale[cur.hk] : 1.0f);
+            const float c = a.scale2 * (KIND == kCacheHeads ? a.k_scale[cur.hk] : 1.0f);
             const int row0 = 32 * RB * wave, ctx = s.len - s.n;
             const int32_t* table = a.table + (int64_t)cur.b * a.ldt;
             // page id of the keys that this wave brings of tile t
@@ -197,6 +208,7 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
                 i32x4 desc;
                 uint32_t m0;
                 int slot;
+                uint32_t power, power_m0;
             };
             auto part_of = [&](const PagedCache& cache, int t, int id, bool is_v) {
                 constexpr int ES = F8 ? 1 : 2;
@@ -206,15 +218,20 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
                 const uint32_t bytes = there > 0 ? (uint32_t)(((there - 1) * cache.slot + D) * ES) : 0;
                 return Part{make_desc(static_cast<const char*>(cache.data) + (bytes ? at * ES : 0), bytes),
                             (uint32_t)__builtin_amdgcn_readfirstlane(lds0 + (is_v ? 2 * L::HALF : 0) + (t & 1) * L::HALF + kKeys * part * L::ROWB),
-                            (int)cache.slot * ES};
+                            (int)cache.slot * ES, there > 0 ? power_index(a, id, key, cur.hk) : kNoPower,
+                            (uint32_t)__builtin_amdgcn_readfirstlane(powers + (is_v ? 2048 : 0) + (t & 1) * 1024 + part * 256)};
             };
             auto bring = [&](const Part& p, int i, bool is_v) {
                 const int r = L::RPI * i + lane / L::LPR;  // kKeys * part is a multiple of 16: no part in xk, xv
                 const int ch = (lane % L::LPR) ^ (is_v ? L::xv(r) : L::xk(r));
                 dma<false>(p.m0 + i * 1024, (uint32_t)(r * p.slot + ch * 16), p.desc);
             };
+            auto bring_power = [&](const Part& p, bool is_v) {
+                if constexpr (BLOCKS) dma_byte(p.power_m0, p.power, power_desc(a, is_v ? a.v_pow : a.k_pow));
+            };
             auto bring_all = [&](const PagedCache& cache, int t, int id, bool is_v) {
                 const Part p = part_of(cache, t, id, is_v);
+                bring_power(p, is_v);
 #pragma unroll
                 for (int i = 0; i < L::NI; ++i) bring(p, i, is_v);
             };
@@ -259,11 +276,19 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
             constexpr int AHEAD = 4, AK = NK < AHEAD ? NK : AHEAD;
             static_assert(NV % AHEAD == 0 && (NK % AHEAD == 0 || NK < AHEAD));
             u32x4 f[AHEAD];
+            float kp = 1.0f, vp[2] = {1.0f, 1.0f};  // powers of two, read with a phase's first fragment
             auto load_k = [&](uint32_t kb, int sub, int i) {
+                if constexpr (BLOCKS)
+                    if (i == 0) kp = k_power(kb, sub);
                 f[i % AK] = read16((kb ^ ((2 * i & (L::PICK - 1)) << 4)) + 32 * sub * L::ROWB + (2 * i & ~(L::PICK - 1)) * 16);
             };
             auto load_v = [&](uint32_t vb, int sub, int i) {
                 const int ks = i / (D / 32), dt = i % (D / 32);
+                if constexpr (BLOCKS)
+                    if (i == 0) {
+                        vp[0] = v_power(vb, sub, 0);
+                        vp[1] = v_power(vb, sub, 1);
+                    }
                 if constexpr (F8) {
                     const u32x2 w = __builtin_bit_cast(u32x2, read_tr8((vb ^ (dt << 5)) + (32 * sub + 16 * ks) * L::ROWB));
                     f[i % AHEAD].x = w.x;
@@ -284,7 +309,7 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
 #pragma unroll
                     for (int e = 0; e < PER; ++e) {
                         const u32x4 w = f[i % AK];
-                        const u32x4 k = F8 ? __builtin_bit_cast(u32x4, e ? codes8_bf16(w.z, w.w) : codes8_bf16(w.x, w.y)) : w;
+                        const u32x4 k = F8 ? __builtin_bit_cast(u32x4, e ? codes8_bf16(w.z, w.w, kp, kp) : codes8_bf16(w.x, w.y, kp, kp)) : w;
 #pragma unroll
                         for (int rb = 0; rb < RB; ++rb) {
                             if (i + e == 0) mfma_first(st[rb], k, qf[rb][0]);
@@ -346,7 +371,7 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
                     if constexpr (PV) {
                         const int ks = i / (D / 32), dt = i % (D / 32);
                         const u32x4 w = f[i % AHEAD];
-                        const u32x4 v = F8 ? __builtin_bit_cast(u32x4, codes8_bf16(w.x, w.y)) : w;
+                        const u32x4 v = F8 ? __builtin_bit_cast(u32x4, codes8_bf16(w.x, w.y, vp[ks], vp[ks])) : w;
 #pragma unroll
                         for (int rb = 0; rb < RB; ++rb) mfma_o(o[rb][dt], v, pw[rb][ks]);
                         if (i + AHEAD < NV) load_v(vb, sub, i + AHEAD);
@@ -434,7 +459,7 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
             std::bool_constant<false> no;
             auto nothing = [](int) {};
 
-            wait_vm<W == 4 ? 2 * L::NI : 0>();  // K of the first tile
+            wait_vm<W == 4 ? 2 * (L::NI + BLOCKS) : 0>();  // K of the first tile
             __syncthreads();
             const uint32_t kb0 = k_lane + (k0 & 1) * L::HALF;
 #pragma unroll
@@ -459,6 +484,8 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
                 const Part pk = part_of(a.k, t + 2, id, false), pv = part_of(a.v, t + 1, id1, true);
                 id1 = id;
                 weigh(yes, yes, vb, sub0, t * kBN + 32, kn, sub0, [&](int i) {
+                    if (i == 0 && of_k) bring_power(pk, false);
+                    if (i == 0 && of_v) bring_power(pv, true);
 #pragma unroll
                     for (int x = 0; x < 2 * L::NI; ++x)
                         if (x * NV / (2 * L::NI) == i && (x < L::NI ? of_k : of_v)) bring(x < L::NI ? pk : pv, x % L::NI, x >= L::NI);
@@ -512,7 +539,7 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
                 for (int rb = 0; rb < RB; ++rb) {
                     const int row = row0 + 32 * rb + col, flat = r0 + min(row, nr - 1), tok = s.off + flat / a.G;
                     const int64_t head = cur.hk * a.G + flat % a.G;
-                    const float sum = rb ? l[RB - 1] : l[0], vs = F8 ? a.v_scale[cur.hk] : 1.0f;
+                    const float sum = rb ? l[RB - 1] : l[0], vs = KIND == kCacheHeads ? a.v_scale[cur.hk] : 1.0f;
                     finish_row<D>(a, mine + rb * D / 8 * 64, sum == 0.0f ? 0.0f : vs / sum, a.gate + tok * a.g_tok + head * a.g_head + 4 * half,
                                a.out + tok * a.o_tok + head * a.o_head + 4 * half, row < nr);
                 }
@@ -541,18 +568,19 @@ namespace {
 constexpr int kFewJoin = 2 * kGroups, kTileJoin = 8 * kGroups;  // workgroups
 
 // The joins of a mixed batch: the first workgroups the few-rows kernel's.
-template <int D, bool F8>
+template <int D, int KIND>
 __global__ __launch_bounds__(256) void join_mixed_kernel(PagedAttention few, PagedAttention a) {
     if (blockIdx.x < kFewJoin)
-        join<kMixedRows, D, F8, 4, FewOrder<D>>(few, blockIdx.x, kFewJoin);
+        join<kMixedRows, D, KIND, 4, FewOrder<D>>(few, blockIdx.x, kFewJoin);
     else
-        join<kBM, D, F8, 1, TileOrder<D>>(a, blockIdx.x - kFewJoin, kTileJoin);
+        join<kBM, D, KIND, 1, TileOrder<D>>(a, blockIdx.x - kFewJoin, kTileJoin);
 }
 
-template <int D, bool F8, int RB>
+template <int D, int KIND, int RB>
 hipError_t run(const PagedAttention& a, const PagedAttention* few, hipStream_t stream) {
-    constexpr int LDS = std::max<int>(Tile<D, F8>::LDS, PagedSplit<kBM, kBN, 0>::lds_bytes(kPagedMaxRequests));
-    auto* kern = tile_kernel<D, F8, RB>;
+    using L = Tile<D, KIND != kCacheBf16>;
+    constexpr int LDS = std::max<int>(L::LDS + (KIND == kCacheBlocks ? 4096 : 0), PagedSplit<kBM, kBN, 0>::lds_bytes(kPagedMaxRequests));
+    auto* kern = tile_kernel<D, KIND, RB>;
     static OncePerDevice once;
     const hipError_t attr = allow_lds(once, reinterpret_cast<const void*>(kern), LDS);
     if (attr != hipSuccess) return attr;
@@ -560,18 +588,25 @@ hipError_t run(const PagedAttention& a, const PagedAttention* few, hipStream_t s
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (few)
-        hipLaunchKernelGGL((join_mixed_kernel<D, F8>), dim3(kFewJoin + kTileJoin), dim3(256), 0, stream, *few, a);
+        hipLaunchKernelGGL((join_mixed_kernel<D, KIND>), dim3(kFewJoin + kTileJoin), dim3(256), 0, stream, *few, a);
     else
-        hipLaunchKernelGGL((join_kernel<kBM, D, F8, 1, TileOrder<D>>), dim3(kTileJoin), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((join_kernel<kBM, D, KIND, 1, TileOrder<D>>), dim3(kTileJoin), dim3(256), 0, stream, a);
     return hipGetLastError();
+}
+
+template <int D, int RB>
+hipError_t run_kind(const PagedAttention& a, const PagedAttention* few, CacheKind kind, hipStream_t stream) {
+    if (kind == kCacheBlocks) return run<D, kCacheBlocks, RB>(a, few, stream);
+    if (kind == kCacheHeads) return run<D, kCacheHeads, RB>(a, few, stream);
+    return run<D, kCacheBf16, RB>(a, few, stream);
 }
 
 }  // namespace
 
-hipError_t launch_tile(const PagedAttention& a, const PagedAttention* few, int D, bool fp8, hipStream_t stream) {
-    if (D == 64) return fp8 ? run<64, true, 1>(a, few, stream) : run<64, false, 1>(a, few, stream);
-    if (D == 128) return fp8 ? run<128, true, 1>(a, few, stream) : run<128, false, 1>(a, few, stream);
-    return fp8 ? run<256, true, 2>(a, few, stream) : run<256, false, 2>(a, few, stream);
+hipError_t launch_tile(const PagedAttention& a, const PagedAttention* few, int D, CacheKind kind, hipStream_t stream) {
+    if (D == 64) return run_kind<64, 1>(a, few, kind, stream);
+    if (D == 128) return run_kind<128, 1>(a, few, kind, stream);
+    return run_kind<256, 2>(a, few, kind, stream);
 }
 
 static int64_t ws_floats(int D, int64_t bm) { return kBeginFloats + 2 * kGroups * (bm * D + 2 * bm); }
@@ -593,18 +628,18 @@ size_t paged_attention_ws_bytes(int D, int64_t max_rows) {
 // 256-row tile streams its keys at the pace of one wave's steps (13 requests,
 // three of them chunks of 400 to 700 tokens, 32/8 heads of 128: 153 us in two
 // against 165).  One launch joins both kernels' partial sums: two cost 6 us more.
-hipError_t launch_paged_attention(PagedAttention a, int D, bool fp8, int64_t max_rows, hipStream_t stream) {
+hipError_t launch_paged_attention(PagedAttention a, int D, CacheKind kind, int64_t max_rows, hipStream_t stream) {
     a.rows_from = 0;
     a.rows_to = INT64_MAX;
-    if (max_rows <= attn::kFewRows) return attn::launch_few(a, D, fp8, (int)max_rows, true, stream);
-    if (a.B == 1) return attn::launch_tile(a, nullptr, D, fp8, stream);
+    if (max_rows <= attn::kFewRows) return attn::launch_few(a, D, kind, (int)max_rows, true, stream);
+    if (a.B == 1) return attn::launch_tile(a, nullptr, D, kind, stream);
     PagedAttention few = a;
     few.rows_to = attn::kFewRows;
     few.ws = a.ws + attn::ws_floats(D, attn::kTileRows);
-    const hipError_t e = attn::launch_few(few, D, fp8, attn::kFewRows, false, stream);
+    const hipError_t e = attn::launch_few(few, D, kind, attn::kFewRows, false, stream);
     if (e != hipSuccess) return e;
     a.rows_from = attn::kFewRows;
-    return attn::launch_tile(a, &few, D, fp8, stream);
+    return attn::launch_tile(a, &few, D, kind, stream);
 }
 
 }  // namespace fp8lin

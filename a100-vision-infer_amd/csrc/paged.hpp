@@ -8,8 +8,12 @@
 
 namespace fp8lin {
 
+// What a cache's elements are: BF16, or E4M3FN codes with a scale per head, or
+// with a power of two per block of tokens and head.
+enum CacheKind { kCacheBf16 = 0, kCacheHeads = 1, kCacheBlocks = 2 };
+
 // A K or V cache [pages, page_size, kv_heads, D] with strides in elements
-// (the last dimension contiguous); fp8: E4M3FN codes, else BF16.
+// (the last dimension contiguous).
 struct PagedCache {
     const void* data;
     int64_t page, slot, head;
@@ -21,6 +25,8 @@ struct PagedAttention {
     int64_t q_tok, q_head, g_tok, g_head, o_tok, o_head;
     PagedCache k, v;
     const float *k_scale, *v_scale;  // [HK] or null
+    const uint8_t *k_pow, *v_pow;    // E8M0 [pages, blocks of a page, HK] or null
+    int block_bits;                  // of such a block's tokens
     const int32_t *table, *offsets, *lengths;
     int64_t ldt;
     int width, page_bits, pages;
@@ -38,7 +44,7 @@ constexpr int kPagedMinPage = 16;
 // (the most rows, tokens times heads per kv head, that a request should
 // bring) selects; the workspace that goes with them.
 size_t paged_attention_ws_bytes(int D, int64_t max_rows);
-hipError_t launch_paged_attention(PagedAttention a, int D, bool fp8, int64_t max_rows, hipStream_t stream);
+hipError_t launch_paged_attention(PagedAttention a, int D, CacheKind kind, int64_t max_rows, hipStream_t stream);
 
 hipError_t launch_paged_append(const uint16_t* k, const uint16_t* v, int64_t k_tok, int64_t k_head, int64_t v_tok,
                                int64_t v_head, const int64_t* slots, const PagedCache& kc, const PagedCache& vc, bool fp8,

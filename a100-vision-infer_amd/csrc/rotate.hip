@@ -331,10 +331,13 @@ __device__ void append_rows(const RotateAppend& a, int lane_bits, int chunks, in
     }
 }
 
-// The exponent byte of the least 2^e (e from -120 on) with top <= 448 2^e.
+// The exponent byte of the least 2^e with top <= 448 2^e, e from -120 (so that
+// its reciprocal and every code times it are normal numbers) to 119 (so that
+// they stay below 2^128).
+constexpr int kMinPower = 7, kMaxPower = 246;
 __device__ __forceinline__ int block_power(float top) {
     const uint32_t u = __builtin_bit_cast(uint32_t, top);
-    return min(max((int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u), 7), 247);
+    return min(max((int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u), kMinPower), kMaxPower);
 }
 __device__ __forceinline__ float power_of(int exponent) {  // 2^(exponent - 127), 0 below
     return __builtin_bit_cast(float, exponent > 0 ? (uint32_t)exponent << 23 : 0u);
@@ -413,7 +416,7 @@ __device__ void append_run(const RotateAppend& a, int lane_bits, int64_t t0, int
     uint8_t* byte = (is_v ? a.v_pow : a.k_pow) + ((page << (a.page_bits - a.block_bits)) + (in_page >> a.block_bits)) * a.k.n + h;
     int power = block_power(top);
     if (!(written[0] & 1)) {
-        const int old = min((int)*byte, 247);
+        const int old = min((int)*byte, kMaxPower);
         if (old < power) {
             const float f = power_of(127 + old - power);
             for (int e = tid; e < block * (D / 4); e += kThreads) {

@@ -50,6 +50,7 @@ EXPORTED = [
     "fp8lin_paged_attention_workspace_bytes", "fp8lin_paged_attention",
     "fp8lin_verify_drafts_workspace_bytes", "fp8lin_verify_drafts",
     "fp8lin_rotary_frequencies", "fp8lin_rotary_steps", "fp8lin_rotate", "fp8lin_paged_rotate_append",
+    "fp8lin_paged_attention_blocks",
 ]
 
 
@@ -192,6 +193,8 @@ def lib():
         "fp8lin_paged_rotate_append": (i32, [ctypes.POINTER(PagedCacheRecord), ctypes.POINTER(BlockScalesRecord),
                                              ctypes.POINTER(RotaryRecord), vp, i64, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp,
                                              dbl, i32, vp, i64, i64, vp, i64, vp, i64, i64, vp]),
+        "fp8lin_paged_attention_blocks": (i32, [ctypes.POINTER(PagedCacheRecord), ctypes.POINTER(BlockScalesRecord), vp, i64, i64, vp,
+                                                i64, i64, vp, i64, i64, vp, vp, i64, i64, i64, i64, i32, dbl, vp, i64, i64, vp, sz, vp]),
         "fp8lin_verify_drafts_workspace_bytes": (sz, [i64, i64, i64]),
         "fp8lin_verify_drafts": (i32, [vp, i32, i64, vp, i64, i64, vp, vp, vp, vp, i64, i64, i64, vp, vp, vp, sz, vp]),
     }

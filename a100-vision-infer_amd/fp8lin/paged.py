@@ -222,8 +222,6 @@ def paged_attention(q, k_cache, v_cache, block_table, offsets, lengths, max_coun
     `out` if given, which overlaps no input and whose rows behind the last
     request stay as they were."""
     rec, blocks = _cache(k_cache, v_cache, k_scale, v_scale)
-    if blocks is not None:
-        _fail(ERR_ARGUMENT, "Paged attention does not take scales of blocks")
     device, kv_heads, dim = k_cache.device, rec.kv_heads, rec.head_dim
     if not (isinstance(q, torch.Tensor) and q.dim() == 3 and q.dtype is _bf16 and q.stride(2) == 1 and q.device == device and
             q.size(2) == dim):
@@ -252,7 +250,8 @@ def paged_attention(q, k_cache, v_cache, block_table, offsets, lengths, max_coun
     need = lib().fp8lin_paged_attention_workspace_bytes(heads, kv_heads, dim, count)
     ws = torch.empty(need, dtype=torch.uint8, device=device)
     qs, os = q.stride(), out.stride()
-    _call("fp8lin_paged_attention", device, _byref(rec), q.data_ptr(), qs[0], qs[1], gate_at, gs[0], gs[1],
+    name, cache = ("fp8lin_paged_attention", (_byref(rec),)) if blocks is None else ("fp8lin_paged_attention_blocks", (_byref(rec), _byref(blocks)))
+    _call(name, device, *cache, q.data_ptr(), qs[0], qs[1], gate_at, gs[0], gs[1],
           block_table.data_ptr(), _row_stride(block_table, width), width, offsets.data_ptr(), lengths.data_ptr(), requests,
           tokens, heads, count, int(causal), dim ** -0.5 if scale is None else float(scale), out.data_ptr(), os[0], os[1],
           ws.data_ptr(), need)

@@ -707,7 +707,7 @@ int fp8lin_rotate(const fp8lin_rotary* rotary, const uint16_t* x, int64_t x_toke
 /* ---------------------------------------------------------------------------
  * An 8-bit paged cache with a scale for each block of `block` tokens of a page
  * and kv head: codes that stand for code * 2^(b - 127), b = k[page][slot /
- * block][head] (v), bytes 7 .. 247 of E8M0 [pages, page_size / block, kv_heads].
+ * block][head] (v), bytes 7 .. 246 of E8M0 [pages, page_size / block, kv_heads].
  * block: 16, 32, 64 or 128, at most page_size.  The cache's record has fp8 and
  * null scales then.  A power of two: codes keep their value when a block's
  * scale grows, and the matrix cores' operands are converted with it.
@@ -725,7 +725,7 @@ typedef struct fp8lin_block_scales {
  * with one rounding into q_out (BF16) and into the cache: BF16; with scales
  * null in an 8-bit cache E4M3FN(x / scale) as fp8lin_paged_append's; else block
  * scales:
- *   A block's scale is the least 2^e, e from -120 on, with |x| <= 448 2^e for
+ *   A block's scale is the least 2^e, e of -120 .. 119, with |x| <= 448 2^e for
  *   the finite values of the call's rows in it, and no less than the scale
  *   that the block had, unless the rows write the block's first slot: then it
  *   starts anew, and what its slots hold that the call does not write is lost.
@@ -748,6 +748,19 @@ int fp8lin_paged_rotate_append(const fp8lin_paged_cache* cache, const fp8lin_blo
                                double eps, int centered, const int64_t* positions, int64_t axes, int64_t axis_stride,
                                const int64_t* slots, int64_t tokens, uint16_t* q_out, int64_t out_token,
                                int64_t out_head, fp8lin_stream_t stream);
+
+/* fp8lin_paged_attention over a cache with block scales: all that is said there,
+ * with K and V = code * 2^(b - 127), exact in BF16 for bytes b of 7 .. 246 (what
+ * the append writes); others give no defined values.  Same
+ * workspace.
+ */
+int fp8lin_paged_attention_blocks(const fp8lin_paged_cache* cache, const fp8lin_block_scales* scales, const uint16_t* q,
+                                  int64_t q_token, int64_t q_head, const uint16_t* gate, int64_t gate_token,
+                                  int64_t gate_head, const int32_t* table, int64_t table_ld, int64_t width,
+                                  const int32_t* offsets, const int32_t* lengths, int64_t requests, int64_t tokens,
+                                  int64_t heads, int64_t max_count, int causal, double scale, uint16_t* out,
+                                  int64_t out_token, int64_t out_head, void* workspace, size_t workspace_bytes,
+                                  fp8lin_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * Deterministic synthetic inputs (no reference counterpart; used by the

@@ -91,9 +91,9 @@ def row_bound(y, reach, normed):
 
 
 def power(top):
-    """The exponent of the least 2^e, e from -120, with top <= 448 2^e."""
+    """The exponent of the least 2^e, e of -120 .. 119, with top <= 448 2^e."""
     e = -120
-    while top > 448.0 * 2.0 ** e:
+    while top > 448.0 * 2.0 ** e and e < 119:
         e += 1
     return e
 

@@ -379,6 +379,11 @@ def test_append_values(fp8lin, gpu):
     assert c[0, 0, 0, :2].tolist() == [448.0, -448.0] and math.isnan(c[0, 0, 0, 2]) and float(c[0, 0, 0, 3]) == 3.0 * 2.0 ** -e
     assert (c[1, 0] == 0).all() and float(c[3, 0, 0, 1]) == 448.0 and float(c[3, 0, 0, 0]) == 0.0
     assert torch.equal(c[2, 0], (x[2].float() * 2.0 ** 120).to(torch.float8_e4m3fn).float()) and float(c[2, 0, 0, 0]) == 2.0 ** -9
+    # the largest finite values saturate, as their block's range ends at 448 2^119
+    big = torch.full((1, 1, 16), 3.38e38, dtype=torch.bfloat16, device=gpu)
+    fp8lin.paged_append(big, -big, torch.tensor([48], device=gpu), *cache, k_scale=scale[0], v_scale=scale[1])
+    assert [int(x.view(torch.uint8)[3, 0, 0]) for x in scale] == [246, 246]
+    assert [x.float()[3, 0, 0].unique().tolist() for x in cache] == [[448.0], [-448.0]]
     # a later token: the codes of the slots before it, and NaN, under the greater scale
     y = torch.full((1, 1, 16), 1000.0, dtype=torch.bfloat16, device=gpu)
     fp8lin.paged_append(y, y, torch.tensor([1], device=gpu), *cache, k_scale=scale[0], v_scale=scale[1])
