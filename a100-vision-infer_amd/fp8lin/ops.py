@@ -39,6 +39,25 @@ def _stream(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice
+
+
+def call(name, device, *args):
+    """A library call on the device's current torch stream, with that device
+    current: the library launches on the current one."""
+    index = device.index
+    if index not in _ready_devices:
+        _stream(torch.empty(0, device=device))  # prepares the device once
+    if index == _current():
+        rc = getattr(lib(), name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(lib(), name)(*args, _raw_stream(index))
+    if rc:
+        check(rc)
+
+
 def _is_dev(t):
     return isinstance(t, torch.Tensor) and t.is_cuda
 

@@ -15,7 +15,7 @@ from collections import namedtuple
 import torch
 
 from ._lib import ERR_ARGUMENT, ERR_SHAPE, BlockScalesRecord, PagedCacheRecord, check, lib
-from .ops import _fail, _is_dev, _ready_devices, _stream
+from .ops import _fail, _is_dev, call as _call
 from .rotary import plan_record, positions_of
 
 PagedLayout = namedtuple("PagedLayout", "offsets lengths slots positions block_table cursor")
@@ -27,25 +27,8 @@ _FP8 = (torch.float8_e4m3fn, torch.uint8)
 
 # Calls of this module take the host about as long as the GPU where batches are
 # small, so their checks are one expression each and call nothing twice.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current = torch._C._cuda_getDevice
 _byref, _i32, _i64, _f32, _bf16 = ctypes.byref, torch.int32, torch.int64, torch.float32, torch.bfloat16
-_e8m0 = torch.float8_e8m0fnu
-
-
-def _call(name, device, *args):
-    """A library call on the device's current torch stream, with that device
-    current: the library launches on the current one."""
-    index = device.index
-    if index not in _ready_devices:
-        _stream(torch.empty(0, device=device))  # prepares the device once
-    if index == _current():
-        rc = getattr(lib(), name)(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = getattr(lib(), name)(*args, _raw_stream(index))
-    if rc:
-        check(rc)
+_e8m0, _contiguous = torch.float8_e8m0fnu, torch.contiguous_format
 
 
 def _vector(t, n, dtype, device):
@@ -103,8 +86,9 @@ def _cache(k_cache, v_cache, k_scale, v_scale):
     (torch.float8_e4m3fn or uint8) with a float32 scale per kv head or E8M0
     scales [pages, blocks, kv_heads] (torch.float8_e8m0fnu, contiguous) of
     page_size / blocks tokens each: the cache's, and the blocks' or None."""
-    if not (_is_dev(k_cache) and isinstance(v_cache, torch.Tensor) and k_cache.dim() == 4 and
-            k_cache.shape == v_cache.shape and k_cache.dtype is v_cache.dtype and k_cache.device == v_cache.device):
+    shape = k_cache.shape if isinstance(k_cache, torch.Tensor) else ()
+    if not (len(shape) == 4 and k_cache.is_cuda and isinstance(v_cache, torch.Tensor) and
+            shape == v_cache.shape and k_cache.dtype is v_cache.dtype and k_cache.device == v_cache.device):
         _fail(ERR_ARGUMENT, "Paged caches must be equal device tensors [pages, page_size, kv_heads, head_dim]")
     fp8 = k_cache.dtype in _FP8
     if not fp8 and k_cache.dtype is not _bf16:
@@ -112,30 +96,29 @@ def _cache(k_cache, v_cache, k_scale, v_scale):
     ks, vs = k_cache.stride(), v_cache.stride()
     if ks[3] != 1 or vs[3] != 1:
         _fail(ERR_ARGUMENT, "Paged caches need a contiguous last dimension")
-    pages, page_size, kv_heads, head_dim = k_cache.shape
-    blocks = None
+    pages, page_size, kv_heads, head_dim = shape
+    blocks = k_at = v_at = None
     if fp8 and isinstance(k_scale, torch.Tensor) and k_scale.dtype is _e8m0:
-        if not (isinstance(v_scale, torch.Tensor) and v_scale.dtype is _e8m0 and k_scale.dim() == 3 and k_scale.shape == v_scale.shape and
+        each = k_scale.shape
+        if not (isinstance(v_scale, torch.Tensor) and v_scale.dtype is _e8m0 and len(each) == 3 and each == v_scale.shape and
                 k_scale.is_contiguous() and v_scale.is_contiguous() and k_scale.device == v_scale.device == k_cache.device):
             _fail(ERR_ARGUMENT, "Scales of blocks must be equal contiguous E8M0 tensors [pages, blocks, kv_heads] on the cache's device")
-        n = k_scale.size(1)
-        if not (k_scale.size(0) == pages and k_scale.size(2) == kv_heads and n > 0 and page_size % n == 0):
+        if each[0] != pages or each[2] != kv_heads or not each[1] or page_size % each[1]:
             _fail(ERR_SHAPE, "Scales of blocks do not match the cache")
-        blocks = BlockScalesRecord(k_scale.data_ptr(), v_scale.data_ptr(), page_size // n)
+        blocks = BlockScalesRecord(k_scale.data_ptr(), v_scale.data_ptr(), page_size // each[1])
     elif fp8:
         if not (_vector(k_scale, kv_heads, _f32, k_cache.device) and _vector(v_scale, kv_heads, _f32, k_cache.device)):
             _fail(ERR_ARGUMENT, "An 8-bit cache needs float32 k_scale and v_scale [kv_heads]")
+        k_at, v_at = k_scale.data_ptr(), v_scale.data_ptr()
     elif k_scale is not None or v_scale is not None:
         _fail(ERR_ARGUMENT, "A BF16 cache has no scales")
-    own = fp8 and blocks is None
     return PagedCacheRecord(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages, page_size,
-                            kv_heads, head_dim, int(fp8), k_scale.data_ptr() if own else None,
-                            v_scale.data_ptr() if own else None), blocks
+                            kv_heads, head_dim, fp8, k_at, v_at), blocks
 
 
 def _heads(t, shape, device):
     """Whether t is a BF16 tensor of that shape on the device, its last dimension contiguous."""
-    return (isinstance(t, torch.Tensor) and t.dtype is _bf16 and t.shape == shape and t.device == device and t.stride(2) == 1)
+    return isinstance(t, torch.Tensor) and t.dtype is _bf16 and t.shape == shape and t.device == device and t.stride(2) == 1
 
 
 def paged_append(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
@@ -182,28 +165,27 @@ def paged_rotate_append(q, k, v, positions, slots, k_cache, v_cache, plan, q_nor
     dim = rec.head_dim
     if not (isinstance(q, torch.Tensor) and q.dim() == 3):
         _fail(ERR_ARGUMENT, "Paged rotate append expects BF16 queries [tokens, heads, head_dim]")
-    tokens, heads = q.shape[:2]
+    tokens, heads, _ = q.shape
     shape, kv_shape = (tokens, heads, dim), (tokens, rec.kv_heads, dim)
     if not (_heads(q, shape, device) and _heads(k, kv_shape, device) and _heads(v, kv_shape, device)):
         _fail(ERR_ARGUMENT, "Paged rotate append expects BF16 queries, keys and values [tokens, heads, head_dim]")
     if not _vector(slots, tokens, _i64, device):
         _fail(ERR_ARGUMENT, "Paged rotate append expects int64 slots [tokens]")
-    for w in (q_norm, k_norm):
-        if w is not None and not _vector(w, dim, _bf16, device):
-            _fail(ERR_ARGUMENT, "Paged rotate append expects BF16 norms [head_dim]")
+    if not ((q_norm is None or _vector(q_norm, dim, _bf16, device)) and (k_norm is None or _vector(k_norm, dim, _bf16, device))):
+        _fail(ERR_ARGUMENT, "Paged rotate append expects BF16 norms [head_dim]")
     rotary, axes, axis, at = None, 1, 0, None
     if plan is not None:
         rotary = _byref(plan_record(plan, device))
         axes, axis, at = positions_of(positions, tokens, device)
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q, memory_format=_contiguous)
     elif not _heads(out, shape, device):
         _fail(ERR_ARGUMENT, "Paged rotate append expects a BF16 output as the queries")
     if tokens:
         qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
         _call("fp8lin_paged_rotate_append", device, _byref(rec), None if blocks is None else _byref(blocks), rotary, q.data_ptr(),
               qs[0], qs[1], heads, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-              None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), float(eps), int(bool(centered)),
+              None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), float(eps), bool(centered),
               at, axes, axis, slots.data_ptr(), tokens, out.data_ptr(), os[0], os[1])
     return out
 
@@ -243,7 +225,7 @@ def paged_attention(q, k_cache, v_cache, block_table, offsets, lengths, max_coun
     else:
         gs, gate_at = (0, 0), None
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q, memory_format=_contiguous)
     elif not _heads(out, shape, device):
         _fail(ERR_ARGUMENT, "Paged attention expects a BF16 output as the queries")
     count = max(tokens - requests + 1, 1) if max_count is None else int(max_count)

@@ -11,7 +11,7 @@ from collections import namedtuple
 import torch
 
 from ._lib import ERR_ARGUMENT, ERR_SHAPE, RotaryRecord, check, lib
-from .ops import _fail, _is_dev, _ready_devices, _stream
+from .ops import _fail, call
 
 RotaryPlan = namedtuple("RotaryPlan", "steps magnitude neighbours")
 RotaryPlan.__doc__ = """What rotates heads: steps int64 [rotary / 2] on the device (4 * round(frequency / 2 pi * 2^62) + axis of each pair, as
@@ -66,21 +66,22 @@ def rotary_plan(rotary, theta=10000.0, scaling=None, neighbours=False, sections=
 
 def plan_record(plan, device):
     """The library's record of a plan whose steps are on the device."""
-    steps = plan.steps if isinstance(plan, RotaryPlan) else None
+    steps = plan[0] if isinstance(plan, RotaryPlan) else None
     if not (isinstance(steps, torch.Tensor) and steps.dtype is torch.int64 and steps.dim() == 1 and steps.is_contiguous() and
             steps.device == device):
         _fail(ERR_ARGUMENT, "Rotation expects a RotaryPlan on the tensors' device")
-    return RotaryRecord(steps.data_ptr(), 2 * steps.size(0), int(plan.neighbours), float(plan.magnitude))
+    return RotaryRecord(steps.data_ptr(), 2 * steps.size(0), bool(plan[2]), float(plan[1]))
 
 
 def positions_of(positions, tokens, device):
     """(axes, elements between them, pointer) of positions int64 [tokens] or [axes, tokens], a row contiguous."""
-    if not (isinstance(positions, torch.Tensor) and positions.dtype is torch.int64 and positions.device == device and
-            1 <= positions.dim() <= 2 and positions.size(-1) == tokens and (tokens <= 1 or positions.stride(-1) == 1)):
+    shape = positions.shape if isinstance(positions, torch.Tensor) else ()
+    if not (1 <= len(shape) <= 2 and positions.dtype is torch.int64 and positions.device == device and shape[-1] == tokens and
+            (tokens <= 1 or positions.stride(-1) == 1)):
         _fail(ERR_ARGUMENT, "Rotation expects int64 positions [tokens] or [axes, tokens]")
-    if positions.dim() == 1:
+    if len(shape) == 1:
         return 1, 0, positions.data_ptr()
-    return positions.size(0), positions.stride(0) if positions.size(0) > 1 else 0, positions.data_ptr()
+    return shape[0], positions.stride(0) if shape[0] > 1 else 0, positions.data_ptr()
 
 
 def rotate(x, positions, plan, transposed=False, out=None):
@@ -89,21 +90,17 @@ def rotate(x, positions, plan, transposed=False, out=None):
     transposed: turned back (times the magnitude), which is also the gradient
     with respect to x of one with respect to the result.  Returns BF16 [tokens,
     heads, head_dim]: `out` if given, which may be x and overlaps no other input."""
-    if not (_is_dev(x) and x.dim() == 3 and x.dtype is torch.bfloat16 and x.stride(2) == 1):
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 3 and x.dtype is torch.bfloat16 and x.stride(2) == 1):
         _fail(ERR_ARGUMENT, "Rotation expects BF16 heads [tokens, heads, head_dim]")
     device, (tokens, heads, dim) = x.device, x.shape
     record = plan_record(plan, device)
     axes, axis, at = positions_of(positions, tokens, device)
     if out is None:
-        out = x.new_empty(x.shape)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif not (isinstance(out, torch.Tensor) and out.shape == x.shape and out.dtype is torch.bfloat16 and out.device == device and
               out.stride(2) == 1):
         _fail(ERR_ARGUMENT, "Rotation expects a BF16 output as the input")
     xs, os = x.stride(), out.stride()
-    index = device.index
-    if index not in _ready_devices:
-        _stream(x)  # prepares the device once
-    with torch.cuda.device(index):
-        check(lib().fp8lin_rotate(ctypes.byref(record), x.data_ptr(), xs[0], xs[1], tokens, heads, dim, at, axes, axis, int(bool(transposed)),
-                                  out.data_ptr(), os[0], os[1], torch._C._cuda_getCurrentRawStream(index)))
+    call("fp8lin_rotate", device, ctypes.byref(record), x.data_ptr(), xs[0], xs[1], tokens, heads, dim, at, axes, axis, bool(transposed),
+         out.data_ptr(), os[0], os[1])
     return out
