@@ -751,8 +751,8 @@ int fp8lin_paged_rotate_append(const fp8lin_paged_cache* cache, const fp8lin_blo
 
 /* fp8lin_paged_attention over a cache with block scales: all that is said there,
  * with K and V = code * 2^(b - 127), exact in BF16 for bytes b of 7 .. 246 (what
- * the append writes); others give no defined values.  Same
- * workspace.
+ * the append writes); others give no defined values.  Weights below 2^-114 of a
+ * row's largest may be lost.  Same workspace.
  */
 int fp8lin_paged_attention_blocks(const fp8lin_paged_cache* cache, const fp8lin_block_scales* scales, const uint16_t* q,
                                   int64_t q_token, int64_t q_head, const uint16_t* gate, int64_t gate_token,
