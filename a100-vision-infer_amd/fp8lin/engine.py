@@ -17,7 +17,8 @@ import torch
 
 from ._lib import (ERR_ARGUMENT, PATH_FP8_GEMM, PATH_FP8_GEMV, PATH_TENSOR_SMALL, Fp8linError, LinearOptions, Weight, check, lib)
 from .ops import fp8_decode, fused_swiglu, qk_norm_rope
-from .paged import paged_append, paged_attention
+from .paged import paged_append, paged_attention, paged_rotate_append
+from .rotary import RotaryPlan
 
 
 def check_options(options):
@@ -196,8 +197,11 @@ class LinearEngine:
         q and k are RMS-normalised per head (centered, q_norm / k_norm) and
         rotated by the interleaved mRoPE of `rope` (the model config's
         rope_parameters: partial_rotary_factor, mrope_section, rope_theta), in
-        one launch; gate and v are as in qkv_gate_views.  Returns
+        one launch; gate and v are as in qkv_gate_views (a RotaryPlan is
+        full_attention's alone).  Returns
         (q [T,H,D], gate [T,H*D], k [T,HK,D], v [T,HK,D])."""
+        if isinstance(rope, RotaryPlan):
+            raise Fp8linError(ERR_ARGUMENT, "full_attention_inputs takes the config's rope_parameters")
         projected = self.linear(x, prefix + ".qkv_gate")
         _, gate, _, v = self.qkv_gate_views(projected, heads, kv_heads, head_dim)
         rotary = int(head_dim * rope.get("partial_rotary_factor", 0.25))
@@ -214,21 +218,31 @@ class LinearEngine:
         slots, attention over the requests' pages with the output gate, and
         linear(o_proj); the cross-rank reduce is the caller's.  layout: the
         step's PagedLayout (paged_layout).  positions int64 [3, tokens]: the
-        mRoPE positions (default: layout.positions on every axis).  The gate
+        mRoPE positions (default: layout.positions on every axis).  The caches
+        and scales are paged_append's.  rope: the config's rope_parameters, for
+        the reference's arithmetic (qk_norm_rope, then paged_append), or a
+        RotaryPlan, for paged_rotate_append's: frequencies scaled for long
+        contexts, either pairing, one rounding, and one launch.  The gate
         and the values are read where the projection wrote them.  Rows of no
         request (behind the last one) come out as o_proj of zeros."""
         projected = self.linear(x, prefix + ".qkv_gate")
         T, H, HK, D = projected.size(0), heads, kv_heads, head_dim
         if projected.size(-1) != 2 * (H + HK) * D:
             raise Fp8linError(ERR_ARGUMENT, "QKV-gate output width does not match the head layout")
-        if positions is None:
-            positions = layout.positions.expand(3, T)
-        rotary, sections = int(D * rope.get("partial_rotary_factor", 0.25)), rope["mrope_section"]
-        q, k = qk_norm_rope(projected, q_norm, k_norm, positions, H, HK, D, rotary, rope["rope_theta"], sections[1],
-                            sections[2], eps)
-        gate = projected[:, :2 * H * D].view(T, H, 2 * D)[..., D:]
+        query_gate = projected[:, :2 * H * D].view(T, H, 2 * D)
+        gate = query_gate[..., D:]
         v = projected[:, (2 * H + HK) * D:].view(T, HK, D)
-        paged_append(k, v, layout.slots, k_cache, v_cache, k_scale=k_scale, v_scale=v_scale)
+        if isinstance(rope, RotaryPlan):
+            k = projected[:, 2 * H * D:(2 * H + HK) * D].view(T, HK, D)
+            q = paged_rotate_append(query_gate[..., :D], k, v, layout.positions if positions is None else positions, layout.slots, k_cache,
+                                    v_cache, rope, q_norm=q_norm, k_norm=k_norm, eps=eps, k_scale=k_scale, v_scale=v_scale)
+        else:
+            if positions is None:
+                positions = layout.positions.expand(3, T)
+            rotary, sections = int(D * rope.get("partial_rotary_factor", 0.25)), rope["mrope_section"]
+            q, k = qk_norm_rope(projected, q_norm, k_norm, positions, H, HK, D, rotary, rope["rope_theta"], sections[1],
+                                sections[2], eps)
+            paged_append(k, v, layout.slots, k_cache, v_cache, k_scale=k_scale, v_scale=v_scale)
         # the attention leaves rows of no request as they are: zeros, not what the memory held
         core = paged_attention(q, k_cache, v_cache, layout.block_table, layout.offsets, layout.lengths, max_count=max_count,
                                gate=gate, k_scale=k_scale, v_scale=v_scale, out=torch.zeros_like(q))
