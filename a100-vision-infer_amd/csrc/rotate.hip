@@ -420,6 +420,50 @@ int run_lds(int half, int block_bits, int lane_bits) {
     return (int)sizeof(RunLds) + 8 * turns_of(half) * (1 + cap) + 32 * kThreads * (cap >> (8 - lane_bits));
 }
 
+// The slots of a block that n rows write.
+template <class SLOT>
+__device__ __forceinline__ void written_slots(SLOT slot_at, int64_t n, int block, uint32_t (&written)[4]) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) written[w] = 0;
+#pragma unroll 1
+    for (int64_t i = 0; i < n; ++i) {
+        const int s = (int)(slot_at(i) & (block - 1));
+#pragma unroll
+        for (int w = 0; w < 4; ++w) written[w] |= s >> 5 == w ? 1u << (s & 31) : 0;
+    }
+}
+// The codes of a block's other slots times f, by `team` lanes, 16 a lane and 4 of
+// those in flight.  The blocks of a decode step's requests grow now and then, so
+// each step has some (61 requests, blocks of 64, 2 heads of 256: 7 us without one,
+// GROW with every block).
+__device__ __forceinline__ void grow_block(uint8_t* codes, int64_t slot_stride, int block, int D, float f, const uint32_t (&written)[4], int tid,
+                                           int team) {
+    constexpr int UN = 4;
+    const int per = D / 16, pieces = block * per;
+#pragma unroll 1
+    for (int p0 = tid; p0 < pieces; p0 += UN * team) {
+        u32x4 w[UN];
+        u32x4* at[UN];
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+            const int p = p0 + i * team, s = p / per;
+            const uint32_t mask = s < 32 ? written[0] : s < 64 ? written[1] : s < 96 ? written[2] : written[3];
+            at[i] = p < pieces && !(mask >> (s & 31) & 1) ? reinterpret_cast<u32x4*>(codes + s * slot_stride + 16 * (p - s * per)) : nullptr;
+            if (at[i]) w[i] = *at[i];
+        }
+#pragma unroll
+        for (int i = 0; i < UN; ++i)
+            if (at[i]) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f32x2 lo = fp8x2_to_f32<false>(w[i][k]), hi = fp8x2_to_f32<true>(w[i][k]);
+                    w[i][k] = codes4(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
+                }
+                *at[i] = w[i];
+            }
+    }
+}
+
 // Rows i0 .. i0 + n of the window, all of one block of one head, by the lanes that
 // hold a row (which take the rows in turn), by a wave or by the workgroup: their
 // largest value gives the block's power of two; where that grows, the block's
@@ -470,7 +514,7 @@ __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, i
     uint8_t* codes = static_cast<uint8_t*>(const_cast<void*>(is_v ? a.vc.data : a.kc.data)) + page * (is_v ? a.vc.page : a.kc.page) +
                      in_page * slot_stride + h * (is_v ? a.vc.head : a.kc.head);
     uint8_t* byte = (is_v ? a.v_pow : a.k_pow) + ((page << (a.page_bits - a.block_bits)) + (in_page >> a.block_bits)) * a.k.n + h;
-    const int old = min((int)*byte, kMaxPower);
+    const int old = n ? min((int)*byte, kMaxPower) : 0;
     float wx[kPairs] = {}, wy[kPairs] = {};
     if (norm && live) unpack<LAYOUT>(load_pairs<LAYOUT>(norm, at, half, D, nb), wx, wy);
     add_center(wx, wy, a.center);
@@ -478,10 +522,35 @@ __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, i
     float x[kPairs], y[kPairs], top = 0.0f, factor = 1.0f;
     int power = 0;
     bool fresh = false, odd = false;  // odd: some value does not fit its block's range, infinities are left out of it
+    bool any_odd = false;             // of the wave's blocks: the passes are the whole wave's, as it shares the growing
     enum { kLargest, kLargestFinite, kStore };
 #pragma unroll 1
     for (int pass = kLargest; pass <= kStore; ++pass) {
-        if (pass == kLargestFinite && !odd) continue;
+        if (pass == kLargestFinite && !any_odd) continue;
+        if (pass == kStore) {
+            // by the whole wave or workgroup, whosever block it is
+            const bool grows = n && !fresh && old < power;
+            if constexpr (TEAM == kAll) {
+                if (grows) {
+                    uint32_t written[4];
+                    written_slots(slot_at, n, block, written);
+                    grow_block(codes, slot_stride, block, D, power_of(127 + old - power), written, tid, kThreads);
+                }
+            } else {
+                for (uint64_t left = __ballot(grows); left;) {
+                    const int from = __builtin_ctzll(left);
+                    left &= TEAM == kWave ? 0 : ~(((lanes < 64 ? 1ull << lanes : 0) - 1) << from);
+                    const int first = __builtin_amdgcn_readlane(i0, from), rows = __builtin_amdgcn_readlane((int)n, from);
+                    const uint64_t to = (uint64_t)(uintptr_t)codes;
+                    const uint64_t at0 = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)to, from) |
+                                         (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(to >> 32), from) << 32;
+                    const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, power_of(127 + old - power)), from));
+                    uint32_t written[4];
+                    written_slots([&](int64_t i) { return lds.slots[first + i]; }, rows, block, written);
+                    grow_block(reinterpret_cast<uint8_t*>(at0), slot_stride, block, D, f, written, threadIdx.x & 63, 64);
+                }
+            }
+        }
 #pragma unroll 1
         for (int64_t k = 0; k * G < n; ++k) {
             const int64_t i = k * G + g;
@@ -507,8 +576,8 @@ __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, i
 #pragma unroll
                 for (int j = 0; j < kPairs; ++j) {
                     const float u = fabsf(x[j]), v = fabsf(y[j]);
-                    top = fmaxf(top, u < __builtin_inff() ? u : 0.0f);
-                    top = fmaxf(top, v < __builtin_inff() ? v : 0.0f);
+                    top = fmaxf(top, odd && u < __builtin_inff() ? u : 0.0f);
+                    top = fmaxf(top, odd && v < __builtin_inff() ? v : 0.0f);
                 }
             } else if (live && i < n) {
 #pragma unroll
@@ -532,31 +601,17 @@ __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, i
             for (int w = 0; w < kThreads / 64; ++w) top = fmaxf(top, lds.tops[w]);
             __syncthreads();
         }
-        if (pass == kLargest && top > 448.0f * power_of(kMaxPower)) {
-            odd = true;
-            top = 0.0f;
-            continue;
+        if (pass == kLargest) {
+            odd = top > 448.0f * power_of(kMaxPower);
+            any_odd = TEAM == kAll ? odd : __any(odd);
+            if (odd) top = 0.0f;
+            if (any_odd) continue;
         }
         power = block_power(top);
-        if (!fresh && old < power) {
-            // 4 codes a lane of the slots that the rows do not write: seldom, so each lane looks its slot up
-            const float f = power_of(127 + old - power);
-#pragma unroll 1
-            for (int e = tid; e < block * (D / 4); e += team) {
-                const int s = e / (D / 4), d = 4 * (e % (D / 4));
-                bool written = false;
-#pragma unroll 1
-                for (int64_t i = 0; i < n; ++i) written |= (int)(slot_at(i) & (block - 1)) == s;
-                if (written) continue;
-                uint32_t* w = reinterpret_cast<uint32_t*>(codes + s * slot_stride + d);
-                const f32x2 lo = fp8x2_to_f32<false>(*w), hi = fp8x2_to_f32<true>(*w);
-                *w = codes4(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
-            }
-        }
         if (!fresh) power = max(power, old);
         factor = power_of(254 - power);
     }
-    if (tid == 0) *byte = (uint8_t)power;
+    if (tid == 0 && n) *byte = (uint8_t)power;
 }
 
 // The runs of one head of the keys or values that begin in the tokens first ..
@@ -597,12 +652,13 @@ __device__ __forceinline__ void append_runs(const RotateAppend& a, RunLds& lds, 
     const bool is_border = i < 64 ? border[0] >> i & 1 : border[1] & 1;
     const uint64_t begins = __ballot(first + lane < last && is_border && block_of(lds.slots[i]) >= 0);
     const uint64_t ones = begins & __ballot(rows <= 2), waves = begins & __ballot(rows > 2 && rows <= 2 * few), all = begins & ~ones & ~waves;
+    // in turn over the waves, which grow their blocks one after the other
     uint64_t left = ones;
-    for (int skip = tid >> lane_bits; left && skip; --skip) left &= left - 1;
+    for (int skip = (lane >> lane_bits) * WORDS + wave; left && skip; --skip) left &= left - 1;
 #pragma unroll 1
     while (__any(left != 0)) {
         const int at = left ? __builtin_ctzll(left) : 0, n = __shfl(rows, at, 64);
-        if (left) append_run<LAYOUT, kOne>(a, lds, lane_bits, window, at + 1, n, h, is_v);
+        append_run<LAYOUT, kOne>(a, lds, lane_bits, window, at + 1, left ? n : 0, h, is_v);
         for (int skip = kThreads >> lane_bits; left && skip; --skip) left &= left - 1;
     }
     int turn = 0;
@@ -684,11 +740,13 @@ hipError_t launch_rotate_append(const RotateAppend& a, hipStream_t stream) {
     const int mode = a.k_pow ? kBlocks : a.fp8 ? kHeads : kBf16, waves = kThreads / 64;
     const int bits = lane_bits_of(a.D), per = 64 >> bits, rows = a.q.n + (mode == kBlocks ? 0 : 2 * a.k.n);
     const int groups = (rows + per - 1) / per, units = mode == kBlocks ? 2 * a.k.n : 0;
-    // as many tokens as a workgroup's lanes hold rows, for the short runs of a decode
-    // step; where those are many workgroups, a block, as one that finds no run takes
-    // some us, too (a prompt of 2000 tokens in blocks of 64, heads of 256: 17 us with 64
-    // tokens, 22 with 16; 3913: 18 and 38)
-    int run_bits = std::min(8 - bits, 6);
+    // few tokens each, so that the runs of a decode step spread over the chip, but no
+    // fewer than waves, and no more than the lanes hold rows; where that makes many
+    // workgroups, a block, as one that finds no run takes some us, too (a prompt of
+    // 2000 tokens in blocks of 64, heads of 256: 17 us with 64 tokens, 22 with 16; 3913:
+    // 18 and 38)
+    int run_bits = 2;
+    while (run_bits < std::min(8 - bits, 6) && (a.T * units >> run_bits) > kManyRuns) ++run_bits;
     if ((a.T * units >> run_bits) > kManyRuns) run_bits = std::max(run_bits, std::min(a.block_bits, 6));
     const int64_t run_groups = ((a.T + (1 << run_bits) - 1) >> run_bits) * units;
     const int lds = std::max(mode == kBlocks ? run_lds(a.r.half, a.block_bits, bits) : 0, waves * turns_of(a.r.half) * (int)sizeof(f32x2));
