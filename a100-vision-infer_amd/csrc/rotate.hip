@@ -408,16 +408,16 @@ struct RunLds {
     __device__ __forceinline__ f32x2* turns(int half) { return reinterpret_cast<f32x2*>(steps() + turns_of(half)); }
     __device__ __forceinline__ u32x4* rows(int half, int cap) { return reinterpret_cast<u32x4*>(turns(half) + cap * turns_of(half)); }
 };
-// Rows in hand: a block's, of two to kKeep times what the workgroup's lanes hold at once.
+// Rows in hand: a block's, of one to kKeep times what the workgroup's lanes hold at once.
 __host__ __device__ __forceinline__ int cap_of(int block_bits, int lane_bits) {
     const int once = kThreads >> lane_bits, block = 1 << block_bits;
-    return block < 2 * once ? 2 * once : block < kKeep * once ? block : kKeep * once;
+    return block < once ? once : block < kKeep * once ? block : kKeep * once;
 }
 // The most: heads of 1024, all of them rotated (16 rows' turns of 512).
 constexpr int kMaxLds = 112 * 1024;
 int run_lds(int half, int block_bits, int lane_bits) {
     const int cap = cap_of(block_bits, lane_bits);
-    return (int)sizeof(RunLds) + 8 * turns_of(half) * (1 + cap) + 32 * kThreads * (cap >> (8 - lane_bits));
+    return (int)sizeof(RunLds) + 8 * turns_of(half) * (1 + cap) + 32 * kThreads * ((cap >> (8 - lane_bits)) - 1);
 }
 
 // The slots of a block that n rows write.
@@ -434,8 +434,8 @@ __device__ __forceinline__ void written_slots(SLOT slot_at, int64_t n, int block
 }
 // The codes of a block's other slots times f, by `team` lanes, 16 a lane and 4 of
 // those in flight.  The blocks of a decode step's requests grow now and then, so
-// each step has some (61 requests, blocks of 64, 2 heads of 256: 7 us without one,
-// GROW with every block).
+// most steps have some (61 requests, blocks of 64, 2 heads of 256: 7.5 us, and 13
+// where every block grows; by the lanes of the row alone 200).
 __device__ __forceinline__ void grow_block(uint8_t* codes, int64_t slot_stride, int block, int D, float f, const uint32_t (&written)[4], int tid,
                                            int team) {
     constexpr int UN = 4;
@@ -465,7 +465,7 @@ __device__ __forceinline__ void grow_block(uint8_t* codes, int64_t slot_stride, 
 }
 
 // Rows i0 .. i0 + n of the window, all of one block of one head, by the lanes that
-// hold a row (which take the rows in turn), by a wave or by the workgroup: their
+// hold a row, by a wave or by the workgroup: their
 // largest value gives the block's power of two; where that grows, the block's
 // other codes are multiplied; then the rows' codes.
 //
@@ -477,7 +477,6 @@ __device__ __forceinline__ void grow_block(uint8_t* codes, int64_t slot_stride, 
 enum Team { kOne, kWave, kAll };
 template <int LAYOUT, int TEAM>
 __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, int lane_bits, int64_t window, int i0, int64_t n, int h, bool is_v) {
-    constexpr int KEEP = TEAM == kAll ? kKeep : 2;  // rows of a lane whose loads go out together
     const int lanes = 1 << lane_bits, team = TEAM == kAll ? kThreads : TEAM == kWave ? 64 : lanes, tid = threadIdx.x & (team - 1), l = tid & (lanes - 1), g = tid >> lane_bits;
     const int G = team >> lane_bits;
     const bool nb = a.r.neighbours;
@@ -487,8 +486,8 @@ __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, i
     const int64_t t0 = window + i0, row_stride = is_v ? a.v.tok : a.k.tok;
     const uint16_t* rows = (is_v ? a.v.x + h * a.v.head : a.k.x + h * a.k.head) + t0 * row_stride;
     const uint16_t* norm = is_v ? nullptr : a.k_norm;
-    const int all_cap = cap_of(a.block_bits, lane_bits), cap = TEAM == kAll ? all_cap : 2 * G;
-    f32x2* turns = lds.turns(half) + ((int)threadIdx.x - tid >> lane_bits) * 2 * turns_of(half);  // kAll: the first
+    const int all_cap = cap_of(a.block_bits, lane_bits), cap = TEAM == kAll ? all_cap : G;
+    f32x2* turns = lds.turns(half) + ((int)threadIdx.x - tid >> lane_bits) * turns_of(half);  // kAll: the first
     u32x4* held = lds.rows(half, all_cap) + threadIdx.x;
     auto slot_at = [&](int64_t i) { return i0 + i < kThreads ? lds.slots[i0 + i] : a.slots[t0 + i]; };
     auto load = [&](int64_t i) __attribute__((always_inline)) {
@@ -497,16 +496,16 @@ __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, i
         return p;
     };
     Packed mine = load(g);
-    {
-        Packed more[KEEP - 1];
+    if constexpr (TEAM == kAll) {
+        Packed more[kKeep - 1];
 #pragma unroll
-        for (int k = 1; k < KEEP; ++k)
+        for (int k = 1; k < kKeep; ++k)
             if (k * G < cap) more[k - 1] = load(k * G + g);
 #pragma unroll
-        for (int k = 1; k < KEEP; ++k)
+        for (int k = 1; k < kKeep; ++k)
             if (k * G < cap) {
-                held[2 * k * kThreads] = more[k - 1].a;
-                held[(2 * k + 1) * kThreads] = more[k - 1].b;
+                held[2 * (k - 1) * kThreads] = more[k - 1].a;
+                held[(2 * k - 1) * kThreads] = more[k - 1].b;
             }
     }
     const int64_t slot0 = slot_at(0) >> a.block_bits << a.block_bits, page = slot0 >> a.page_bits, slot_stride = is_v ? a.vc.slot : a.kc.slot;
@@ -556,7 +555,7 @@ __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, i
             const int64_t i = k * G + g;
             if (pass == kLargest || n > G) {
                 Packed w = mine;
-                if (k) w = k * G < cap ? Packed{held[2 * k * kThreads], held[(2 * k + 1) * kThreads]} : load(i);
+                if (TEAM == kAll && k) w = k * G < cap ? Packed{held[2 * (k - 1) * kThreads], held[(2 * k - 1) * kThreads]} : load(i);
                 unpack<LAYOUT>(w, x, y);
                 if (!is_v) {
                     if (norm) norm_pairs(x, y, wx, wy, lanes, D, a.eps);
@@ -615,9 +614,9 @@ __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, i
 }
 
 // The runs of one head of the keys or values that begin in the tokens first ..
-// last, at most 64: those of one or two rows (a decode step's) by the lanes of a row
-// each, those of up to two times the rows that a wave holds (drafted tokens) by a
-// wave each, the others by the workgroup.  A run's end is in the window, as it has
+// last, at most 64: those of one row (a decode step's) by the lanes of a row each,
+// those of up to the rows that a wave holds (drafted tokens) by a wave each, the
+// others by the workgroup.  A run's end is in the window, as it has
 // no more rows than a block has slots, if none comes twice.
 template <int LAYOUT>
 __device__ __forceinline__ void append_runs(const RotateAppend& a, RunLds& lds, int lane_bits, int64_t first, int64_t last, int unit) {
@@ -651,7 +650,7 @@ __device__ __forceinline__ void append_runs(const RotateAppend& a, RunLds& lds, 
     const int rows = end - i, few = 64 >> lane_bits;
     const bool is_border = i < 64 ? border[0] >> i & 1 : border[1] & 1;
     const uint64_t begins = __ballot(first + lane < last && is_border && block_of(lds.slots[i]) >= 0);
-    const uint64_t ones = begins & __ballot(rows <= 2), waves = begins & __ballot(rows > 2 && rows <= 2 * few), all = begins & ~ones & ~waves;
+    const uint64_t ones = begins & __ballot(rows == 1), waves = begins & __ballot(rows > 1 && rows <= few), all = begins & ~ones & ~waves;
     // in turn over the waves, which grow their blocks one after the other
     uint64_t left = ones;
     for (int skip = (lane >> lane_bits) * WORDS + wave; left && skip; --skip) left &= left - 1;
