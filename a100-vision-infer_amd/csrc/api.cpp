@@ -569,6 +569,11 @@ bool overlap(const Extent& a, const Extent& b) {
     if (a.rows > b.rows) return overlap(b, a);
     const __int128 a0 = (intptr_t)a.at, b0 = (intptr_t)b.at, stride = b.rows > 1 ? b.stride : b.width;
     if (a0 >= b0 + (b.rows - 1) * stride + b.width || b0 >= a0 + (a.rows - 1) * (__int128)a.stride + a.width) return false;
+    if (a.rows > 1 && a.stride == b.stride && a.width <= a.stride && b.width <= b.stride) {
+        // parts of one matrix' rows, side by side
+        const __int128 d = ((b0 - a0) % stride + stride) % stride;
+        if (d >= a.width && d + b.width <= stride) return false;
+    }
     for (int64_t i = 0; i < a.rows; ++i) {
         const __int128 lo = a0 + i * (__int128)a.stride, hi = lo + a.width;
         if (hi <= b0) continue;
@@ -598,7 +603,7 @@ Extent heads_extent(const void* at, int64_t tokens, int64_t heads, int64_t dim, 
     return Extent{at, heads ? 1 : 0, all, all};
 }
 void check_heads(int64_t tokens, int64_t heads, int64_t token, int64_t head, const char* what) {
-    require(token >= 0 && head >= 0 && heads < kMaxDim && tokens < kMaxDim && (double)tokens * token < 0x1p56 && (double)heads * head < 0x1p56,
+    require(token >= 0 && head >= 0 && heads < kMaxDim / 2 && tokens < kMaxDim && (double)tokens * token < 0x1p56 && (double)heads * head < 0x1p56,
             FP8LIN_ERR_SHAPE, what);
 }
 
@@ -1330,7 +1335,7 @@ int fp8lin_paged_rotate_append(const fp8lin_paged_cache* cache, const fp8lin_blo
         fp8lin::RotateAppend a{};
         check_cache(cache, a.kc, a.vc, scales);
         const int64_t dim = cache->head_dim, hk = cache->kv_heads;
-        require(tokens >= 0 && tokens < kMaxDim && heads >= 0 && heads < kMaxDim, FP8LIN_ERR_SHAPE,
+        require(tokens >= 0 && tokens < kMaxDim && heads >= 0 && heads < kMaxDim / 2 && hk < kMaxDim / 4, FP8LIN_ERR_SHAPE,
                 "paged rotate append: invalid number of tokens or heads");
         require(dim % 16 == 0 && dim <= kMaxRotateDim, FP8LIN_ERR_UNSUPPORTED,
                 "paged rotate append: head_dim must be a multiple of 16, at most 1024");

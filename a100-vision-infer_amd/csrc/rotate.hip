@@ -568,9 +568,13 @@ __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, i
                 }
             }
             if (pass == kLargest) {
-                // NaN does not count
+                // NaN does not count: by comparisons, as a maximum with a signalling NaN is NaN
 #pragma unroll
-                for (int j = 0; j < kPairs; ++j) top = fmaxf(fmaxf(top, fabsf(x[j])), fabsf(y[j]));
+                for (int j = 0; j < kPairs; ++j) {
+                    const float u = fabsf(x[j]), v = fabsf(y[j]);
+                    top = u > top ? u : top;
+                    top = v > top ? v : top;
+                }
             } else if (pass == kLargestFinite) {
 #pragma unroll
                 for (int j = 0; j < kPairs; ++j) {

@@ -394,6 +394,28 @@ def test_append_values(fp8lin, gpu):
     assert torch.equal(c[0, 0, 0, :4].isnan(), want.isnan()) and torch.equal(c[0, 0, 0, :4].nan_to_num(), want.nan_to_num())
 
 
+@pytest.mark.parametrize("bits", [0x7f81, 0x7fc1, 0xff85])
+def test_append_nan_beside_large_values(fp8lin, gpu, bits):
+    """Quiet and signalling NaN count for nothing in their block's scale, wherever they stand, and stay NaN."""
+    g = torch.Generator().manual_seed(15)
+    for rows in (1, 3, 40):
+        x = torch.randn(rows, 2, 64, generator=g).to(torch.bfloat16)
+        x[0, :, 5], x[rows - 1, :, 44] = 70.0, -90.0
+        for r, d in ((0, 0), (0, 6), (rows - 1, 43), (rows // 2, 63)):
+            x.view(torch.int16)[r, :, d] = bits - (1 << 16 if bits >> 15 else 0)
+        cache = [torch.zeros(3, 32, 2, 64, dtype=torch.float8_e4m3fn, device=gpu) for _ in range(2)]
+        scale = [torch.full((3, 1, 2), 7, dtype=torch.uint8, device=gpu).view(torch.float8_e8m0fnu) for _ in range(2)]
+        fp8lin.paged_append(x.to(gpu), x.to(gpu), torch.arange(rows, device=gpu), *cache, k_scale=scale[0], v_scale=scale[1])
+        fine = x.float().nan_to_num(0.0)
+        for c, s in zip(cache, scale):
+            for lo in range(0, rows, 32):
+                e = [RO.power(float(fine[lo:lo + 32, h].abs().max())) for h in range(2)]
+                assert s.view(torch.uint8)[lo // 32, 0].tolist() == [p + 127 for p in e]
+                want = (x[lo:lo + 32].float() / torch.tensor([2.0 ** p for p in e])[:, None]).to(torch.float8_e4m3fn).float()
+                have = c.float().cpu()[lo // 32, :want.size(0)]
+                assert torch.equal(have.isnan(), want.isnan()) and torch.equal(have.nan_to_num(), want.nan_to_num())
+
+
 def test_append_strided_caches_and_outputs(fp8lin, gpu):
     """Caches [pages, kv_heads, page_size, dim] in memory, keys and values in one tensor, queries turned in place."""
     s = Step(fp8lin, gpu, [(7, 40), (64, 1)], 4, 2, 64, 32, "blocks", block=16, rotary=32, seed=12)

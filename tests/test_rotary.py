@@ -94,7 +94,7 @@ def rotate(fp8lin, plan=None, null=False, **kw):
     (dict(head_dim=63), 1), (dict(head_dim=0), 1), (dict(head_dim=1026), 1), (dict(axes=0), 1), (dict(axes=5), 1), (dict(axis_stride=-1), 1),
     (dict(x_token=-256), 1), (dict(y_head=1 << 60), 1), (dict(tokens=1 << 30), 1), (dict(tokens=0), 0), (dict(heads=0), 0),
     (dict(y=A + 2), 2), (dict(y=A + 64 * 2), 2), (dict(y=A, y_token=512), 2), (dict(positions=A + 0x400000), 2), (dict(y_token=128), 2),
-    (dict(y_head=32), 2), (dict(y_token=0), 2), (dict(y_token=64, y_head=64), 2), (dict(y=A + 0x900000), 2),
+    (dict(heads=1 << 30, tokens=1), 1), (dict(y_head=32), 2), (dict(y_token=0), 2), (dict(y_token=64, y_head=64), 2), (dict(y=A + 0x900000), 2),
 ], ids=str)
 def test_rotate_validation(fp8lin, change, code):
     assert rotate(fp8lin, **change) == code
@@ -170,6 +170,22 @@ def test_python_refuses_host_tensors(fp8lin):
                  lambda: fp8lin.paged_append(x, x, at, cache, cache, k_scale=scale, v_scale=scale)):
         with pytest.raises(fp8lin.Fp8linError):
             call()
+
+
+@pytest.mark.parametrize("change,code", [
+    # a token's row of 1024: queries of 64 in each 128 of its first 448, keys from 512 on, values from 640 on; 5 tokens
+    (dict(), 0), (dict(k=A + 2 * 447), 2), (dict(k=A + 2 * 448), 0), (dict(k=A + 2 * 896), 0), (dict(k=A + 2 * 897), 2),
+    (dict(k=A + 2 * (4 * 1024 + 447)), 2), (dict(k=A + 2 * (4 * 1024 + 448)), 0), (dict(v=A - 2 * (4 * 1024 + 127)), 2),
+    (dict(v=A - 2 * (4 * 1024 + 128)), 0),
+], ids=str)
+def test_append_in_place_in_one_matrix(fp8lin, change, code):
+    """Queries turned in place in the projection's rows, beside the keys and values."""
+    if not code and torch.cuda.is_available():
+        pytest.skip("what passes the checks would be launched on these addresses")
+    d = dict(q=A, q_token=1024, q_head=128, q_out=A, out_token=1024, out_head=128, k=A + 2 * 512, k_token=1024, v=A + 2 * 640, v_token=1024,
+             q_norm=A + 0x300000, k_norm=A + 0x301000)
+    # without a GPU what passes ends at the device
+    assert append(fp8lin, **{**d, **change}) == (code or 6)
 
 
 def test_the_oracle_by_differences():
