@@ -257,7 +257,7 @@ constexpr int kMixedRows = 32;  // rows of a few-rows tile of a mixed batch
 // and writes their rows.  Every workgroup lists the split units from the
 // pieces' beginnings and takes every gridDim.x-th part of them: 64 (WAVES 4:
 // its waves share the pieces of a unit, which are many and small in a decode
-// step) or 256 (WAVES 1) groups of 4 values.  ORDER::place(e, row, d): row and
+// step) or 1024 (WAVES 1) groups of 4 values.  ORDER::place(e, row, d): row and
 // first dimension of the e-th 4 floats of a piece's O.  The units of workgroups
 // with marked waves are computed again, row by row, instead.
 template <int BM, int D, int KIND, int WAVES, class ORDER>
@@ -295,65 +295,138 @@ __device__ __forceinline__ void join(const PagedAttention& a, int block, int blo
     if (tid > 0 && mine.x >= 0 && mine.w > 0 && (tid == kGroups - 1 || !same(begin[tid + 1], mine)))
         unit_last[at + (first ? 0 : -1)] = tid;
     __syncthreads();
-    const int q = WAVES > 1 ? wave : 0, et = WAVES > 1 ? lane : tid;
-    for (int item = block; item < units * PARTS; item += blocks) {
-        const int w = unit[item / PARTS], e = (item % PARTS) * PER + et;
-        const i32x4v u = begin[w];
-        const int r0 = u.z * BM, off = rows[w].x, nr = rows[w].y;
-        int row, d;
-        ORDER::place(e, row, d);
-        const bool ok = row < nr;
-        const int flat = r0 + min(row, nr - 1), tok = off + flat / a.G, head = u.y * a.G + flat % a.G;
-        u32x2 gate = {0, 0};
-        if (a.gate) gate = load_gate4(a.gate + tok * a.g_tok + head * a.g_head + d);
-        // the unit's pieces: workgroups w - 1 (slot 1), w, .. last (slot 0)
-        const int last = unit_last[item / PARTS];
-        if (any_bad) {
-            bool skip = false;
-            for (int g = w - 1; g <= last; ++g) skip |= bad[g] != 0;
-            if (skip) continue;
-        }
-        float M = -__builtin_inff(), l = 0.0f;
-        f32x4 o = {0, 0, 0, 0};
-        // A factor of 0 is multiplied in like any other: a part whose scores are
-        // all NaN has m = -inf and l = NaN, and a NaN stays one however little
-        // its part weighs; a part of nothing adds l = 0, O = 0.
-        auto add = [&](float m1, float l1, f32x4 o1) {
-            const float mn = fmaxf(M, m1);
-            const float f0 = M == -__builtin_inff() ? 0.0f : exp2_fast(M - mn);
-            const float f1 = m1 == -__builtin_inff() ? 0.0f : exp2_fast(m1 - mn);
-            l = l * f0 + l1 * f1;
+    if constexpr (WAVES == 1) {
+        // Bound by its vector instructions: what a row's values share (its place, its
+        // factors, 2^x of the maxima) is computed once for the SHARE groups of 4 that
+        // a thread takes of it, 64 apart in this order.  A prompt of 3913 tokens, heads
+        // of 256, took 167 us with one group a thread and takes 159 (join and all).
+        constexpr int SHARE = 4, ITEMS = PARTS / SHARE;
+        for (int item = block; item < units * ITEMS; item += blocks) {
+            const int w = unit[item / ITEMS], e = (item % ITEMS) * (PER * SHARE) + wave * (64 * SHARE) + lane;
+            const i32x4v u = begin[w];
+            const int r0 = u.z * BM, off = rows[w].x, nr = rows[w].y;
+            int row, d;
+            ORDER::place(e, row, d);
+            if (row >= nr) continue;
+            const int flat = r0 + row, tok = off + flat / a.G, head = u.y * a.G + flat % a.G;
+            u32x2 gate[SHARE];
+            if (a.gate) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = o[i] * f0 + o1[i] * f1;
-            M = mn;
-        };
-        if (ok) {
-            constexpr int UN = WAVES > 1 ? 8 : 4;  // pieces whose loads are in flight together
-            for (int g0 = w - 1 + q; g0 <= last; g0 += WAVES * UN) {
+                for (int k = 0; k < SHARE; ++k) gate[k] = load_gate4(a.gate + tok * a.g_tok + head * a.g_head + d + ORDER::kNext * k);
+            }
+            // the unit's pieces: workgroups w - 1 (slot 1), w, .. last (slot 0)
+            const int last = unit_last[item / ITEMS];
+            if (any_bad) {
+                bool skip = false;
+                for (int g = w - 1; g <= last; ++g) skip |= bad[g] != 0;
+                if (skip) continue;
+            }
+            float M = -__builtin_inff(), l = 0.0f;
+            f32x4 o[SHARE];
+#pragma unroll
+            for (int k = 0; k < SHARE; ++k) o[k] = f32x4{0, 0, 0, 0};
+            constexpr int UN = 2;  // pieces whose loads are in flight together
+            for (int g0 = w - 1; g0 <= last; g0 += UN) {
                 float m1[UN], l1[UN];
-                f32x4 o1[UN];
+                f32x4 o1[UN][SHARE];
+                bool there[UN];
 #pragma unroll
                 for (int i = 0; i < UN; ++i) {
-                    const int g = g0 + i * WAVES;
+                    const int g = g0 + i;
                     // an empty piece: the next one begins where it does
-                    const bool there = g <= last && !(g < last && g >= w && begin[g + 1].w == begin[g].w);
+                    there[i] = g <= last && !(g < last && g >= w && begin[g + 1].w == begin[g].w);
                     // loaded without a condition (another piece's), so that all are in flight
-                    const int from = there ? g : w - 1;
+                    const int from = there[i] ? g : w - 1;
                     const float* part = Partial<BM, D>::at(a.ws, from, from < w);
                     m1[i] = part[(int64_t)BM * D + row];
                     l1[i] = part[(int64_t)BM * D + BM + row];
-                    o1[i] = *reinterpret_cast<const f32x4*>(part + 4 * (int64_t)e);
-                    if (!there) {
-                        m1[i] = -__builtin_inff();
-                        l1[i] = 0.0f;
-                        o1[i] = f32x4{0, 0, 0, 0};
-                    }
+#pragma unroll
+                    for (int k = 0; k < SHARE; ++k) o1[i][k] = *reinterpret_cast<const f32x4*>(part + 4 * (int64_t)(e + 64 * k));
                 }
 #pragma unroll
-                for (int i = 0; i < UN; ++i) add(m1[i], l1[i], o1[i]);
+                for (int i = 0; i < UN; ++i) {
+                    if (!there[i]) continue;
+                    // as below, the products' places in the fused operations said
+                    const float mn = fmaxf(M, m1[i]);
+                    const float f0 = M == -__builtin_inff() ? 0.0f : exp2_fast(M - mn);
+                    const float f1 = m1[i] == -__builtin_inff() ? 0.0f : exp2_fast(m1[i] - mn);
+                    l = __builtin_fmaf(l1[i], f1, l * f0);
+#pragma unroll
+                    for (int k = 0; k < SHARE; ++k)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[k][j] = __builtin_fmaf(o1[i][k][j], f1, o[k][j] * f0);
+                    M = mn;
+                }
             }
+            const float inv = l == 0.0f ? 0.0f : (a.v_scale ? a.v_scale[u.y] : 1.0f) / l;
+#pragma unroll
+            for (int k = 0; k < SHARE; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[k][j] = l == 0.0f ? 0.0f : o[k][j] * inv;
+            if (a.gate) apply_gates<SHARE>(o, gate);
+            uint16_t* out = a.out + tok * a.o_tok + head * a.o_head + d;
+#pragma unroll
+            for (int k = 0; k < SHARE; ++k) store_bf16x4(out + ORDER::kNext * k, o[k]);
         }
-        if constexpr (WAVES > 1) {
+    } else {
+        const int q = wave, et = lane;
+        for (int item = block; item < units * PARTS; item += blocks) {
+            const int w = unit[item / PARTS], e = (item % PARTS) * PER + et;
+            const i32x4v u = begin[w];
+            const int r0 = u.z * BM, off = rows[w].x, nr = rows[w].y;
+            int row, d;
+            ORDER::place(e, row, d);
+            const bool ok = row < nr;
+            const int flat = r0 + min(row, nr - 1), tok = off + flat / a.G, head = u.y * a.G + flat % a.G;
+            u32x2 gate = {0, 0};
+            if (a.gate) gate = load_gate4(a.gate + tok * a.g_tok + head * a.g_head + d);
+            // the unit's pieces: workgroups w - 1 (slot 1), w, .. last (slot 0)
+            const int last = unit_last[item / PARTS];
+            if (any_bad) {
+                bool skip = false;
+                for (int g = w - 1; g <= last; ++g) skip |= bad[g] != 0;
+                if (skip) continue;
+            }
+            float M = -__builtin_inff(), l = 0.0f;
+            f32x4 o = {0, 0, 0, 0};
+            // A factor of 0 is multiplied in like any other: a part whose scores are
+            // all NaN has m = -inf and l = NaN, and a NaN stays one however little
+            // its part weighs; a part of nothing adds l = 0, O = 0.
+            auto add = [&](float m1, float l1, f32x4 o1) {
+                const float mn = fmaxf(M, m1);
+                const float f0 = M == -__builtin_inff() ? 0.0f : exp2_fast(M - mn);
+                const float f1 = m1 == -__builtin_inff() ? 0.0f : exp2_fast(m1 - mn);
+                l = l * f0 + l1 * f1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = o[i] * f0 + o1[i] * f1;
+                M = mn;
+            };
+            if (ok) {
+                constexpr int UN = 8;  // pieces whose loads are in flight together
+                for (int g0 = w - 1 + q; g0 <= last; g0 += WAVES * UN) {
+                    float m1[UN], l1[UN];
+                    f32x4 o1[UN];
+#pragma unroll
+                    for (int i = 0; i < UN; ++i) {
+                        const int g = g0 + i * WAVES;
+                        // an empty piece: the next one begins where it does
+                        const bool there = g <= last && !(g < last && g >= w && begin[g + 1].w == begin[g].w);
+                        // loaded without a condition (another piece's), so that all are in flight
+                        const int from = there ? g : w - 1;
+                        const float* part = Partial<BM, D>::at(a.ws, from, from < w);
+                        m1[i] = part[(int64_t)BM * D + row];
+                        l1[i] = part[(int64_t)BM * D + BM + row];
+                        o1[i] = *reinterpret_cast<const f32x4*>(part + 4 * (int64_t)e);
+                        if (!there) {
+                            m1[i] = -__builtin_inff();
+                            l1[i] = 0.0f;
+                            o1[i] = f32x4{0, 0, 0, 0};
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < UN; ++i) add(m1[i], l1[i], o1[i]);
+                }
+            }
             __syncthreads();
             so[q][et] = o;
             sm[q][et] = M;
@@ -362,13 +435,13 @@ __device__ __forceinline__ void join(const PagedAttention& a, int block, int blo
             if (q == 0)
 #pragma unroll
                 for (int i = 1; i < WAVES; ++i) add(sm[i][et], sl[i][et], so[i][et]);
-        }
-        if (q == 0 && ok) {
-            const float inv = l == 0.0f ? 0.0f : (a.v_scale ? a.v_scale[u.y] : 1.0f) / l;
+            if (q == 0 && ok) {
+                const float inv = l == 0.0f ? 0.0f : (a.v_scale ? a.v_scale[u.y] : 1.0f) / l;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : o[i] * inv;
-            if (a.gate) apply_gate(o, gate);
-            store_bf16x4(a.out + tok * a.o_tok + head * a.o_head + d, o);
+                for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : o[i] * inv;
+                if (a.gate) apply_gate(o, gate);
+                store_bf16x4(a.out + tok * a.o_tok + head * a.o_head + d, o);
+            }
         }
     }
     if (any_bad) {
@@ -414,6 +487,7 @@ struct FewOrder {
 // as their registers hold it.
 template <int D>
 struct TileOrder {
+    static constexpr int kNext = 8;  // dimensions between a lane's groups of one row, up to 4 of them
     static __device__ __forceinline__ void place(int e, int& row, int& d) {
         const int lane = e & 63, b = (e >> 6) & 3, dt = (e >> 8) % (D / 32), wave = (e >> 8) / (D / 32);
         row = 32 * wave + (lane & 31);
