@@ -370,18 +370,25 @@ __device__ __forceinline__ void join(const PagedAttention& a, int block, int blo
         }
     } else {
         const int q = wave, et = lane;
+        // A tile's rows from its first to its last part, of all units before the next
+        // part: a decode step has a few of a tile's 16 rows, and the parts of the others,
+        // at the end, are passed over by all alike (61 requests, 12/2 heads of 256: 99 us a
+        // call, 103 with each unit's parts side by side).
         for (int item = block; item < units * PARTS; item += blocks) {
-            const int w = unit[item / PARTS], e = (item % PARTS) * PER + et;
+            const int at_unit = item % units, e0 = item / units * PER, e = e0 + et;
+            const int w = unit[at_unit];
             const i32x4v u = begin[w];
             const int r0 = u.z * BM, off = rows[w].x, nr = rows[w].y;
             int row, d;
+            ORDER::place(e0, row, d);
+            if (row >= nr) continue;  // of the whole workgroup
             ORDER::place(e, row, d);
             const bool ok = row < nr;
             const int flat = r0 + min(row, nr - 1), tok = off + flat / a.G, head = u.y * a.G + flat % a.G;
             u32x2 gate = {0, 0};
             if (a.gate) gate = load_gate4(a.gate + tok * a.g_tok + head * a.g_head + d);
             // the unit's pieces: workgroups w - 1 (slot 1), w, .. last (slot 0)
-            const int last = unit_last[item / PARTS];
+            const int last = unit_last[at_unit];
             if (any_bad) {
                 bool skip = false;
                 for (int g = w - 1; g <= last; ++g) skip |= bad[g] != 0;
