@@ -4,8 +4,9 @@
 // and its own key tiles, which it brings into its own part of LDS by
 // direct-to-LDS DMA, so that the stream needs no barrier between waves and no
 // registers for loads in flight; the waves' sums are joined in LDS when a unit
-// ends.  61 requests, 465 MB of 8-bit keys and values, 12/2 heads of 256: 86 us,
-// 5.4 TB/s; 7 requests with drafts, 205 MB of BF16: 47 us, 4.4 TB/s.
+// ends.  61 requests, 465 MB of 8-bit keys and values, 12/2 heads of 256: 84 us,
+// 5.6 TB/s; 7 requests with drafts, 205 MB of BF16: 46 us, 4.5 TB/s.  539 MB of codes and
+// powers of blocks: 97 us, 5.6 TB/s.
 //
 // Per key tile (KT keys: 16, or 32 of an 8-bit cache), MFMA 16x16x32:
 //   S^T [keys, rows] = K Q^T, so that a lane holds 4 consecutive keys of one

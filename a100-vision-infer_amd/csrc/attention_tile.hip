@@ -37,9 +37,9 @@
 // this tile and V of the last one are no longer read, so the DMAs of the tiles
 // after go out.
 //
-// Heads of 256, 12/2, BF16: a prompt of 3913 tokens (94 GFLOP) 137 us, and 33 us
+// Heads of 256, 12/2, BF16: a prompt of 3913 tokens (94 GFLOP) 138 us, and 26 us
 // for the join, MFMAs busy in 42 % of the cycles; 512 tokens after 6919 (45
-// GFLOP) 68 and 17 us: a launch's 256 pieces each write 256 KB of partial sums.
+// GFLOP) 68 and 16 us: a launch's 256 pieces each write 256 KB of partial sums.
 #include <algorithm>
 
 #include "attention.hpp"
@@ -52,7 +52,7 @@ constexpr int kBM = kTileRows, kBN = 64, kKeys = 16;  // kKeys: keys of a tile t
 // A unit's start and end, in keys (heads of 256: up to 30 us at 64 keys in 4 us).
 // With 192, 320, 448 and 640 at 256 a prompt of 3913 tokens takes 217, 173, 164
 // and 167 us, a chunk of 512 77, 78, 78 and 79, a mixed batch (heads of 128)
-// 170, 160, 153 and 150.
+// 170, 160, 153 and 150 (each with a join of prompts that took 7 us more).
 template <int D>
 constexpr int kTileStart = 448 * D / 256;
 constexpr int kTileMinTiles = 4;
@@ -285,7 +285,8 @@ __global__ __launch_bounds__(64 * kBM / (32 * RB), 2 / RB) void tile_kernel(Page
             // How far a maximum that moves goes past the score that moved it.  A cache of
             // blocks has keys of many sizes, so the largest scores keep growing for a while, and
             // each move costs all of O a round through the vector registers: 179 us
-            // for a prompt of 3913 tokens without a margin, 165 with 12 or 16, 171 with 4.  The
+            // for a prompt of 3913 tokens without a margin, 165 with 12 or 16, 171 with 4 (with 12 it is 159
+            // since the join is faster).  The
             // weights are that much smaller, which loses nothing while their products with the
             // values stay above 2^-126: not where the values are next to nothing.
             auto margin = [&] { return BLOCKS && fminf(vp[0], vp[1]) > 0x1p-90f ? 12.0f : 0.0f; };
@@ -638,7 +639,7 @@ size_t paged_attention_ws_bytes(int D, int64_t max_rows) {
 // rows 61 and 65, 66 rows 89 and 67).  Where some request may have more than
 // kFewRows rows, a batch is computed in two: a request of a few rows in a
 // 256-row tile streams its keys at the pace of one wave's steps (13 requests,
-// three of them chunks of 400 to 700 tokens, 32/8 heads of 128: 153 us in two
+// three of them chunks of 400 to 700 tokens, 32/8 heads of 128: 151 us in two
 // against 165).  One launch joins both kernels' partial sums: two cost 6 us more.
 hipError_t launch_paged_attention(PagedAttention a, int D, CacheKind kind, int64_t max_rows, hipStream_t stream) {
     a.rows_from = 0;
