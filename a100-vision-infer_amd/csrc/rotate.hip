@@ -178,7 +178,7 @@ __device__ __forceinline__ Place place_of(const Rotation& r, int64_t t) {
     return Place{t, r.steps ? (uint64_t)r.positions[t] : 0};
 }
 // A token's turns in LDS: its cosines and sines times the magnitude, and of 8
-// pairs that the rotated ones end in (1, 0) for the rest.
+// pairs that the rotated ones end in (1, 0) for the rest, which nothing takes.
 __host__ __device__ __forceinline__ int turns_of(int half) { return (half + kPairs - 1) & ~(kPairs - 1); }
 // By `lanes` lanes of a wave (lane l of them): each computes every lanes-th, as one is
 // some 40 instructions and every lane of the heads needs 8.  The lanes of a wave
@@ -200,17 +200,20 @@ __device__ __forceinline__ void fill_turns(const Rotation& r, const uint64_t* st
     }
     __builtin_amdgcn_wave_barrier();
 }
-// The lane's pairs, turned; those behind the rotated ones stay.
+// The lane's pairs, turned; those behind the rotated ones stay as they are: chosen,
+// not multiplied by (1, 0), as 0 times an infinity is NaN.  In kHalves no lane has both.
+template <int LAYOUT>
 __device__ __forceinline__ void rotate_pairs(const Rotation& r, const f32x2* turns, int j0, float (&a)[kPairs], float (&b)[kPairs]) {
     if (!r.steps || j0 >= r.half) return;
+    const int turned = LAYOUT == kHalves ? kPairs : r.half - j0;
 #pragma unroll
     for (int i = 0; i < kPairs; i += 2) {
         const f32x4 t = *reinterpret_cast<const f32x4*>(turns + j0 + i);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const float x = a[i + k], y = b[i + k], c = t[2 * k], z = t[2 * k + 1];
-            a[i + k] = x * c - y * z;
-            b[i + k] = y * c + x * z;
+            a[i + k] = i + k < turned ? x * c - y * z : x;
+            b[i + k] = i + k < turned ? y * c + x * z : y;
         }
     }
 }
@@ -290,7 +293,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(Rotate a, int lane_bit
         if (!live || h >= a.x.n) break;
         float u[kPairs], v[kPairs];
         unpack<LAYOUT>(p[i], u, v);
-        rotate_pairs(a.r, turns, at.j0, u, v);
+        rotate_pairs<LAYOUT>(a.r, turns, at.j0, u, v);
         store_bf16<LAYOUT>(y + h * a.y_head, at, half, D, nb, u, v);
     }
 }
@@ -356,7 +359,7 @@ __device__ __forceinline__ void append_rows(const RotateAppend& a, int lane_bits
             norm_pairs(x, y, wx, wy, lanes, D, a.eps, normed);
         }
         if (!live || row >= rows) continue;
-        if (!is_v) rotate_pairs(a.r, turns, at.j0, x, y);
+        if (!is_v) rotate_pairs<LAYOUT>(a.r, turns, at.j0, x, y);
         if (is_q) {
             store_bf16<LAYOUT>(a.y + t * a.y_tok + h * a.y_head, at, half, D, nb, x, y);
             continue;
@@ -564,7 +567,7 @@ __device__ __forceinline__ void append_run(const RotateAppend& a, RunLds& lds, i
                         const int64_t t = min(t0 + i, a.T - 1);
                         fill_turns(a.r, lds.steps(), Place{t, i0 + i < kThreads ? lds.positions[i0 + i] : (uint64_t)a.r.positions[t]}, row, l, lanes);
                     }
-                    rotate_pairs(a.r, row, at.j0, x, y);
+                    rotate_pairs<LAYOUT>(a.r, row, at.j0, x, y);
                 }
             }
             if (pass == kLargest) {
