@@ -6,7 +6,9 @@ angles, BF16 between the products.  Here pairs are halves or neighbours, the
 angle is exact at any position, and the result is rounded once.
 """
 import ctypes
+import math
 from collections import namedtuple
+from collections.abc import Mapping
 
 import torch
 
@@ -18,47 +20,119 @@ RotaryPlan.__doc__ = """What rotates heads: steps int64 [rotary / 2] on the devi
 rotary_plan makes them), magnitude of the cosines and sines, and whether pairs are neighbours (2j, 2j + 1) or halves (j, j + rotary / 2)."""
 
 _SCALINGS = {"default": 0, "linear": 1, "ntk": 2, "yarn": 3, "wavelength": 4}
+# A config's keys that a plan of any kind reads, and those that its kind reads beside them.
+_KEYS = {"rope_type", "type", "attention_factor", "original_max_position_embeddings", "rope_theta", "partial_rotary_factor", "mrope_section",
+         "mrope_interleaved"}
+_KEYS_OF = {"default": set(), "linear": {"factor"}, "ntk": {"factor"},
+            "yarn": {"factor", "beta_slow", "beta_fast", "mscale", "mscale_all_dim", "truncate"},
+            "wavelength": {"factor", "low_freq_factor", "high_freq_factor"}}
 
 
-def rotary_plan(rotary, theta=10000.0, scaling=None, neighbours=False, sections=None, frequencies=None, magnitude=None, device="cuda"):
+def _read_scaling(scaling):
+    """(kind, the dict without its null values): every key is one that the kind reads."""
+    if not isinstance(scaling, Mapping):
+        _fail(ERR_ARGUMENT, "A rotary scaling is a dict")
+    scaling = {key: value for key, value in scaling.items() if value is not None}
+    kinds = [scaling[key] for key in ("rope_type", "type") if key in scaling] or ["default"]
+    kind = kinds[0]
+    if not isinstance(kind, str) or kind not in _SCALINGS or kinds[-1] != kind:
+        _fail(ERR_ARGUMENT, f"Unknown rotary scaling {' and '.join(map(repr, kinds))}: one of {', '.join(_SCALINGS)}")
+    unread = [str(key) for key in scaling if key not in _KEYS and key not in _KEYS_OF[kind]]
+    if unread:
+        _fail(ERR_ARGUMENT, f"A rotary scaling {kind!r} does not read {', '.join(unread)} (frequencies= and magnitude= take any form)")
+    if not scaling.get("truncate", True):
+        _fail(ERR_ARGUMENT, "A rotary scaling 'yarn' rounds its borders to whole pairs: truncate must be true (frequencies= takes any form)")
+    if kind != "default" and "factor" not in scaling:
+        _fail(ERR_ARGUMENT, f"A rotary scaling {kind!r} needs a factor")
+    if ("mscale" in scaling) != ("mscale_all_dim" in scaling) or ("mscale" in scaling and "attention_factor" in scaling):
+        _fail(ERR_ARGUMENT, "A rotary scaling's magnitude is its attention_factor, or mscale and mscale_all_dim")
+    return kind, scaling
+
+
+def _number(scaling, key, default=None, positive=False):
+    try:
+        value = float(scaling.get(key, default))
+    except (TypeError, ValueError):
+        value = math.nan
+    if math.isnan(value) or (positive and not 0 < value < math.inf):
+        _fail(ERR_ARGUMENT, f"A rotary scaling's {key} must be a {'positive ' if positive else ''}number")
+    return value
+
+
+def _sections_of(scaling, sections):
+    """The sections: the argument's, or the dict's, which have to be the same."""
+    lists = [s for s in (sections, scaling.get("mrope_section")) if s is not None]
+    try:
+        lists = [[int(n) for n in s] for s in lists]
+    except (TypeError, ValueError):
+        lists = [[]]
+    if any(len(s) != 3 or s != lists[0] for s in lists):
+        _fail(ERR_ARGUMENT, "Sections are of three axes, and the config's are those given")
+    if not scaling.get("mrope_interleaved", sections is not None or not lists):
+        _fail(ERR_ARGUMENT, "Sections are interleaved: mrope_interleaved must be true, or the sections given")
+    return lists[0] if lists else None
+
+
+def rotary_plan(rotary, theta=None, scaling=None, neighbours=False, sections=None, frequencies=None, magnitude=None, device="cuda", head_dim=None):
     """A RotaryPlan of the first `rotary` dimensions of a head, with frequencies
-    theta^(-2j / rotary) scaled by `scaling` (a model config's dict: rope_type
-    "default", "linear", "ntk", "yarn" or "wavelength", factor,
-    original_max_position_embeddings, and the turns between which "yarn"
-    (beta_slow, beta_fast) and "wavelength" (low_freq_factor, high_freq_factor)
-    blend; attention_factor sets the magnitude: fp8lin_rotary_frequencies has
-    the formulas), or with the given `frequencies` (rotary / 2 numbers, radians
-    per position).  sections: the config's mrope_section of three axes (pair j
-    takes axis 1 where j % 3 == 1 and j < 3 sections[1], axis 2 where j % 3 == 2
-    and j < 3 sections[2], else axis 0)."""
+    theta^(-2j / rotary) (theta: by default the config's rope_theta, or 10000)
+    scaled by `scaling`, a model config's dict, or with the given `frequencies`
+    (rotary / 2 numbers, radians per position).  fp8lin_rotary_frequencies has
+    the formulas.  The dict's keys, null ones being those that are not there:
+    - rope_type (or type) "default", "linear", "ntk", "yarn" or "wavelength",
+      and for all but the first its factor;
+    - original_max_position_embeddings, and the turns between which "yarn"
+      (beta_slow, beta_fast) and "wavelength" (low_freq_factor,
+      high_freq_factor) blend;
+    - the magnitude of a plan, unless `magnitude` is given: attention_factor, or
+      of "yarn" mscale and mscale_all_dim together, the ratio of the two
+      magnitudes 0.1 mscale ln(factor) + 1;
+    - rope_theta and mrope_section, which may not differ from the arguments, and
+      partial_rotary_factor: with head_dim given, rotary has to be that part of
+      it (without, that is the caller's to see to);
+    - what has one form here: truncate true, mrope_interleaved true (needed
+      where the dict has sections and the call none).
+    Any other key is refused, as it may change the formula.
+    sections: the config's mrope_section of three axes (pair j takes axis 1
+    where j % 3 == 1 and j < 3 sections[1], axis 2 where j % 3 == 2 and j < 3
+    sections[2], else axis 0)."""
     rotary = int(rotary)
     if rotary <= 0 or rotary % 2:
         _fail(ERR_SHAPE, "A rotary plan needs an even, positive number of dimensions")
     half = rotary // 2
     freq, mag = (ctypes.c_double * half)(), ctypes.c_double(1.0)
+    if frequencies is not None and scaling is not None:
+        _fail(ERR_ARGUMENT, "A rotary plan takes rotary / 2 frequencies, or a scaling")
+    kind, scaling = _read_scaling({} if scaling is None else scaling)
+    sections = _sections_of(scaling, sections)
+    part = _number(scaling, "partial_rotary_factor", 1.0, positive=True)
+    if part > 1 or (head_dim is not None and (rotary > head_dim or ("partial_rotary_factor" in scaling and rotary != int(head_dim * part)))):
+        _fail(ERR_SHAPE, "A rotary plan's dimensions are not the config's partial_rotary_factor of the head's")
     if frequencies is not None:
         values = [float(f) for f in frequencies]
-        if len(values) != half or scaling is not None:
+        if len(values) != half:
             _fail(ERR_ARGUMENT, "A rotary plan takes rotary / 2 frequencies, or a scaling")
         freq[:] = values
     else:
-        scaling = scaling or {}
-        kind = scaling.get("rope_type", scaling.get("type", "default"))
-        if kind not in _SCALINGS:
-            _fail(ERR_ARGUMENT, f"Unknown rotary scaling {kind!r}: one of {', '.join(_SCALINGS)}")
-        low, high = [scaling.get(n) or 0.0 for n in (("low_freq_factor", "high_freq_factor") if kind == "wavelength" else ("beta_slow", "beta_fast"))]
-        check(lib().fp8lin_rotary_frequencies(rotary, float(theta), _SCALINGS[kind], float(scaling.get("factor", 1.0)),
-                                              float(scaling.get("original_max_position_embeddings", 0.0)), float(low), float(high), freq,
-                                              ctypes.byref(mag)))
-        if scaling.get("attention_factor") is not None:
-            mag.value = float(scaling["attention_factor"])
+        base = _number(scaling, "rope_theta", 10000.0 if theta is None else theta, positive=True)
+        if theta is not None and float(theta) != base:
+            _fail(ERR_ARGUMENT, "A rotary plan's theta is not the config's rope_theta")
+        low, high = ("low_freq_factor", "high_freq_factor") if kind == "wavelength" else ("beta_slow", "beta_fast")
+        # 0: the usual border, which a dict cannot ask for
+        low, high = [_number(scaling, key, positive=True) if key in scaling else 0.0 for key in (low, high)]
+        factor = _number(scaling, "factor", 1.0)
+        check(lib().fp8lin_rotary_frequencies(rotary, base, _SCALINGS[kind], factor, _number(scaling, "original_max_position_embeddings", 0.0), low, high,
+                                              freq, ctypes.byref(mag)))
+        if "attention_factor" in scaling:
+            mag.value = _number(scaling, "attention_factor")
+        elif "mscale" in scaling:
+            of, all_dim = [0.1 * _number(scaling, key, positive=True) * math.log(max(factor, 1.0)) + 1 for key in ("mscale", "mscale_all_dim")]
+            mag.value = of / all_dim
     if magnitude is not None:
         mag.value = float(magnitude)
     axes = None
     if sections is not None:
-        if len(sections) != 3:
-            _fail(ERR_ARGUMENT, "Sections are of three axes")
-        axes = (ctypes.c_int32 * half)(*[j % 3 if j % 3 and j < 3 * int(sections[j % 3]) else 0 for j in range(half)])
+        axes = (ctypes.c_int32 * half)(*[j % 3 if j % 3 and j < 3 * sections[j % 3] else 0 for j in range(half)])
     steps = torch.empty(half, dtype=torch.int64)
     check(lib().fp8lin_rotary_steps(freq, axes, half, ctypes.c_void_p(steps.data_ptr())))
     return RotaryPlan(steps.to(device), mag.value, bool(neighbours))
