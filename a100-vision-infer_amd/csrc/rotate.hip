@@ -8,7 +8,8 @@
 // position in units of 2^-64, so that position * step modulo 2^64 is the angle
 // modulo a turn, exactly, however far the position: an FP32 product of a
 // position of 10^6 and a frequency is off by 0.06 rad.  The axis of a pair's
-// position (0..3) stands in the step's two lowest bits, 2^-62 turns.
+// position (0..3) stands in the step's two lowest bits; they and the rounding to
+// 2^-62 put the step up to 1.25 * 2^-62 turns a position off its frequency.
 //
 // A lane holds 8 pairs of a head, so D / 16 lanes hold a head, whatever the
 // pairing: a head's sum of squares is a butterfly over them, its rotation stays
@@ -37,7 +38,9 @@ dim3 grid_of(int64_t groups) {
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;  // gfx950 takes unaligned global accesses
 
 // cos and sin of 2 pi phase / 2^64: the nearest quarter turn, then the series
-// of the rest, |r| <= pi / 4, to r^8 and r^9 (next terms 2.5e-8 and 2e-9).
+// of the rest, |r| <= pi / 4, to r^8 and r^9 (next terms 2.5e-8 and 2e-9).  r is off
+// by up to 2^-26 turns: the phase's upper 32 bits (2^-32), their FP32 (2^-28), the
+// constant's rounding (2^-28) and the product's (2^-27.6).
 __device__ __forceinline__ void cos_sin(uint64_t phase, float& c, float& s) {
     const uint32_t turn = (uint32_t)(phase >> 32), quarter = (turn + 0x20000000u) >> 30;
     const float r = (float)(int32_t)(turn - (quarter << 30)) * (float)(6.283185307179586 / 4294967296.0), z = r * r;

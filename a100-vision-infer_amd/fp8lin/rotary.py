@@ -2,8 +2,9 @@
 the rotation of heads by them (include/fp8lin.h describes the operators).
 
 `fused_rope` and `qk_norm_rope` are the reference's form: half layout, FP32
-angles, BF16 between the products.  Here pairs are halves or neighbours, the
-angle is exact at any position, and the result is rounded once.
+angles, BF16 between the products.  Here pairs are halves or neighbours, a
+position times a plan's step is exact modulo a turn (a step is its frequency in
+units of 2^-62 turns a position), and the result is rounded once.
 """
 import ctypes
 import math

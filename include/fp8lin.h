@@ -658,9 +658,14 @@ int fp8lin_verify_drafts(const void* logits, int logits_f32, int64_t logits_ld, 
  * x_2j+1) with `neighbours`, else (x_j, x_j+rotary/2), at position p:
  *   x_a' = magnitude (x_a cos a - x_b sin a),  x_b' = magnitude (x_b cos a + x_a sin a),
  *   a = p frequency_j (radians);
- * the dimensions behind stay.  FP32 with one rounding of the result, the angle
- * exact modulo a turn to 2^-33 turns at any 64-bit position (fp8lin_rope and
- * fp8lin_qk_norm_rope are the reference's form: FP32 angles, BF16 in between).
+ * the dimensions behind stay.  FP32 with one rounding of the result (fp8lin_rope
+ * and fp8lin_qk_norm_rope are the reference's form: FP32 angles, BF16 in between).
+ * p * steps[j] is taken modulo a turn in whole numbers, exactly at any 64-bit
+ * position, and its cosine and sine of an angle that is off by up to 2^-26 turns.
+ * The steps themselves are off their frequencies, by so many turns per position:
+ * up to 1.25 * 2^-62 (their unit and the axis in it) and 2^-52 |frequency_j| /
+ * (2 pi) (the quotient in 64-bit floating point; 2^-54 more below 0).  A position
+ * multiplies that: a frequency of 1 is within 2^-30 turns at 2^24, 2^-14 at 2^40.
  *
  * steps[j] holds frequency_j as the part of a turn per position in units of
  * 2^-64, modulo a turn, and in its two lowest bits the axis whose position the
