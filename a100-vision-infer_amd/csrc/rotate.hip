@@ -440,8 +440,8 @@ __device__ __forceinline__ void written_slots(SLOT slot_at, int64_t n, int block
 }
 // The codes of a block's other slots times f, by `team` lanes, 16 a lane and 4 of
 // those in flight.  The blocks of a decode step's requests grow now and then, so
-// most steps have some (61 requests, blocks of 64, 2 heads of 256: 7.5 us, and 13
-// where every block grows; by the lanes of the row alone 200).
+// most steps have some (61 requests, blocks of 64, 2 heads of 256, a call in a graph:
+// 7.6 us, and 13 where every block grows; by the lanes of the row alone 200).
 __device__ __forceinline__ void grow_block(uint8_t* codes, int64_t slot_stride, int block, int D, float f, const uint32_t (&written)[4], int tid,
                                            int team) {
     constexpr int UN = 4;
